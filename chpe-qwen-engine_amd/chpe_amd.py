@@ -30,7 +30,9 @@ ENGINE_SYMBOLS = [
     "chpe_generate", "chpe_verify", "chpe_prefill", "chpe_block_ready", "chpe_last_error", "chpe_build_id", "chpe_get_max_seq_len", "chpe_get_hidden",
     "chpe_time_steps", "chpe_time_stage", "chpe_time_stage_live", "chpe_stage_bytes", "chpe_step_bytes", "chpe_stage_kernel",
     "chpe_debug_gemv", "chpe_debug_flat_tile_weights", "chpe_debug_gemv_flat", "chpe_debug_gemv_cells", "chpe_debug_gemv_poly", "chpe_debug_gemv_raw", "chpe_debug_embed_row_cell",
-    "chpe_debug_attention", "chpe_debug_attention_block", "chpe_attention_noalloc", "chpe_debug_deltanet_conv", "chpe_debug_deltanet_step",
+    "chpe_debug_attention", "chpe_debug_attention_block", "chpe_attention_noalloc", "chpe_paged_append",
+    "chpe_paged_attention", "chpe_paged_attention_workspace", "chpe_paged_evict", "chpe_paged_evict_workspace",
+    "chpe_debug_deltanet_conv", "chpe_debug_deltanet_step",
 ]
 
 _c_float_p = ctypes.POINTER(ctypes.c_float)
@@ -38,6 +40,13 @@ _c_u32_p = ctypes.POINTER(ctypes.c_uint32)
 _c_u8_p = ctypes.POINTER(ctypes.c_uint8)
 _engine_lib = None
 _pack_lib = None
+
+
+class _KvPages(ctypes.Structure):  # chpe_kv_pages
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int),
+                *[(n, ctypes.c_uint32) for n in ("kv_heads", "head_dim", "page_size", "n_pages")],
+                *[(n, ctypes.c_uint64) for n in ("page_stride", "head_stride", "slot_stride")],
+                ("table", ctypes.c_void_p), *[(n, ctypes.c_uint32) for n in ("rows", "pages_per_row", "table_stride")]]
 
 
 def _fp(a):
@@ -72,6 +81,7 @@ def load_engine_lib():
                           f"run `make -C {PKG_DIR}`")
         V, S, I, U64, F, D = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint64,
                               ctypes.c_float, ctypes.c_double)
+        U32, P = ctypes.c_uint32, ctypes.POINTER(_KvPages)
         sig = {
             "chpe_init": (V, [ctypes.c_char_p]),
             "chpe_forward_tokens": (I, [V, _c_u32_p, S, _c_float_p]),
@@ -118,6 +128,12 @@ def load_engine_lib():
                                                ctypes.c_uint32, _c_float_p, _c_float_p, _c_float_p, _c_float_p]),
             "chpe_attention_noalloc": (I, [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, I, ctypes.c_uint32,
                                            ctypes.c_uint32, V, V, V, V, V]),
+            "chpe_paged_append": (I, [P, U32, U32, V, U64, U64, V, U64, V, U64, V, V, F, V, V, U32, U32, I, V, V, V, V, V,
+                                      V, U64, V]),
+            "chpe_paged_attention": (I, [P, U32, V, U32, V, U64, F, U32, V, U64, V, V, U64, V, S, V]),
+            "chpe_paged_attention_workspace": (S, [P, U32, U32, I]),
+            "chpe_paged_evict": (I, [P, V, U32, U32, U32, U32, V, V, U64, V, V, V, V, V, S, V]),
+            "chpe_paged_evict_workspace": (S, [P, U32]),
             "chpe_debug_deltanet_conv": (I, [ctypes.c_uint32, ctypes.c_uint32, _c_float_p, _c_float_p, _c_float_p,
                                              _c_float_p]),
             "chpe_debug_deltanet_step": (I, [ctypes.c_uint32] * 3 + [_c_float_p] * 9 + [F, _c_float_p, _c_float_p]),
@@ -350,6 +366,163 @@ class Engine:
             return out.stdout.strip() or name
         except (OSError, subprocess.SubprocessError):
             return name
+
+
+class KvPages:
+    """A paged key/value cache in torch tensors and its operators (chpe_paged_*, include/chpe.h): k, v
+    [n_pages, kv_heads, page_size, head_dim] (f32, fp16 or bf16; any strides but the last dimension's, the
+    same for both), table [rows, pages_per_row] int32.  The tensors stay the caller's: the table's and the
+    pages' contents may change between calls.  Calls enqueue on torch's current stream of the tensors'
+    device."""
+
+    def __init__(self, k, v, table):
+        import torch
+        self._torch, self.lib = torch, load_engine_lib()
+        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        if k.dim() != 4 or k.shape != v.shape or k.dtype not in types or v.dtype != k.dtype:
+            raise ValueError("k and v: [n_pages, kv_heads, page_size, head_dim], both f32, fp16 or bf16")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("k and v: the same strides, the last dimension's 1")
+        if table.dim() != 2 or table.dtype != torch.int32 or (table.numel() and table.stride(1) != 1):
+            raise ValueError("table: [rows, pages_per_row] int32, the last stride 1")
+        if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError("table: rows that do not lie in each other")
+        if not k.is_cuda or v.device != k.device or table.device != k.device:
+            raise ValueError("k, v and table: on one GPU")
+        self.k, self.v, self.table, self.device = k, v, table, k.device
+        self.rows, self.kv_heads, self.page_size, self.head_dim = table.shape[0], k.shape[1], k.shape[2], k.shape[3]
+        self.capacity = table.shape[1] * self.page_size
+        self._c = _KvPages(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[1], k.shape[3], k.shape[2], k.shape[0],
+                           k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), table.shape[0], table.shape[1],
+                           table.stride(0) if table.shape[0] > 1 else table.shape[1])
+
+    def _call(self, name, *args):
+        t = self._torch
+        if t.cuda.current_device() != self.device.index:
+            with t.cuda.device(self.device):
+                return self._call(name, *args)
+        rc = getattr(self.lib, name)(self._c, *args, t.cuda.current_stream(self.device).cuda_stream)
+        if rc:
+            raise EngineError(f"{name} failed: {rc}")
+
+    def _take(self, t, name, dtype, shape):
+        """The address of a contiguous tensor of this type and shape on the cache's device."""
+        if t.dtype != dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}")
+        return t.data_ptr()
+
+    def _slots(self, t, name, dtype, least):
+        """The address of a contiguous [rows, kv_heads, n >= least] tensor."""
+        if t.dim() != 3 or t.shape[2] < least:
+            raise ValueError(f"{name}: [rows, kv_heads, at least {least}]")
+        return self._take(t, name, dtype, (self.rows, self.kv_heads, t.shape[2]))
+
+    def append(self, k, v, rows, slots, positions, q=None, q_norm=None, k_norm=None, eps=1e-6, rope=None,
+               interleaved=False, q_out=None, slot_pos=None, slot_weight=None):
+        """chpe_paged_append: k, v [tokens, kv_heads, head_dim] f32 at slot slots[t] of row rows[t], rotated by
+        positions[t] (int32); rope = (cos, sin), each [n, rot_dim / 2].  q [tokens, heads, head_dim] f32 (its
+        first two strides free) gives the rotated queries, which are returned (q_out, or a new tensor)."""
+        f32, i32, t = self._torch.float32, self._torch.int32, k.shape[0]
+        for x, name in ((k, "k"), (v, "v")):
+            if x.dtype != f32 or x.shape != (t, self.kv_heads, self.head_dim) or x.device != self.device:
+                raise ValueError(f"{name}: [tokens, {self.kv_heads}, {self.head_dim}] f32 on {self.device}")
+            if t and (x.stride(2) != 1 or (self.kv_heads > 1 and x.stride(1) != self.head_dim)):
+                raise ValueError(f"{name}: contiguous within a token")
+        width = self.kv_heads * self.head_dim
+        heads = qs = qh = qp = qo = 0
+        if q is not None:
+            if q.dim() != 3 or q.dtype != f32 or q.shape[0] != t or q.shape[2] != self.head_dim or q.device != self.device:
+                raise ValueError(f"q: [tokens, heads, {self.head_dim}] f32 on {self.device}")
+            if q.numel() and q.stride(2) != 1:
+                raise ValueError("q: the last stride 1")
+            heads, qp = q.shape[1], q.data_ptr()
+            qh = q.stride(1) if heads > 1 else self.head_dim
+            qs = q.stride(0) if t > 1 else heads * qh
+            if q_out is None:
+                q_out = self._torch.empty(q.shape, dtype=f32, device=self.device)
+            qo = self._take(q_out, "q_out", f32, q.shape)
+        gains = [None if g is None else self._take(g, "a norm's gains", f32, (self.head_dim,)) for g in (q_norm, k_norm)]
+        cos = sin = None
+        n = half = 0
+        if rope is not None:
+            n, half = rope[0].shape
+            cos, sin = (self._take(x, "rope", f32, (n, half)) for x in rope)
+        idx = [self._take(x, "rows, slots, positions", i32, (t,)) for x in (rows, slots, positions)]
+        track, sp, sw = 0, None, None
+        if slot_pos is not None:
+            sp, track = self._slots(slot_pos, "slot_pos", i32, 1), slot_pos.shape[2]
+        if slot_weight is not None:
+            sw = self._slots(slot_weight, "slot_weight", f32, 1)
+            if track and slot_weight.shape[2] != track:
+                raise ValueError("slot_pos and slot_weight: the same shape")
+            track = slot_weight.shape[2]
+        self._call("chpe_paged_append", t, heads, qp, qs, qh, k.data_ptr(), k.stride(0) if t > 1 else width,
+                   v.data_ptr(), v.stride(0) if t > 1 else width, *gains, eps, cos, sin, 2 * half, n, int(interleaved),
+                   *idx, qo, sp, sw, track)
+        return q_out
+
+    def attention_workspace(self, heads, max_len, weights=False):
+        """Bytes that attention() needs for these sizes."""
+        n = self.lib.chpe_paged_attention_workspace(self._c, heads, max_len, int(weights))
+        if n == 0 and self.rows:
+            raise ValueError("chpe_paged_attention_workspace rejected the arguments")
+        return n
+
+    def attention(self, q, lens, max_len, scale=None, window=0, out=None, weight_in=None, weight_out=None,
+                  workspace=None):
+        """chpe_paged_attention: q [rows, heads, head_dim] f32 over the first lens[r] <= max_len slots of row r.
+        weight_out [rows, kv_heads, >= max_len] receives weight_in (or 0) plus what each slot was given."""
+        f32 = self._torch.float32
+        if q.dim() != 3:
+            raise ValueError("q: [rows, heads, head_dim]")
+        heads, width = q.shape[1], q.shape[1] * self.head_dim
+        qp = self._take(q, "q", f32, (self.rows, heads, self.head_dim))
+        if out is None:
+            out = self._torch.empty(q.shape, dtype=f32, device=self.device)
+        op = self._take(out, "out", f32, q.shape)
+        wi = wo = None
+        stride = 0
+        if weight_out is not None:
+            wo, stride = self._slots(weight_out, "weight_out", f32, max_len), weight_out.shape[2]
+        if weight_in is not None:
+            if weight_out is None:
+                raise ValueError("weight_in without weight_out")
+            wi = self._take(weight_in, "weight_in", f32, weight_out.shape)
+        if workspace is None:
+            workspace = self._torch.empty(self.attention_workspace(heads, max_len, wo is not None),
+                                          dtype=self._torch.uint8, device=self.device)
+        lp = self._take(lens, "lens", self._torch.int32, (self.rows,))
+        ws = self._take(workspace, "workspace", self._torch.uint8, (workspace.numel(),))
+        self._call("chpe_paged_attention", heads, lp, max_len, qp, width,
+                   1.0 / self.head_dim ** 0.5 if scale is None else scale, window, op, width, wi, wo, stride, ws,
+                   workspace.numel())
+        return out
+
+    def evict_workspace(self, max_len):
+        """Bytes that evict() needs."""
+        n = self.lib.chpe_paged_evict_workspace(self._c, max_len)
+        if n == 0 and self.rows:
+            raise ValueError("chpe_paged_evict_workspace rejected the arguments")
+        return n
+
+    def evict(self, lens, max_len, budget, slot_weight, slot_pos, recent=0, sinks=0, lens_out=None, weight_out=None,
+              pos_out=None, slot_src=None, workspace=None):
+        """chpe_paged_evict: every row and kv head down to `budget` slots.  lens_out, weight_out and pos_out
+        default to the inputs themselves; returns lens_out."""
+        f32, i32 = self._torch.float32, self._torch.int32
+        lens_out, weight_out, pos_out = (i if o is None else o for o, i in
+                                         ((lens_out, lens), (weight_out, slot_weight), (pos_out, slot_pos)))
+        w = self._slots(slot_weight, "slot_weight", f32, max_len)
+        shape = slot_weight.shape
+        args = [self._take(slot_pos, "slot_pos", i32, shape), shape[2], self._take(lens_out, "lens_out", i32, (self.rows,)),
+                self._take(weight_out, "weight_out", f32, shape), self._take(pos_out, "pos_out", i32, shape),
+                None if slot_src is None else self._take(slot_src, "slot_src", i32, shape)]
+        if workspace is None:
+            workspace = self._torch.empty(self.evict_workspace(max_len), dtype=self._torch.uint8, device=self.device)
+        ws = self._take(workspace, "workspace", self._torch.uint8, (workspace.numel(),))
+        self._call("chpe_paged_evict", self._take(lens, "lens", i32, (self.rows,)), max_len, budget, recent, sinks, w,
+                   *args, ws, workspace.numel())
+        return lens_out
 
 
 def gpu_flat_tile_weights(cell):

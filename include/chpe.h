@@ -207,6 +207,88 @@ int chpe_debug_attention_block(uint32_t head_dim, uint32_t heads, uint32_t kv_he
 int chpe_attention_noalloc(uint32_t head_dim, uint32_t heads, uint32_t kv_heads, int kv_f16, uint32_t pos,
                            uint32_t max_seq, const float *q, const void *k_cache, const void *v_cache,
                            float *out, void *stream);
+/* ---- the paged key/value cache (no counterpart in the reference, whose KVCache is one f32 block per
+ * layer, src/chpe_engine.zig:755-801) ----
+ * For serving loops with many sequences: what writes the cache, what reads it and what shrinks it, on
+ * caller device buffers.  The calls allocate nothing, keep nothing between calls and only enqueue on
+ * `stream` (a hipStream_t of the current device; null: the default stream), so they can be captured into
+ * a graph.  All pointers but the description's own are device addresses on the current device.
+ *
+ * Keys and values lie in pages of page_size slots (a power of two): the head_dim elements of kv head h at
+ * slot s of page p start at element p * page_stride + h * head_stride + s * slot_stride of k and of v, so
+ * that either of heads and slots may be the inner one.  Slot s of row r (a sequence) is slot
+ * s % page_size of page table[r * table_stride + s / page_size].  type: 0 f32, 1 fp16, 2 bf16; head_dim
+ * 64, 128 or 256; k and v at 16-byte boundaries, strides multiples of 16 bytes, no two rows in each other.
+ * Page ids are checked on the device: an id outside 0 .. n_pages - 1 is never followed. */
+typedef struct chpe_kv_pages {
+  void *k, *v;
+  int type;
+  uint32_t kv_heads, head_dim, page_size, n_pages;
+  uint64_t page_stride, head_stride, slot_stride;   /* elements */
+  const int32_t *table;                             /* [rows][table_stride], device */
+  uint32_t rows, pages_per_row, table_stride;
+} chpe_kv_pages;
+
+/* What a layer does between the q/k/v projections and the attention, for `tokens` tokens of any rows (one
+ * each for a step, whole prompts): queries and keys are RMS-normalised per head (q_norm / k_norm
+ * [head_dim] gains; null: not), rotated by the token's position over the first rot_dim dims (a multiple
+ * of 8; 0: not) with the tables rope_cos / rope_sin [rope_rows][rot_dim / 2] -- pairs (i, i + rot_dim/2),
+ * or (2i, 2i + 1) if interleaved --, keys and values rounded to the cache type and written at slot
+ * token_slot[t] of row token_row[t].  The rotation goes by token_pos[t]: after an eviction the slot is
+ * not the position.  q [tokens] rows of q_stride floats, its heads q_head_stride apart (a model with
+ * output gates has them between the queries); k, v [tokens][kv_heads][head_dim] in rows of k_stride /
+ * v_stride floats; q_out [tokens][heads][head_dim], not overlapping q.  heads 0: no queries.
+ * slot_pos / slot_weight (optional) [rows][kv_heads][track_stride]: receive the position and 0 at the
+ * written slot, if it is below track_stride (chpe_paged_evict's inputs).
+ * Float arrays at 16-byte boundaries, their strides multiples of 4.  A token whose row is not one of the
+ * table's, whose slot is past the row's pages or whose page id is outside the pool is not written (a row
+ * of -1 pads a batch); one whose position is outside the tables is not written and its queries are NaN.
+ * Two tokens of one call at the same slot of the same row: either may stay.
+ * Returns 0, -1 bad arguments, -3 device error. */
+int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t heads, const float *q, uint64_t q_stride,
+                      uint64_t q_head_stride, const float *k, uint64_t k_stride, const float *v, uint64_t v_stride,
+                      const float *q_norm, const float *k_norm, float eps, const float *rope_cos, const float *rope_sin,
+                      uint32_t rot_dim, uint32_t rope_rows, int interleaved, const int32_t *token_row,
+                      const int32_t *token_slot, const int32_t *token_pos, float *q_out, int32_t *slot_pos,
+                      float *slot_weight, uint64_t track_stride, void *stream);
+
+/* The attention of one new token per row: row r's query heads over its slots 0 .. lens[r] - 1 (window > 0:
+ * the last `window` of them), softmax((q . k) * scale) . V, every head over kv head h / (heads / kv_heads).
+ * q and out: `heads` x head_dim floats per row, rows q_stride / out_stride apart.  lens is read on the
+ * device; max_len bounds it (and sizes the launch).  A row of length 0 gives zeros; one of a length
+ * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN, and so may an
+ * infinite value among a head's keys or queries.  What lies in slots outside the range is never used.
+ * weight_out (optional) [rows][kv_heads][weight_stride]: at each slot below the length, weight_in (null:
+ * 0) plus the slot's softmax weights summed over the query heads of its kv head; weight_in may be
+ * weight_out.  Rows may share pages (a common prefix, or one sequence's drafts as rows of growing length).
+ * workspace: chpe_paged_attention_workspace bytes for the same cache, heads and max_len, at a 16-byte boundary, any
+ * content; calls that may overlap need one each.
+ * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
+int chpe_paged_attention(const chpe_kv_pages *cache, uint32_t heads, const int32_t *lens, uint32_t max_len,
+                         const float *q, uint64_t q_stride, float scale, uint32_t window, float *out,
+                         uint64_t out_stride, const float *weight_in, float *weight_out, uint64_t weight_stride,
+                         void *workspace, size_t workspace_bytes, void *stream);
+/* bytes; 0 for arguments that the call refuses */
+size_t chpe_paged_attention_workspace(const chpe_kv_pages *cache, uint32_t heads, uint32_t max_len, int weights);
+
+/* Cuts every row to at most `budget` slots per kv head, each head its own: the slots whose position is
+ * among the newest `recent` ones (above the head's newest minus recent) or below `sinks` stay, then those of the
+ * largest weight (equal: the lower slot; NaN last); recent + sinks <= budget.  Of the kept slots those at
+ * lens_out[r] = min(lens[r], budget) and above move, in ascending order, into the freed slots below it,
+ * in ascending order; no other slot moves.  weight, slot_pos [rows][kv_heads][stride] as
+ * chpe_paged_attention and chpe_paged_append leave them; weight_out, pos_out and slot_src (optional: the
+ * slot that each one held before) of the same layout receive the slots below lens_out[r], the others keep
+ * what they hold.  weight_out may be weight, pos_out slot_pos, lens_out lens; they do not overlap
+ * otherwise.  Rows whose length is outside 0 .. max_len are left as they are.  The pages of a row that is
+ * cut belong to it alone; a move from or to a page id outside the pool is left out.
+ * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
+int chpe_paged_evict(const chpe_kv_pages *cache, const int32_t *lens, uint32_t max_len, uint32_t budget,
+                     uint32_t recent, uint32_t sinks, const float *weight, const int32_t *slot_pos, uint64_t stride,
+                     int32_t *lens_out, float *weight_out, int32_t *pos_out, int32_t *slot_src, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* bytes; 0 for arguments that the call refuses */
+size_t chpe_paged_evict_workspace(const chpe_kv_pages *cache, uint32_t max_len);
+
 /* Gated-DeltaNet (Qwen3.5 linear-attention layers) decode-step kernels on caller data.  The
  * reference has no code for these layers (README claims only); the arithmetic is the gated
  * delta rule as defined by transformers 5.15.0 models/qwen3_5/modeling_qwen3_5.py.
