@@ -1,8 +1,8 @@
 // paged_attention.hip -- chpe_paged_attention: the attention of one new token per row over the paged
 // cache.  s_j = scale q.k_j over the row's slots lo <= j < len, p = softmax(s), out = sum_j p_j v_j, and,
 // for a cache that is kept to a budget, each slot's p summed over the query heads of its kv head.
-// The slots are split over workgroups: each leaves its maximum, sum of exp(s - max) and exp-weighted sum
-// of V rows, and a second launch rescales and joins them (and turns the scores into weights).
+// The slots are split over workgroups: each leaves its maximum, sum of 2^(s - max) and so weighted sum of V
+// rows, and a second launch rescales and joins them (and turns the scores into weights).
 #include <algorithm>
 #include <cmath>
 
@@ -18,11 +18,11 @@ struct PagedAttnArgs {
   const int32_t* lens;
   float* out;
   float *part_ml, *part_acc;      // [row][head][split][2], [row][head][split][hd]
-  float* scores;                  // [row][head][max_len], or null
+  float* scores;                  // [row][head][score_stride] from the range's first slot, or null
   const float* weight_in;
   float* weight_out;
   uint64_t q_stride, out_stride, weight_stride;
-  uint32_t rows, H, max_len, window, splits, chunk;
+  uint32_t rows, H, max_len, window, splits, chunk, score_stride;
   float scale;
 };
 
@@ -34,130 +34,583 @@ __device__ __forceinline__ bool row_range(const PagedAttnArgs& a, uint32_t row, 
   return n <= a.max_len;
 }
 
-// one wave per (row, query head, split): slot after slot, lane l holds dims l, l + 64, ..
-template <int HD, class T>
-__global__ void __launch_bounds__(64) k_paged_partial(PagedAttnArgs a) {
-  constexpr int N = HD / 64;
-  const uint32_t split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, h = item % a.H, row = item / a.H;
-  const int lane = threadIdx.x;
-  uint32_t lo, len;
-  row_range(a, row, &lo, &len);
-  const uint32_t b = lo + split * a.chunk, e = min(len, b + a.chunk);
-  const uint32_t kvh = h / (a.H / a.c.KV);
-  float q[N], acc[N];
+// ---- the partial sums of one split -----------------------------------------------------------------------
+// One workgroup of 4 waves per (row, kv head, group of HT query heads, split); wave w takes the tiles w, w + 4,
+// .. of the split.  A tile's scores are S^T = K . Q^T on the matrix cores (rows: slots, columns: query heads),
+// its output O^T = V^T . P^T (rows: dims, columns: heads): with the heads as columns of both, a lane (G, n) =
+// (lane / 16, lane % 16) keeps the running maximum and sum of column n in scalars of its own, and the result
+// layout of the first product (slots 4 G + i of column n) is the operand layout of the second, so the weights
+// never leave the registers.  The order of the dims inside the first product and of the slots inside the
+// second is free as long as both operands agree, which is what lets every lane load 16 bytes in a row:
+// K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
+// The running maximum is in units of log2 (scores times scale * log2 e).
+constexpr int kWaves = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+// 16-bit elements with f32 queries and weights: x is taken apart into parts that the products hold exactly.
+// fp16: two parts, 22 bits, in columns h and h + 8 of one operand; x is brought near 2^14 by a power of two
+// first, so that the second part does not fall below fp16's range.  bf16: three parts, 24 bits, the third in
+// an operand of its own.  Both columns' results are added at the end: no precision of the f32 queries or
+// weights is lost to the cache's type.
+template <class T>
+struct Parts;
+template <>
+struct Parts<_Float16> {
+  using Vec = h8_t;
+  static constexpr int kOps = 1, kScaleExp = 15;  // (weights <= 1 times 2^15)
+  static __device__ void split(const float (&x)[8], bool second, Vec (&out)[1]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = a.q[row * a.q_stride + h * HD + lane + 64 * i];
-    acc[i] = 0.0f;
+    for (int e = 0; e < 8; ++e) {
+      const _Float16 hi = _Float16(x[e]);
+      out[0][e] = second ? _Float16(x[e] - float(hi)) : hi;
+    }
   }
-  float m = -INFINITY, l = 0.0f;
-  for (uint32_t j = b; j < e; ++j) {
-    uint32_t page;
-    const bool ok = a.c.page_of(row, j, &page);
-    const size_t at = a.c.at(page, kvh, j);
-    float s = 0.0f;
+  static __device__ f4_t mfma(Vec a, Vec b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Parts<Bf16> {
+  using Vec = b8_t;
+  static constexpr int kOps = 2, kScaleExp = 0;
+  static __device__ void split(const float (&x)[8], bool second, Vec (&out)[2]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(q[i], Elem<T>::get(reinterpret_cast<const T*>(a.c.k) + at + lane + 64 * i), s);
-    s = ok ? wave_sum(s) * a.scale : __builtin_nanf("");
-    if (a.scores && lane == 0) a.scores[(size_t(row) * a.H + h) * a.max_len + j] = s;
-    const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
-    const float f = expf(m - base), p = expf(s - base);
-    l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      acc[i] = acc[i] * f + p * Elem<T>::get(reinterpret_cast<const T*>(a.c.v) + at + lane + 64 * i);
-    m = m2;
+    for (int e = 0; e < 8; ++e) {
+      const __bf16 hi = __bf16(x[e]);
+      const float r = x[e] - float(hi);
+      const __bf16 mid = __bf16(r);
+      const __bf16 lo = __bf16(r - float(mid));
+      out[0][e] = second ? mid : hi;
+      out[1][e] = second ? __bf16(0.0f) : lo;
+    }
   }
-  const size_t pt = size_t(item) * a.splits + split;
+  static __device__ f4_t mfma(Vec a, Vec b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// where a workgroup works
+struct Place {
+  uint32_t row, kvh, h0, nh, begin, end, lo, len, split;  // query heads h0 .. h0 + nh - 1, slots begin .. end - 1
+  bool ok;
+};
+template <int HT>
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a) {
+  Place p;
+  const uint32_t gq = a.H / a.c.KV, hz = (gq + HT - 1) / HT;
+  uint32_t b = blockIdx.x;
+  p.split = b % a.splits;
+  b /= a.splits;
+  const uint32_t z = b % hz;
+  b /= hz;
+  p.kvh = b % a.c.KV;
+  p.row = b / a.c.KV;
+  p.h0 = p.kvh * gq + z * HT;
+  p.nh = min(uint32_t(HT), gq - z * HT);
+  p.ok = row_range(a, p.row, &p.lo, &p.len);
+  p.begin = p.lo + p.split * a.chunk;
+  p.end = min(p.len, p.begin + a.chunk);
+  return p;
+}
+
+// The tile's row offsets (bytes from k or v): lane r of the wave finds row r's page and leaves the
+// offset in LDS for the lanes that load the row.  `next` requests the table entry ahead of its use.
+template <int ROWS, int ES>
+struct TileRows {
+  uint64_t (*s)[ROWS];
+  uint32_t id, slot;
+  bool bad = false;
+  __device__ void next(const PagedAttnArgs& a, const Place& p, uint32_t t, int lane) {
+    slot = min(t + uint32_t(lane % ROWS), p.end - 1);
+    id = uint32_t(gld(a.c.table + size_t(p.row) * a.c.table_stride + (slot >> a.c.shift)));
+  }
+  __device__ void put(const PagedAttnArgs& a, const Place& p, int buf, int lane) {
+    const bool in = id < a.c.n_pages;
+    bad |= !in;
+    if (lane < ROWS) s[buf][lane] = a.c.at(in ? id : 0u, p.kvh, slot) * ES;
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// joins waves 1 .. 3 into wave 0: each lane's maximum, sum and N accumulators, through LDS
+template <int N, int LANES>
+__device__ __forceinline__ void join_waves(float* s, int wave, int slot, bool mine, float* m, float* l, f4_t* o) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) a.part_acc[pt * HD + lane + 64 * i] = acc[i];
-  if (lane == 0) {
+  for (int half = kWaves / 2; half >= 1; half /= 2) {
+    __syncthreads();
+    if (wave >= half && wave < 2 * half && mine) {
+      float* d = s + (wave - half) * (N * 4 + 4) * LANES;
+#pragma unroll
+      for (int i = 0; i < N; ++i) *reinterpret_cast<f4_t*>(d + (i * LANES + slot) * 4) = o[i];
+      d[N * 4 * LANES + slot] = *m;
+      d[(N * 4 + 1) * LANES + slot] = *l;
+    }
+    __syncthreads();
+    if (wave < half && mine) {
+      const float* d = s + wave * (N * 4 + 4) * LANES;
+      const float m2 = d[N * 4 * LANES + slot], l2 = d[(N * 4 + 1) * LANES + slot];
+      const float M = fmaxf(*m, m2), base = M == -INFINITY ? 0.0f : M;
+      const float f = __builtin_amdgcn_exp2f(*m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = o[i] * f + *reinterpret_cast<const f4_t*>(d + (i * LANES + slot) * 4) * f2;
+      *l = *l * f + l2 * f2;
+      *m = M;
+    }
+  }
+}
+
+// leaves a column's split for the join, or, where the row has one split at most, the output itself.
+// o[j][i] is dim dim_of(j, i) of the column's head.
+template <int HD, int N, int E>
+__device__ __forceinline__ void leave(const PagedAttnArgs& a, const Place& p, uint32_t head, int G, float m, float l,
+                                      const f4_t* o) {
+  const size_t item = size_t(p.row) * a.H + head, pt = item * a.splits + p.split;
+  float* dst = a.part_acc + pt * HD;
+  float f = 1.0f;
+  if (a.splits == 1) {
+    dst = a.out + p.row * a.out_stride + size_t(head) * HD;
+    f = l == 0.0f ? 0.0f : 1.0f / l;
+  }
+  if (G == 0) {
     a.part_ml[pt * 2] = m;
     a.part_ml[pt * 2 + 1] = l;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < N; j += 4)
+      *reinterpret_cast<float4*>(dst + (j / E) * 16 * E + (4 * G + i) * E + j % E) =
+          make_float4(o[j][i] * f, o[j + 1][i] * f, o[j + 2][i] * f, o[j + 3][i] * f);
 }
 
-// maximum and sum over an item's splits
-__device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, float* M, float* L) {
-  float m = -INFINITY, l = 0.0f;
-  for (uint32_t s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(size_t(item) * a.splits + s) * 2]);
-  const float base = m == -INFINITY ? 0.0f : m;
-  for (uint32_t s = 0; s < a.splits; ++s) {
-    const size_t pt = (size_t(item) * a.splits + s) * 2;
-    l += a.part_ml[pt + 1] * expf(a.part_ml[pt] - base);
+// a split without slots: nothing for the join (it goes by the row's length); the output of a row of one
+// split at most
+template <int HD, int HT>
+__device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& p) {
+  if (a.splits != 1) return;
+  const float v = p.ok ? 0.0f : __builtin_nanf("");
+  for (uint32_t i = threadIdx.x; i < p.nh * HD; i += kWaves * 64) a.out[p.row * a.out_stride + size_t(p.h0) * HD + i] = v;
+}
+
+template <int HD, class T, int NT>
+__global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
+  using P = Parts<T>;
+  using Vec = typename P::Vec;
+  constexpr int HT = 8 * NT, KS = HD / 32, VD = HD / 16, E = VD < 8 ? 4 : 8, VP = VD / E;
+  __shared__ uint64_t s_off[kWaves][2][32];
+  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 32];
+  const Place p = place_of<HT>(a);
+  if (p.begin >= p.end) return leave_none<HD, HT>(a, p);  // (the whole workgroup)
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+  const bool second = n >= 8;
+
+  TileRows<32, 2> rows{s_off[wave]};
+  uint32_t t = p.begin + 32 * wave;
+  uint4 kf[2][KS], vf[8][VP];
+  auto load_k = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* src = a.c.k + rows.s[buf][16 * u + n] + G * 16;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[u][s] = ld_u128(src + 64 * s);
+    }
+  };
+  auto load_v = [&](int buf) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const uint8_t* src = a.c.v + rows.s[buf][(r >> 2) * 16 + 4 * G + (r & 3)] + n * (2 * E);
+#pragma unroll
+      for (int c = 0; c < VP; ++c) {
+        if constexpr (E == 8) {
+          vf[r][c] = ld_u128(src + 256 * c);
+        } else {
+          const uint2 w = ld_u64(src);
+          vf[r][c] = make_uint4(w.x, w.y, 0, 0);
+        }
+      }
+    }
+  };
+  rows.next(a, p, t, lane);
+
+  // the queries of the columns' heads: dims (G + 4 s) * 8 .. + 7 of head n % 8 of each tile of heads
+  Vec qb[NT][KS][P::kOps];
+  float mult[NT], m[NT], l[NT];
+  f4_t o[NT][VD];
+#pragma unroll
+  for (int ht = 0; ht < NT; ++ht) {
+    const uint32_t h = ht * 8 + (n & 7);
+    const float* src = a.q + p.row * a.q_stride + size_t(p.h0 + (h < p.nh ? h : 0)) * HD + G * 8;
+    float x[KS][8], top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const float4 u = ld_f4(src + 32 * s), v = ld_f4(src + 32 * s + 4);
+      const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[s][e] = h < p.nh ? w[e] : 0.0f;
+        top = fmaxf(top, fabsf(x[s][e]));
+      }
+    }
+    mult[ht] = a.scale * kLog2e;
+    if constexpr (P::kScaleExp != 0) {
+      top = pair_max(pair_max(top, 16), 32);
+      int ex = 0;
+      if (top > 0.0f && top < INFINITY) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(x[s][e], ex);
+      mult[ht] = __builtin_amdgcn_ldexpf(mult[ht], -ex);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) P::split(x[s], second, qb[ht][s]);
+    m[ht] = -INFINITY;
+    l[ht] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VD; ++j) o[ht][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  *M = base;
-  *L = l;
+
+  int buf = 0;
+  if (t < p.end) {
+    rows.put(a, p, 0, lane);
+    load_k(0);
+    load_v(0);
+    rows.next(a, p, t + 32 * kWaves, lane);
+  }
+  for (; t < p.end; t += 32 * kWaves) {
+    const bool more = t + 32 * kWaves < p.end;
+    // scores; the K registers are free after them and take the next tile's rows
+    f4_t sc[NT][2];
+#pragma unroll
+    for (int ht = 0; ht < NT; ++ht)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int op = 0; op < P::kOps; ++op) acc = P::mfma(__builtin_bit_cast(Vec, kf[u][s]), qb[ht][s][op], acc);
+        sc[ht][u] = acc;
+      }
+    buf ^= 1;
+    if (more) {
+      rows.put(a, p, buf, lane);
+      load_k(buf);
+      rows.next(a, p, t + 64 * kWaves, lane);
+    }
+    Vec pb[NT][P::kOps];
+#pragma unroll
+    for (int ht = 0; ht < NT; ++ht) {
+      float s8[8], mx = m[ht];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t j = t + (e >> 2) * 16 + 4 * G + (e & 3);
+        const float s = pair_sum(sc[ht][e >> 2][e & 3], 8) * mult[ht];
+        s8[e] = j < p.end ? s : -INFINITY;
+        mx = fmaxf(mx, s8[e]);
+      }
+      if (a.scores && n < 8 && ht * 8 + n < p.nh) {
+        float* d = a.scores + (size_t(p.row) * a.H + p.h0 + ht * 8 + n) * a.score_stride + (t - p.lo) + 4 * G;
+        *reinterpret_cast<float4*>(d) = make_float4(s8[0], s8[1], s8[2], s8[3]);
+        *reinterpret_cast<float4*>(d + 16) = make_float4(s8[4], s8[5], s8[6], s8[7]);
+      }
+      mx = pair_max(pair_max(mx, 16), 32);
+      const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m[ht] - base);
+      if (__ballot(f != 1.0f) != 0) {
+        l[ht] *= f;
+#pragma unroll
+        for (int j = 0; j < VD; ++j) o[ht][j] *= f;
+      }
+      m[ht] = mx;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s8[e] = __builtin_amdgcn_exp2f(s8[e] - base);
+        l[ht] += s8[e];
+        s8[e] *= float(1 << P::kScaleExp);
+      }
+      P::split(s8, second, pb[ht]);
+    }
+#pragma unroll
+    for (int j = 0; j < VD; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint4 x = vf[2 * r][j / E], y = vf[2 * r + 1][j / E];
+        const int wi = (j % E) / 2;
+        const uint32_t lo = wi == 0 ? x.x : wi == 1 ? x.y : wi == 2 ? x.z : x.w;
+        const uint32_t hi = wi == 0 ? y.x : wi == 1 ? y.y : wi == 2 ? y.z : y.w;
+        w[r] = __builtin_amdgcn_perm(hi, lo, (j & 1) ? 0x07060302u : 0x05040100u);
+      }
+      const Vec vv = __builtin_bit_cast(Vec, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int ht = 0; ht < NT; ++ht)
+#pragma unroll
+        for (int op = 0; op < P::kOps; ++op) o[ht][j] = P::mfma(vv, pb[ht][op], o[ht][j]);
+    }
+    if (more) load_v(buf);
+  }
+
+  const bool bad = __ballot(rows.bad) != 0;
+#pragma unroll
+  for (int ht = 0; ht < NT; ++ht) {
+    l[ht] = pair_sum(pair_sum(l[ht], 16), 32);
+    if (bad) l[ht] = __builtin_nanf("");
+#pragma unroll
+    for (int j = 0; j < VD; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[ht][j][i] = pair_sum(o[ht][j][i], 8) * (1.0f / float(1 << P::kScaleExp));
+    join_waves<VD, 32>(s_join, wave, G * 8 + (n & 7), !second, &m[ht], &l[ht], o[ht]);
+    if (wave == 0 && !second && ht * 8 + n < p.nh) leave<HD, VD, E>(a, p, p.h0 + ht * 8 + n, G, m[ht], l[ht], o[ht]);
+  }
 }
 
+// The f32 cache: 16 query heads as columns, tiles of 16 slots, v_mfma_f32_16x16x4f32 (exact f32 products).
 template <int HD>
-__global__ void __launch_bounds__(HD) k_paged_join(PagedAttnArgs a) {
-  const uint32_t item = blockIdx.x, h = item % a.H, row = item / a.H, d = threadIdx.x;
-  uint32_t lo, len;
-  const bool ok = row_range(a, row, &lo, &len);
-  float M, L, o = 0.0f;
-  join_ml(a, item, &M, &L);
-  for (uint32_t s = 0; s < a.splits; ++s) {
-    const size_t pt = size_t(item) * a.splits + s;
-    if (a.part_ml[pt * 2 + 1] != 0.0f) o += a.part_acc[pt * HD + d] * expf(a.part_ml[pt * 2] - M);
+__global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
+  constexpr int KP = HD / 16, VP = HD / 64, VD = HD / 16;
+  __shared__ uint64_t s_off[kWaves][2][16];
+  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 64];
+  const Place p = place_of<16>(a);
+  if (p.begin >= p.end) return leave_none<HD, 16>(a, p);  // (the whole workgroup)
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+
+  TileRows<16, 4> rows{s_off[wave]};
+  uint32_t t = p.begin + 16 * wave;
+  float4 kf[KP], vf[4][VP];
+  auto load_k = [&](int buf) {
+    const uint8_t* src = a.c.k + rows.s[buf][n] + G * 16;
+#pragma unroll
+    for (int c = 0; c < KP; ++c) kf[c] = ld_f4(reinterpret_cast<const float*>(src + 64 * c));
+  };
+  auto load_v = [&](int buf) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t* src = a.c.v + rows.s[buf][4 * G + r] + n * 16;
+#pragma unroll
+      for (int c = 0; c < VP; ++c) vf[r][c] = ld_f4(reinterpret_cast<const float*>(src + 256 * c));
+    }
+  };
+  rows.next(a, p, t, lane);
+  float4 q[KP];  // dims (G + 4 c) * 4 .. + 3 of head n
+  const bool head = uint32_t(n) < p.nh;
+#pragma unroll
+  for (int c = 0; c < KP; ++c) {
+    q[c] = ld_f4(a.q + p.row * a.q_stride + size_t(p.h0 + (head ? n : 0)) * HD + G * 4 + 16 * c);
+    if (!head) q[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
-  a.out[row * a.out_stride + h * HD + d] = !ok ? __builtin_nanf("") : (L == 0.0f ? 0.0f : o / L);
+  const float mult = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.0f;
+  f4_t o[VD];
+#pragma unroll
+  for (int j = 0; j < VD; ++j) o[j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  int buf = 0;
+  if (t < p.end) {
+    rows.put(a, p, 0, lane);
+    load_k(0);
+    load_v(0);
+    rows.next(a, p, t + 16 * kWaves, lane);
+  }
+  for (; t < p.end; t += 16 * kWaves) {
+    const bool more = t + 16 * kWaves < p.end;
+    f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < KP; ++c) {
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, q[c].x, sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, q[c].y, sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, q[c].z, sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, q[c].w, sc, 0, 0, 0);
+    }
+    buf ^= 1;
+    if (more) {
+      rows.put(a, p, buf, lane);
+      load_k(buf);
+      rows.next(a, p, t + 32 * kWaves, lane);
+    }
+    float s4[4], mx = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s4[i] = t + 4 * G + i < p.end ? sc[i] * mult : -INFINITY;
+      mx = fmaxf(mx, s4[i]);
+    }
+    if (a.scores && head)
+      *reinterpret_cast<float4*>(a.scores + (size_t(p.row) * a.H + p.h0 + n) * a.score_stride + (t - p.lo) + 4 * G) =
+          make_float4(s4[0], s4[1], s4[2], s4[3]);
+    mx = pair_max(pair_max(mx, 16), 32);
+    const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - base);
+    if (__ballot(f != 1.0f) != 0) {
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < VD; ++j) o[j] *= f;
+    }
+    m = mx;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s4[i] = __builtin_amdgcn_exp2f(s4[i] - base);
+      l += s4[i];
+    }
+#pragma unroll
+    for (int j = 0; j < VD; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 x = vf[i][j / 4];
+        const float v = j % 4 == 0 ? x.x : j % 4 == 1 ? x.y : j % 4 == 2 ? x.z : x.w;
+        o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s4[i], o[j], 0, 0, 0);
+      }
+    if (more) load_v(buf);
+  }
+  l = pair_sum(pair_sum(l, 16), 32);
+  if (__ballot(rows.bad) != 0) l = __builtin_nanf("");
+  join_waves<VD, 64>(s_join, wave, lane, true, &m, &l, o);
+  if (wave == 0 && head) leave<HD, VD, 4>(a, p, p.h0 + n, G, m, l, o);
 }
 
-__global__ void __launch_bounds__(256) k_paged_weights(PagedAttnArgs a, uint32_t blocks_per_row) {
-  const uint32_t part = blockIdx.x % blocks_per_row, item = blockIdx.x / blocks_per_row;
-  const uint32_t kvh = item % a.c.KV, row = item / a.c.KV, gq = a.H / a.c.KV, j = part * 256 + threadIdx.x;
+// ---- joining the splits, and the slots' weights -------------------------------------------------------------
+// the row's splits that hold slots
+__device__ __forceinline__ uint32_t splits_of(const PagedAttnArgs& a, uint32_t lo, uint32_t len) {
+  return (len - lo + a.chunk - 1) / a.chunk;
+}
+
+// maximum and sum over a head's splits, by one wave
+__device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, uint32_t ns, int lane, float* M, float* L) {
+  const float* ml = a.part_ml + size_t(item) * a.splits * 2;
+  float m = -INFINITY, l = 0.0f;
+  for (uint32_t s = lane; s < ns; s += 64) m = fmaxf(m, gld(ml + 2 * s));
+  m = wave_max(m);
+  if (m == -INFINITY) m = 0.0f;  // (no score above -inf)
+  for (uint32_t s = lane; s < ns; s += 64) l += gld(ml + 2 * s + 1) * __builtin_amdgcn_exp2f(gld(ml + 2 * s) - m);
+  *M = m;
+  *L = wave_sum(l);
+}
+
+// blocks 0 .. joins - 1: the output of one (row, head) each, its splits in 256 / (HD / 4) groups;
+// the others: the weights of 1024 slots of one (row, kv head)
+template <int HD>
+__global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t joins, uint32_t weight_parts) {
+  constexpr int D4 = HD / 4, GR = 256 / D4;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   uint32_t lo, len;
-  if (!row_range(a, row, &lo, &len) || j >= len) return;
-  float w = 0.0f;
-  for (uint32_t g = 0; j >= lo && g < gq; ++g) {
-    const uint32_t hh = row * a.H + kvh * gq + g;
+  if (blockIdx.x < joins) {
+    const uint32_t item = blockIdx.x, h = item % a.H, row = item / a.H;
+    const bool ok = row_range(a, row, &lo, &len);
+    const uint32_t ns = splits_of(a, lo, len);
+    __shared__ __align__(16) float s_o[GR][HD];
     float M, L;
-    join_ml(a, hh, &M, &L);
-    if (L != 0.0f) w += expf(a.scores[size_t(hh) * a.max_len + j] - M) / L;
+    join_ml(a, item, ns, lane, &M, &L);  // (every wave for itself)
+    const float* ml = a.part_ml + size_t(item) * a.splits * 2;
+    const float* acc = a.part_acc + size_t(item) * a.splits * HD + (tid % D4) * 4;
+    f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t s = tid / D4; s < ns; s += GR) {
+      const float4 x = ld_f4(acc + size_t(s) * HD);
+      o += f4_t{x.x, x.y, x.z, x.w} * __builtin_amdgcn_exp2f(gld(ml + 2 * s) - M);
+    }
+    *reinterpret_cast<f4_t*>(&s_o[tid / D4][(tid % D4) * 4]) = o;
+    __syncthreads();
+    if (tid < HD) {
+      float v = 0.0f;
+#pragma unroll
+      for (int g = 0; g < GR; ++g) v += s_o[g][tid];
+      a.out[row * a.out_stride + size_t(h) * HD + tid] = !ok ? __builtin_nanf("") : (L == 0.0f ? 0.0f : v / L);
+    }
+    return;
   }
-  const size_t at = (size_t(row) * a.c.KV + kvh) * a.weight_stride + j;
-  a.weight_out[at] = (a.weight_in ? a.weight_in[at] : 0.0f) + w;
+  const uint32_t b = blockIdx.x - joins, part = b % weight_parts, item = b / weight_parts;
+  const uint32_t kvh = item % a.c.KV, row = item / a.c.KV, gq = a.H / a.c.KV, first = part * 1024;
+  row_range(a, row, &lo, &len);
+  if (first >= len) return;
+  const uint32_t ns = splits_of(a, lo, len);
+  __shared__ float s_ml[64][2];
+  float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t g0 = 0; g0 < gq; g0 += 64) {  // 64 query heads at a time
+    const uint32_t ng = min(64u, gq - g0);
+    __syncthreads();
+    for (uint32_t g = wave; g < ng; g += kWaves) {
+      float M, L;
+      join_ml(a, row * a.H + kvh * gq + g0 + g, ns, lane, &M, &L);
+      if (lane == 0) {
+        s_ml[g][0] = M;
+        s_ml[g][1] = L == 0.0f ? 0.0f : 1.0f / L;
+      }
+    }
+    __syncthreads();
+    for (uint32_t g = 0; g < ng; ++g) {
+      const float* sc = a.scores + (size_t(row) * a.H + kvh * gq + g0 + g) * a.score_stride;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t j = first + k * 256 + tid;
+        if (j >= lo && j < len) w[k] += __builtin_amdgcn_exp2f(gld(sc + (j - lo)) - s_ml[g][0]) * s_ml[g][1];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t j = first + k * 256 + tid;
+    if (j >= len) continue;
+    const size_t at = (size_t(row) * a.c.KV + kvh) * a.weight_stride + j;
+    a.weight_out[at] = (a.weight_in ? a.weight_in[at] : 0.0f) + w[k];
+  }
 }
 
+// ---- host -----------------------------------------------------------------------------------------------------
+// How the rows are split: a workgroup's slots (`chunk`) are a multiple of its tiles; about 4 workgroups per CU
+// where there are few rows, at most 1024 slots a workgroup where there are many (rows of different lengths
+// then still spread evenly: the chip takes the next workgroup where one ends), at most 512 splits.
 struct AttnPlan {
-  uint32_t splits = 1, chunk = 1;
+  uint32_t splits = 1, chunk = 1, score_stride = 0;
+  uint64_t groups = 0;  // (row, kv head, group of query heads)
   size_t off_acc = 0, off_scores = 0, bytes = 0;
 };
 
-// at most this many splits of a range of slots (it grows with the range)
-uint32_t most_splits(uint64_t items, uint32_t range) {
-  const uint64_t want = (8192 + items - 1) / items, most = (uint64_t(range) + 31) / 32;
-  return uint32_t(std::max<uint64_t>(1, std::min(want, most)));
+// query heads a workgroup serves: 16 columns, of which two hold one head with a 16-bit cache; two such tiles
+// of heads where the accumulators of both fit the registers
+uint32_t heads_per_group(const chpe_kv_pages* c, uint32_t heads) {
+  return c->type == 0 || (heads / c->kv_heads > 8 && c->head_dim <= 128) ? 16 : 8;
+}
+
+void split_range(uint64_t groups, uint32_t range, uint32_t step, uint32_t* splits, uint32_t* chunk) {
+  const uint64_t n = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step);  // steps in all
+  uint64_t want = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(range) + 1023) / 1024);
+  want = std::min<uint64_t>(std::min<uint64_t>(want, n), 512);
+  const uint64_t per = (n + want - 1) / want;
+  *chunk = uint32_t(per * step);
+  *splits = uint32_t((n + per - 1) / per);
 }
 
 AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uint32_t window, bool weights) {
   AttnPlan p;
-  const uint32_t range = window != 0 && window < max_len ? window : max_len;
-  const uint64_t items = std::max<uint64_t>(1, uint64_t(c->rows) * heads);
-  p.chunk = std::max(1u, (range + most_splits(items, range) - 1) / most_splits(items, range));
-  p.splits = range ? (range + p.chunk - 1) / p.chunk : 1;
-  // the workspace does not depend on the window
+  const uint32_t gq = heads / c->kv_heads, ht = heads_per_group(c, heads), step = (c->type == 0 ? 16 : 32) * kWaves;
+  p.groups = uint64_t(c->rows) * c->kv_heads * ((gq + ht - 1) / ht);
+  const uint64_t groups = std::max<uint64_t>(1, p.groups), items = uint64_t(c->rows) * heads;
+  split_range(groups, window != 0 && window < max_len ? window : max_len, step, &p.splits, &p.chunk);
+  // the workspace does not depend on the window: room for the most splits of any shorter range, which the
+  // wanted number bounds
+  const uint64_t n = std::max<uint64_t>(1, (uint64_t(max_len) + step - 1) / step);
+  uint64_t room = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(max_len) + 1023) / 1024);
+  room = std::min<uint64_t>(std::min<uint64_t>(room, n), 512);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  const uint32_t room = most_splits(items, max_len);
   p.off_acc = up(items * room * 8);
   p.off_scores = p.off_acc + up(items * room * c->head_dim * 4);
-  p.bytes = p.off_scores + (weights ? up(items * max_len * 4) : 0);
+  p.score_stride = uint32_t((max_len + 63) / 64 * 64);
+  p.bytes = p.off_scores + (weights ? up(items * p.score_stride * 4) : 0);
   return p;
 }
 
-template <class T>
-bool launch_attn(const PagedAttnArgs& a, uint32_t hd, hipStream_t st) {
-  const uint64_t items = uint64_t(a.rows) * a.H, blocks = items * a.splits;
+template <int HD>
+bool launch_attn(const PagedAttnArgs& a, int type, uint64_t groups, hipStream_t st) {
+  const uint64_t blocks = groups * a.splits;
+  const uint32_t thr = kWaves * 64;
   bool ok;
-  if (hd == 64) ok = launch(&k_paged_partial<64, T>, blocks, 64, st, a) && launch(&k_paged_join<64>, items, 64, st, a);
-  else if (hd == 128) ok = launch(&k_paged_partial<128, T>, blocks, 64, st, a) && launch(&k_paged_join<128>, items, 128, st, a);
-  else ok = launch(&k_paged_partial<256, T>, blocks, 64, st, a) && launch(&k_paged_join<256>, items, 256, st, a);
-  if (ok && a.weight_out && a.max_len) {
-    const uint32_t per = (a.max_len + 255) / 256;
-    ok = launch(&k_paged_weights, uint64_t(a.rows) * a.c.KV * per, 256, st, a, per);
-  }
+  if (type == 0) ok = launch(&k_paged_32<HD>, blocks, thr, st, a);
+  else if (type == 1) ok = launch(&k_paged_16<HD, _Float16, 1>, blocks, thr, st, a);
+  else ok = launch(&k_paged_16<HD, Bf16, 1>, blocks, thr, st, a);
   return ok;
+}
+template <int HD>
+bool launch_attn2(const PagedAttnArgs& a, int type, uint64_t groups, hipStream_t st) {  // two tiles of heads
+  const uint64_t blocks = groups * a.splits;
+  return type == 1 ? launch(&k_paged_16<HD, _Float16, 2>, blocks, kWaves * 64, st, a)
+                   : launch(&k_paged_16<HD, Bf16, 2>, blocks, kWaves * 64, st, a);
 }
 
 bool attn_shape_ok(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len) {
@@ -190,7 +643,9 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   if (q_stride % 4 || out_stride % 4 || (cache->rows > 1 && (q_stride < width || out_stride < width))) return -1;
   if ((weight_in && !weight_out) || (weight_out && weight_stride < max_len)) return -1;
   const AttnPlan p = attn_plan(cache, heads, max_len, window, weight_out != nullptr);
-  if (uint64_t(cache->rows) * heads * p.splits > kMaxBlocks) return -1;
+  const uint32_t parts = weight_out ? (max_len + 1023) / 1024 : 0, joins = p.splits > 1 ? cache->rows * heads : 0;
+  const uint64_t joined = uint64_t(joins) + uint64_t(cache->rows) * cache->kv_heads * parts;
+  if (uint64_t(cache->rows) * heads > kMaxBlocks || p.groups * p.splits > kMaxBlocks || joined > kMaxBlocks) return -1;
   if (workspace_bytes < p.bytes) return -2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.q = q;
@@ -211,8 +666,17 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.scale = scale;
-  const bool ok = cache->type == 0 ? launch_attn<float>(a, cache->head_dim, st)
-                                   : cache->type == 1 ? launch_attn<_Float16>(a, cache->head_dim, st)
-                                                      : launch_attn<Bf16>(a, cache->head_dim, st);
+  a.score_stride = p.score_stride;
+  const int type = cache->type;
+  const uint32_t hd = cache->head_dim, ht = heads_per_group(cache, heads);
+  bool ok;
+  if (type != 0 && ht == 16) ok = hd == 64 ? launch_attn2<64>(a, type, p.groups, st) : launch_attn2<128>(a, type, p.groups, st);
+  else ok = hd == 64    ? launch_attn<64>(a, type, p.groups, st)
+            : hd == 128 ? launch_attn<128>(a, type, p.groups, st)
+                        : launch_attn<256>(a, type, p.groups, st);
+  if (ok && joined != 0)
+    ok = hd == 64    ? launch(&k_paged_join<64>, joined, 256, st, a, joins, parts)
+         : hd == 128 ? launch(&k_paged_join<128>, joined, 256, st, a, joins, parts)
+                     : launch(&k_paged_join<256>, joined, 256, st, a, joins, parts);
   return ok ? 0 : -3;
 }

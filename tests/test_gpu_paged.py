@@ -151,6 +151,30 @@ def test_attention_query_ranges(size, scale, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_small_keys_and_values(dtype):
+    """Keys and values among fp16's subnormal numbers."""
+    pool = Pool(2, 200, 2, 128, 16, dtype, seed=12)
+    pool.k.mul_(2.0 ** -17)
+    pool.v.mul_(2.0 ** -17)
+    q = torch.randn(2, 16, 128, generator=torch.Generator().manual_seed(12)) * 1000
+    check_attention(pool, q, [200, 77], 200, scale=3.0, weights=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_splits_of_very_different_scores(dtype):
+    """Scores that fall by hundreds from one split to the next: the join's maximum is the row's, however low."""
+    n = 4000
+    pool = Pool(1, n, 1, 64, 16, dtype, seed=13)
+    at = torch.arange(n)
+    pool.k[pool.table[0, at // 16].long().cuda(), 0, (at % 16).cuda(), 0] = (-at.float()).to(pool.k.dtype).cuda()
+    q = torch.randn(1, 3, 64, generator=torch.Generator().manual_seed(13))
+    q[0, :, 0] = torch.tensor([5.0, -5.0, 40.0])
+    check_attention(pool, q, [n], n, weights=True)
+    pool.k[:, :, :, 0] = -4000.0
+    check_attention(pool, q, [n], n, weights=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_attention_sharp_and_flat_rows(dtype):
     """One slot that takes nearly everything, at the ends of tiles and splits; equal keys, whose weights are
     equal."""
