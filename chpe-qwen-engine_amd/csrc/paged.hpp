@@ -1,7 +1,7 @@
 // paged.hpp -- what the operators of the paged key/value cache share: the cache's addressing on the
 // device, the checks of its description and of the stream on the host, the launch.
 #pragma once
-#include <hip/hip_bf16.h>
+#include <utility>
 
 #include "../../include/chpe.h"
 #include "device_common.hpp"

@@ -3,7 +3,7 @@
 // gains are given), the rotary embedding of its first rot dims, y0 = x0 c - x1 s, y1 = x0 s + x1 c with
 // the pair (i, i + rot/2) or (2i, 2i + 1); keys and values are rounded once to the cache's type, queries
 // stay f32.  The arithmetic of k_hyb_qk (hybrid.hip) on caller buffers.
-#include <utility>
+#include <algorithm>
 
 #include "paged.hpp"
 
@@ -24,60 +24,113 @@ struct AppendArgs {
   float eps;
 };
 
+// HD / 4 lanes hold one head's row, 16 bytes each; a workgroup's 256 / (HD / 4) groups of lanes walk the rows
+// of one token: the query heads, the key heads, the value heads.  A lane keeps the same dims in every row, so
+// its gains, cosines and sines are read once.
 template <int HD, class T>
-__global__ void __launch_bounds__(HD) k_paged_append(AppendArgs a) {
+__global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, uint32_t parts) {
 #pragma clang fp contract(off)
-  const uint32_t per = a.H + 2 * a.c.KV, t = blockIdx.x / per, b = blockIdx.x % per, d = threadIdx.x;
-  const bool is_q = b < a.H, is_k = !is_q && b < a.H + a.c.KV;
-  const uint32_t h = is_q ? b : (is_k ? b - a.H : b - a.H - a.c.KV);
-  __shared__ float s_x[HD], s_red[HD / 64];
-  const int32_t pos = gld(a.pos + t);
-  float x = is_q ? gld(a.q + t * a.q_stride + h * a.q_head_stride + d)
-                 : gld((is_k ? a.k + t * a.k_stride : a.v + t * a.v_stride) + h * HD + d);
-  const float* gain = is_q ? a.q_norm : a.k_norm;
+  constexpr int L = HD / 4, GR = 256 / L, U = 4;  // U rows of a group in flight
+  const uint32_t t = blockIdx.x / parts, part = blockIdx.x % parts;
+  const uint32_t lane = threadIdx.x % L, d = lane * 4, n_rows = a.H + 2 * a.c.KV, half = a.rot / 2;
+  const uint32_t step = parts * GR;
+  uint32_t r = part * GR + threadIdx.x / L;
+  const int32_t pos = gld(a.pos + t), row = gld(a.row + t), slot = gld(a.slot + t);
   const bool turns = a.rot == 0 || (pos >= 0 && uint32_t(pos) < a.rope_rows);
-  if (is_q || is_k) {
-    if (gain) {
-      const float s2 = wave_sum(x * x);
-      if ((d & 63) == 0) s_red[d >> 6] = s2;
-      __syncthreads();
-      float tot = 0.0f;
-      for (int w = 0; w < HD / 64; ++w) tot += s_red[w];
-      x = x * (1.0f / sqrtf(tot / float(HD) + a.eps)) * gain[d];
-    }
-    s_x[d] = x;
-    __syncthreads();
-    const uint32_t half = a.rot / 2;
-    if (d < a.rot && turns) {
-      const uint32_t i = a.interleaved ? d / 2 : (d < half ? d : d - half);
-      const bool first = a.interleaved ? (d & 1) == 0 : d < half;
-      const float c = a.rope_cos[size_t(pos) * half + i], s = a.rope_sin[size_t(pos) * half + i];
-      const float x0 = a.interleaved ? s_x[2 * i] : s_x[i], x1 = a.interleaved ? s_x[2 * i + 1] : s_x[i + half];
-      x = first ? x0 * c - x1 * s : x0 * s + x1 * c;
+  // (uniform in the workgroup)
+  uint32_t page = 0;
+  const bool writes = turns && row >= 0 && uint32_t(row) < a.rows && slot >= 0 && uint32_t(slot) < a.c.capacity &&
+                      a.c.page_of(row, slot, &page);
+  float4 x[U];
+  auto load = [&](uint32_t at, float4& v) {
+    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (at >= n_rows) return;
+    const float* src = at < a.H ? a.q + t * a.q_stride + at * a.q_head_stride
+                       : at < a.H + a.c.KV ? a.k + t * a.k_stride + size_t(at - a.H) * HD
+                                           : a.v + t * a.v_stride + size_t(at - a.H - a.c.KV) * HD;
+    v = ld_f4(src + d);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) load(r + u * step, x[u]);
+  float4 gq = make_float4(1, 1, 1, 1), gk = gq, cs = gq, sn = make_float4(0, 0, 0, 0);
+  if (a.q_norm) gq = ld_f4(a.q_norm + d);
+  if (a.k_norm) gk = ld_f4(a.k_norm + d);
+  const bool in_rot = d < a.rot && turns;
+  if (in_rot) {
+    if (a.interleaved) {  // pairs d / 2 and d / 2 + 1
+      const float2 c = *reinterpret_cast<const float2*>(a.rope_cos + size_t(pos) * half + d / 2);
+      const float2 s = *reinterpret_cast<const float2*>(a.rope_sin + size_t(pos) * half + d / 2);
+      cs = make_float4(c.x, c.x, c.y, c.y);
+      sn = make_float4(-s.x, s.x, -s.y, s.y);
+    } else {
+      const uint32_t i = d < half ? d : d - half;
+      cs = ld_f4(a.rope_cos + size_t(pos) * half + i);
+      sn = ld_f4(a.rope_sin + size_t(pos) * half + i);
+      if (d < half) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);
     }
   }
-  if (is_q) {
-    a.q_out[(size_t(t) * a.H + h) * HD + d] = turns ? x : __builtin_nanf("");
-    return;
-  }
-  const int32_t row = gld(a.row + t), slot = gld(a.slot + t);
-  if (row < 0 || uint32_t(row) >= a.rows || slot < 0 || uint32_t(slot) >= a.c.capacity || !turns) return;
-  uint32_t page;
-  if (!a.c.page_of(row, slot, &page)) return;
-  reinterpret_cast<T*>(is_k ? a.c.k : a.c.v)[a.c.at(page, h, slot) + d] = Elem<T>::put(x);
-  if (is_k && d == 0 && uint64_t(slot) < a.track_stride) {
-    const size_t at = (size_t(row) * a.c.KV + h) * a.track_stride + slot;
-    if (a.slot_pos) a.slot_pos[at] = pos;
-    if (a.slot_weight) a.slot_weight[at] = 0.0f;
+  // the lane of the other half of the pairs
+  const int base = int(threadIdx.x & 63) - int(lane);
+  const int other = base + (!in_rot ? int(lane) : d < half ? int(lane + half / 4) : int(lane - half / 4));
+
+  while (true) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = r + u * step;
+      float4 y = x[u];
+      load(at + U * step, x[u]);
+      if (at - threadIdx.x / L >= n_rows) return;  // (the whole workgroup)
+      const bool is_q = at < a.H, is_v = at >= a.H + a.c.KV;
+      if ((is_q ? a.q_norm : a.k_norm) != nullptr && !is_v) {
+        float s2 = (y.x * y.x + y.y * y.y) + (y.z * y.z + y.w * y.w);
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) s2 += __shfl_xor(s2, o);
+        const float inv = 1.0f / sqrtf(s2 / float(HD) + a.eps);
+        const float4 g = is_q ? gq : gk;
+        y = make_float4(y.x * inv * g.x, y.y * inv * g.y, y.z * inv * g.z, y.w * inv * g.w);
+      }
+      if (a.rot != 0) {
+        float4 z;  // the pairs' other halves
+        if (a.interleaved) z = make_float4(y.y, y.x, y.w, y.z);
+        else z = make_float4(__shfl(y.x, other), __shfl(y.y, other), __shfl(y.z, other), __shfl(y.w, other));
+        if (in_rot && !is_v)
+          y = make_float4(y.x * cs.x + z.x * sn.x, y.y * cs.y + z.y * sn.y, y.z * cs.z + z.z * sn.z, y.w * cs.w + z.w * sn.w);
+      }
+      if (at >= n_rows) continue;
+      if (is_q) {
+        if (!turns) y.x = y.y = y.z = y.w = __builtin_nanf("");
+        *reinterpret_cast<float4*>(a.q_out + (size_t(t) * a.H + at) * HD + d) = y;
+      } else if (writes) {
+        const uint32_t h = is_v ? at - a.H - a.c.KV : at - a.H;
+        T* dst = reinterpret_cast<T*>(is_v ? a.c.v : a.c.k) + a.c.at(page, h, slot) + d;
+        struct alignas(4 * sizeof(T)) Four { T e[4]; };
+        *reinterpret_cast<Four*>(dst) = Four{{Elem<T>::put(y.x), Elem<T>::put(y.y), Elem<T>::put(y.z), Elem<T>::put(y.w)}};
+        if (!is_v && lane == 0 && uint64_t(slot) < a.track_stride) {
+          const size_t i = (size_t(row) * a.c.KV + h) * a.track_stride + slot;
+          if (a.slot_pos) a.slot_pos[i] = pos;
+          if (a.slot_weight) a.slot_weight[i] = 0.0f;
+        }
+      }
+    }
+    r += U * step;
   }
 }
 
+// workgroups per token: one where the tokens alone fill the chip (8 workgroups a CU), as many as its rows
+// allow where they are few
+uint32_t token_parts(uint32_t tokens, uint32_t n_rows, uint32_t groups) {
+  const uint32_t most = (n_rows + groups - 1) / groups, want = (2048 + tokens - 1) / tokens;
+  return std::max(1u, std::min(most, want));
+}
+
+template <int HD, class T>
+bool launch_append_hd(const AppendArgs& a, hipStream_t st) {
+  const uint32_t parts = token_parts(a.tokens, a.H + 2 * a.c.KV, 256 / (HD / 4));
+  return launch(&k_paged_append<HD, T>, uint64_t(a.tokens) * parts, 256, st, a, parts);
+}
 template <class T>
 bool launch_append(const AppendArgs& a, uint32_t hd, hipStream_t st) {
-  const uint64_t blocks = uint64_t(a.tokens) * (a.H + 2 * a.c.KV);
-  if (hd == 64) return launch(&k_paged_append<64, T>, blocks, 64, st, a);
-  if (hd == 128) return launch(&k_paged_append<128, T>, blocks, 128, st, a);
-  return launch(&k_paged_append<256, T>, blocks, 256, st, a);
+  return hd == 64 ? launch_append_hd<64, T>(a, st) : hd == 128 ? launch_append_hd<128, T>(a, st) : launch_append_hd<256, T>(a, st);
 }
 
 }  // namespace
@@ -106,7 +159,9 @@ extern "C" int chpe_paged_append(const chpe_kv_pages* cache, uint32_t tokens, ui
   if (rot_dim > hd || rot_dim % 8 != 0 || (rot_dim != 0 && (!rope_cos || !rope_sin || rope_rows == 0))) return -1;
   if (!aligned16(rope_cos) || !aligned16(rope_sin)) return -1;
   if ((slot_pos || slot_weight) && track_stride == 0) return -1;
-  if (heads > 65536 || cache->kv_heads > 65536 || uint64_t(tokens) * (heads + 2 * cache->kv_heads) > kMaxBlocks) return -1;
+  if (heads > 65536 || cache->kv_heads > 65536 || uint64_t(tokens) * (heads + 2 * cache->kv_heads) > (uint64_t(1) << 31) ||
+      uint64_t(tokens) > kMaxBlocks)
+    return -1;
   a.q = q;
   a.k = k;
   a.v = v;
