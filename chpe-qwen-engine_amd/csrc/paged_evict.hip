@@ -47,53 +47,93 @@ __device__ __forceinline__ int32_t block_max(int32_t v, int32_t* s) {
   return v;
 }
 
-// The threshold T that `keep` of len keys reach, and how many of the keys equal to it stay.  Two bits of T a
-// step, from the top: how many keys reach T + 1, 2, 3 of the step's size says which of the four intervals
-// holds the keep-th largest key.  A step ends the search where an interval's lower end is reached by exactly
-// `keep` keys.  count(cand, n): adds this wave's number of keys >= cand[i] to n[i] (uniform in the wave).
+// inclusive prefix sum over the wave on the vector ALU: row_shr 1, 2, 4, 8 within rows of 16 lanes, then the
+// last lane of row 0 / 2 to row 1 / 3 (row_bcast 15) and lane 31 to the upper half (row_bcast 31)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xa, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xc, 0xf, false));
+  return v;
+}
+// the sum over the waves before this one, and over all, of what every wave's last lane holds
+__device__ __forceinline__ uint32_t waves_before(uint32_t last, uint32_t* s, uint32_t* all) {
+  const uint32_t wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 63) s[wave] = last;
+  __syncthreads();
+  uint32_t before = 0, sum = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kSelWaves; ++w) {
+    const uint32_t x = s[w];
+    before += w < wave ? x : 0u;
+    sum += x;
+  }
+  *all = sum;
+  return before;
+}
+
+// The threshold T that `keep` of len keys reach, and how many of the keys equal to it stay: the digits of T
+// from the top, 11, 11 and 10 bits, each from a histogram of the keys that share the digits above it.  The
+// search ends where a bin is kept whole.  each(f): calls f(valid, key) for every key of this thread, with all
+// lanes of the wave active.
 struct Threshold {
   uint32_t T, ties;
-  bool all;  // every key equal to T stays
+  bool all;  // every key that reaches T stays
 };
-template <class Count>
-__device__ __forceinline__ Threshold find_threshold(uint32_t len, uint32_t keep, uint32_t (*s)[4], Count count) {
+constexpr int kBins = 2048;
+template <class Each>
+__device__ __forceinline__ Threshold find_threshold(uint32_t len, uint32_t keep, uint32_t* hist, uint32_t* s, uint32_t* found,
+                                                    Each each) {
   if (keep == len) return {0u, len, true};
-  uint32_t T = 0, reach = len, above = 0;  // keys >= T; keys >= T + the last step's size
-  int buf = 0;
-  for (int bit = 30; bit >= 0 && reach != keep; bit -= 2, buf = buf == 2 ? 0 : buf + 1) {
-    const uint32_t cand[3] = {T + (1u << bit), T + (2u << bit), T + (3u << bit)};
-    uint32_t n[3] = {0, 0, 0};
-    count(cand, n);
-    // three buffers: this step's was cleared in the step before, when the step before that had been read
-    if (threadIdx.x < 3) s[buf == 2 ? 0 : buf + 1][threadIdx.x] = 0;
-    if ((threadIdx.x & 63) < 3) atomicAdd(&s[buf][threadIdx.x & 63], (threadIdx.x & 63) == 0 ? n[0] : (threadIdx.x & 63) == 1 ? n[1] : n[2]);
+  if (keep == 0) return {0xffffffffu, 0u, false};
+  const uint32_t tid = threadIdx.x;
+  uint32_t T = 0, need = keep;  // the digits so far; keys still to be found below the larger ones
+  for (int shift = 21, bits = 11;; ) {
+    hist[tid] = hist[tid + kSelect] = 0;
     __syncthreads();
-    const uint32_t c1 = s[buf][0], c2 = s[buf][1], c3 = s[buf][2];
-    if (c3 >= keep) T = cand[2], reach = c3;
-    else if (c2 >= keep) T = cand[1], reach = c2, above = c3;
-    else if (c1 >= keep) T = cand[0], reach = c1, above = c2;
-    else above = c1;
+    const uint32_t above = T >> (shift + bits - 1) >> 1;  // (shift + bits may be 32)
+    each([&](bool valid, uint32_t key) {
+      const bool in = valid && key >> (shift + bits - 1) >> 1 == above;
+      const uint32_t bin = key >> shift & ((1u << bits) - 1);
+      // a wave whose keys all fall into one bin (equal weights) counts them at once
+      const uint64_t who = __ballot(in);
+      if (who == 0) return;
+      const uint32_t first = __builtin_amdgcn_readlane(bin, __ffsll((unsigned long long)who) - 1);
+      if (__ballot(in && bin == first) == who) {
+        if ((tid & 63) == 0) atomicAdd(&hist[first], uint32_t(__popcll(who)));
+      } else if (in) {
+        atomicAdd(&hist[bin], 1u);
+      }
+    });
+    __syncthreads();
+    // from the largest bin down, two bins a thread: the bin that holds the need-th key
+    const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid], x = wave_scan(hi + lo);
+    uint32_t all;
+    const uint32_t before = waves_before(x, s, &all) + x - hi - lo;
+    if (before < need && need <= before + hi + lo) {
+      const bool upper = need <= before + hi;
+      found[0] = upper ? kBins - 1 - 2 * tid : kBins - 2 - 2 * tid;
+      found[1] = upper ? before : before + hi;
+      found[2] = upper ? hi : lo;
+    }
+    __syncthreads();
+    T |= found[0] << shift;
+    need -= found[1];
+    if (need == found[2] || shift == 0) return {T, need, need == found[2]};
+    bits = shift == 21 ? 11 : 10;
+    shift = shift == 21 ? 10 : 0;
   }
-  return {T, reach == keep ? keep : keep - above, reach == keep};
 }
 
 // exclusive prefix sums of n <= kSelect values in LDS; returns the total
 __device__ __forceinline__ uint32_t block_scan(uint32_t* tab, uint32_t n, uint32_t* s) {
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x;
   __syncthreads();
-  const uint32_t v = tid < n ? tab[tid] : 0u;
-  uint32_t x = v;
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(x, o);
-    if (lane >= uint32_t(o)) x += y;
-  }
-  if (lane == 63) s[wave] = x;
-  __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (uint32_t w = 0; w < kSelWaves; ++w) {
-    if (w < wave) before += s[w];
-    all += s[w];
-  }
+  const uint32_t v = tid < n ? tab[tid] : 0u, x = wave_scan(v);
+  uint32_t all;
+  const uint32_t before = waves_before(x, s, &all);
   if (tid < n) tab[tid] = before + x - v;
   __syncthreads();
   return all;
@@ -122,17 +162,13 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, uint32_t row, uint
 // movers among the slots, from one table of counts per (1024 slots, wave).
 template <int KPT>
 __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
-  __shared__ uint32_t s_tab[KPT * kSelWaves], s_red[kSelWaves], s_cnt[3][4], s_moves[2 * kFusedMoves];
+  __shared__ uint32_t s_tab[KPT * kSelWaves], s_red[kSelWaves], s_found[3], s_moves[2 * kFusedMoves], s_hist[kBins];
   const uint32_t item = blockIdx.x, row = item / a.c.KV, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
   const uint32_t raw = uint32_t(gld(a.lens + row));
   const bool bad = raw > a.max_len;
   const uint32_t len = bad ? 0u : raw, keep = min(len, a.budget);
   if (tid == 0 && item % a.c.KV == 0) a.lens_out[row] = bad ? int32_t(raw) : int32_t(keep);
-  if (len == 0) {
-    if (tid == 0) a.n_moves[item] = 0;
-    return;
-  }
   const size_t base = size_t(item) * a.stride;
   const float* weight = a.weight + base;
   const int32_t* pos = a.pos + base;
@@ -144,7 +180,8 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
   float w[HOLD];
   int32_t p[HOLD], newest = INT32_MIN;
   uint32_t key[KPT];
-  auto slot_of = [&](int k) { return min(k * kSelect + tid, len - 1); };
+  // (up to max_len, not to the row's length: the loads do not wait for it)
+  auto slot_of = [&](int k) { return min(k * kSelect + tid, a.max_len - 1); };
   if constexpr (kHold) {
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
@@ -152,9 +189,12 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
       w[k] = gld(weight + slot_of(k));
     }
   }
+  if (len == 0) {  // (the whole workgroup)
+    if (tid == 0) a.n_moves[item] = 0;
+    return;
+  }
 #pragma unroll
-  for (int k = 0; k < KPT; ++k) newest = max(newest, kHold ? p[k % HOLD] : gld(pos + slot_of(k)));
-  if (tid < 12) s_cnt[tid / 4][tid % 4] = 0;
+  for (int k = 0; k < KPT; ++k) newest = max(newest, k * kSelect + tid >= len ? INT32_MIN : kHold ? p[k % HOLD] : gld(pos + slot_of(k)));
   newest = block_max(newest, reinterpret_cast<int32_t*>(s_red));
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
@@ -163,41 +203,40 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
     key[k] = k * kSelect + tid < len ? slot_key(a, wk, pk, newest) : 0u;
   }
 
-  const Threshold th = find_threshold(len, keep, s_cnt, [&](const uint32_t (&cand)[3], uint32_t (&n)[3]) {
+  const Threshold th = find_threshold(len, keep, s_hist, s_red, s_found, [&](auto f) {
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
       if (uint32_t(k) * kSelect >= len) break;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) n[i] += __popcll(__ballot(key[k] >= cand[i]));
+      f(k * kSelect + tid < len, key[k]);
     }
   });
 
   // of the keys equal to the threshold the first `ties` slots stay
-  uint64_t kept[KPT];
+  uint32_t kept = 0;  // bit k: slot k * kSelect + tid
 #pragma unroll
-  for (int k = 0; k < KPT; ++k) kept[k] = __ballot(k * kSelect + tid < len && key[k] >= th.T);
+  for (int k = 0; k < KPT; ++k)
+    if (k * kSelect + tid < len && key[k] >= th.T) kept |= 1u << k;
+  auto is_kept = [&](int k) { return (kept >> k & 1) != 0; };
   if (!th.all) {
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
-      const uint64_t eq = __ballot(k * kSelect + tid < len && key[k] == th.T);
+      const uint64_t eq = __ballot(is_kept(k) && key[k] == th.T);
       if (lane == 0) s_tab[k * kSelWaves + wave] = __popcll(eq);
     }
     block_scan(s_tab, KPT * kSelWaves, s_red);
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
-      const bool eq = k * kSelect + tid < len && key[k] == th.T;
+      const bool eq = is_kept(k) && key[k] == th.T;
       const uint32_t rank = s_tab[k * kSelWaves + wave] + below(__ballot(eq), lane);
-      kept[k] &= ~__ballot(eq && rank >= th.ties);
+      if (eq && rank >= th.ties) kept &= ~(1u << k);
     }
     __syncthreads();
   }
-  // holes in the lower, movers in the upper half of a count (either is at most half of 65536 slots)
-  const uint64_t bit = uint64_t(1) << lane;
+  // holes in the lower, movers in the upper half of a count (either is at most half of kLongest)
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
     const uint32_t j = k * kSelect + tid;
-    const uint64_t in = __ballot(j < keep);
-    const uint32_t holes = __popcll(in & ~kept[k]), movers = __popcll(kept[k] & ~in);
+    const uint32_t holes = __popcll(__ballot(j < keep && !is_kept(k))), movers = __popcll(__ballot(j >= keep && is_kept(k)));
     if (lane == 0) s_tab[k * kSelWaves + wave] = holes | movers << 16;
   }
   const uint32_t moves = block_scan(s_tab, KPT * kSelWaves, s_red) & 0xffffu;
@@ -206,11 +245,12 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
     const uint32_t j = k * kSelect + tid;
-    const uint64_t in = __ballot(j < keep);
+    const bool hole = j < keep && !is_kept(k), mover = j >= keep && is_kept(k);
     const uint32_t at = s_tab[k * kSelWaves + wave];
-    if (j < keep && !(kept[k] & bit)) to[(at & 0xffffu) + below(in & ~kept[k], lane)] = j;
-    if (j >= keep && (kept[k] & bit)) from[(at >> 16) + below(kept[k] & ~in, lane)] = j;
-    if (j < keep && (kept[k] & bit)) {
+    const uint32_t rh = (at & 0xffffu) + below(__ballot(hole), lane), rm = (at >> 16) + below(__ballot(mover), lane);
+    if (hole) to[rh] = j;
+    if (mover) from[rm] = j;
+    if (j < keep && is_kept(k)) {
       a.weight_out[base + j] = kHold ? w[k % HOLD] : gld(weight + j);
       a.pos_out[base + j] = kHold ? p[k % HOLD] : gld(pos + j);
       if (a.slot_src) a.slot_src[base + j] = int32_t(j);
@@ -228,7 +268,7 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
 }
 
 // The same for rows past kLongest slots: the keys are read again for every step, the ranks counted in one walk.
-constexpr uint32_t kLongest = 64 * kSelect;
+constexpr uint32_t kLongest = 32 * kSelect;
 __device__ __forceinline__ uint32_t block_rank(bool f, uint32_t* s, uint32_t* total) {
   const uint64_t b = __ballot(f);
   const int wave = threadIdx.x >> 6;
@@ -245,7 +285,7 @@ __device__ __forceinline__ uint32_t block_rank(bool f, uint32_t* s, uint32_t* to
 }
 
 __global__ void __launch_bounds__(kSelect) k_evict_select_long(EvictArgs a) {
-  __shared__ uint32_t s_red[kSelWaves], s_cnt[3][4];
+  __shared__ uint32_t s_red[kSelWaves], s_found[3], s_hist[kBins];
   const uint32_t item = blockIdx.x, row = item / a.c.KV, tid = threadIdx.x;
   const uint32_t raw = uint32_t(gld(a.lens + row));
   const bool bad = raw > a.max_len;
@@ -257,14 +297,10 @@ __global__ void __launch_bounds__(kSelect) k_evict_select_long(EvictArgs a) {
 
   int32_t newest = INT32_MIN;
   for (uint32_t j = tid; j < len; j += kSelect) newest = max(newest, pos[j]);
-  if (tid < 12) s_cnt[tid / 4][tid % 4] = 0;
   newest = block_max(newest, reinterpret_cast<int32_t*>(s_red));
   auto key = [&](uint32_t j) { return slot_key(a, gld(weight + j), gld(pos + j), newest); };
-  const Threshold th = find_threshold(len, keep, s_cnt, [&](const uint32_t (&cand)[3], uint32_t (&n)[3]) {
-    for (uint32_t j0 = 0; j0 < len; j0 += kSelect) {
-      const uint32_t k = j0 + tid < len ? key(j0 + tid) : 0u;
-      for (int i = 0; i < 3; ++i) n[i] += __popcll(__ballot(k >= cand[i]));
-    }
+  const Threshold th = find_threshold(len, keep, s_hist, s_red, s_found, [&](auto f) {
+    for (uint32_t j0 = 0; j0 < len; j0 += kSelect) f(j0 + tid < len, j0 + tid < len ? key(j0 + tid) : 0u);
   });
   uint32_t *to = a.moves + size_t(item) * a.half * 2, *from = to + a.half;
   uint32_t seen = 0, holes = 0, movers = 0;
@@ -364,10 +400,11 @@ extern "C" int chpe_paged_evict(const chpe_kv_pages* cache, const int32_t* lens,
   const uint64_t items = uint64_t(cache->rows) * cache->kv_heads;
   const uint32_t parts = std::max(1u, std::min(8u, most / 64));
   if (items * parts > kMaxBlocks) return -1;
-  const bool ok = max_len <= kSelect        ? launch(&k_evict_select<1>, items, kSelect, st, a)
+  const bool ok = max_len == 0              ? launch(&k_evict_select_long, items, kSelect, st, a)  // (lens_out)
+                  : max_len <= kSelect      ? launch(&k_evict_select<1>, items, kSelect, st, a)
                   : max_len <= 4 * kSelect  ? launch(&k_evict_select<4>, items, kSelect, st, a)
                   : max_len <= 16 * kSelect ? launch(&k_evict_select<16>, items, kSelect, st, a)
-                  : max_len <= kLongest     ? launch(&k_evict_select<64>, items, kSelect, st, a)
+                  : max_len <= kLongest     ? launch(&k_evict_select<32>, items, kSelect, st, a)
                                             : launch(&k_evict_select_long, items, kSelect, st, a);
   if (!ok || (most != 0 && !a.fused && !launch(&k_evict_move, items * parts, 256, st, a, parts))) return -3;
   return 0;
