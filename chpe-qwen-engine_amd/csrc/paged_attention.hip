@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
   using Vec = typename P::Vec;
   constexpr int HT = 8 * NT, KS = HD / 32, VD = HD / 16, E = VD < 8 ? 4 : 8, VP = VD / E;
   __shared__ uint64_t s_off[kWaves][2][32];
+  __shared__ Vec s_q[NT][KS][P::kOps][64];  // the query operands, the same for every wave
   __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 32];
   const Place p = place_of<HT>(a);
   if (p.begin >= p.end) return leave_none<HD, HT>(a, p);  // (the whole workgroup)
@@ -233,7 +234,6 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
   rows.next(a, p, t, lane);
 
   // the queries of the columns' heads: dims (G + 4 s) * 8 .. + 7 of head n % 8 of each tile of heads
-  Vec qb[NT][KS][P::kOps];
   float mult[NT], m[NT], l[NT];
   f4_t o[NT][VD];
 #pragma unroll
@@ -263,7 +263,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
       mult[ht] = __builtin_amdgcn_ldexpf(mult[ht], -ex);
     }
 #pragma unroll
-    for (int s = 0; s < KS; ++s) P::split(x[s], second, qb[ht][s]);
+    for (int s = 0; s < KS; ++s) {
+      if (s % kWaves != wave) continue;
+      Vec q[P::kOps];
+      P::split(x[s], second, q);
+#pragma unroll
+      for (int op = 0; op < P::kOps; ++op) s_q[ht][s][op][lane] = q[op];
+    }
     m[ht] = -INFINITY;
     l[ht] = 0.0f;
 #pragma unroll
@@ -277,8 +283,10 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
     load_v(0);
     rows.next(a, p, t + 32 * kWaves, lane);
   }
+  __syncthreads();  // (the query operands)
   for (; t < p.end; t += 32 * kWaves) {
     const bool more = t + 32 * kWaves < p.end;
+    asm volatile("" ::: "memory");  // (the query operands are read from LDS anew: they would fill the registers)
     // scores; the K registers are free after them and take the next tile's rows
     f4_t sc[NT][2];
 #pragma unroll
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int op = 0; op < P::kOps; ++op) acc = P::mfma(__builtin_bit_cast(Vec, kf[u][s]), qb[ht][s][op], acc);
+          for (int op = 0; op < P::kOps; ++op) acc = P::mfma(__builtin_bit_cast(Vec, kf[u][s]), s_q[ht][s][op][lane], acc);
         sc[ht][u] = acc;
       }
     buf ^= 1;
@@ -369,6 +377,7 @@ template <int HD>
 __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
   constexpr int KP = HD / 16, VP = HD / 64, VD = HD / 16;
   __shared__ uint64_t s_off[kWaves][2][16];
+  __shared__ f4_t s_q[KP][64];
   __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 64];
   const Place p = place_of<16>(a);
   if (p.begin >= p.end) return leave_none<HD, 16>(a, p);  // (the whole workgroup)
@@ -391,12 +400,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
     }
   };
   rows.next(a, p, t, lane);
-  float4 q[KP];  // dims (G + 4 c) * 4 .. + 3 of head n
   const bool head = uint32_t(n) < p.nh;
 #pragma unroll
-  for (int c = 0; c < KP; ++c) {
-    q[c] = ld_f4(a.q + p.row * a.q_stride + size_t(p.h0 + (head ? n : 0)) * HD + G * 4 + 16 * c);
-    if (!head) q[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int c = 0; c < KP; ++c) {  // dims (G + 4 c) * 4 .. + 3 of head n
+    if (c % kWaves != wave) continue;
+    const float4 q = ld_f4(a.q + p.row * a.q_stride + size_t(p.h0 + (head ? n : 0)) * HD + G * 4 + 16 * c);
+    s_q[c][lane] = head ? f4_t{q.x, q.y, q.z, q.w} : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   const float mult = a.scale * kLog2e;
   float m = -INFINITY, l = 0.0f;
@@ -411,15 +420,18 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
     load_v(0);
     rows.next(a, p, t + 16 * kWaves, lane);
   }
+  __syncthreads();  // (the queries)
   for (; t < p.end; t += 16 * kWaves) {
     const bool more = t + 16 * kWaves < p.end;
+    asm volatile("" ::: "memory");  // (the queries are read from LDS anew: they would fill the registers)
     f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < KP; ++c) {
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, q[c].x, sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, q[c].y, sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, q[c].z, sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, q[c].w, sc, 0, 0, 0);
+      const f4_t q = s_q[c][lane];
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, q[0], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, q[1], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, q[2], sc, 0, 0, 0);
+      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, q[3], sc, 0, 0, 0);
     }
     buf ^= 1;
     if (more) {
@@ -516,14 +528,21 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
     return;
   }
   const uint32_t b = blockIdx.x - joins, part = b % weight_parts, item = b / weight_parts;
-  const uint32_t kvh = item % a.c.KV, row = item / a.c.KV, gq = a.H / a.c.KV, first = part * 1024;
+  const uint32_t kvh = item % a.c.KV, row = item / a.c.KV, gq = a.H / a.c.KV;
   row_range(a, row, &lo, &len);
-  if (first >= len) return;
+  const uint32_t first = part * 1024, i = first + tid * 4;  // slots lo + i .. + 3
+  const size_t base = (size_t(row) * a.c.KV + kvh) * a.weight_stride;
+  // slots before the window were given nothing
+  for (uint32_t j = first + tid; j < lo; j += weight_parts * 1024)
+    for (uint32_t k = 0; k < 1024 && j + k < lo; k += 256) a.weight_out[base + j + k] = a.weight_in ? a.weight_in[base + j + k] : 0.0f;
+  if (lo + first >= len) return;
   const uint32_t ns = splits_of(a, lo, len);
   __shared__ float s_ml[64][2];
-  float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  f4_t w = {0.0f, 0.0f, 0.0f, 0.0f};
+  const bool in = lo + i < len;
   for (uint32_t g0 = 0; g0 < gq; g0 += 64) {  // 64 query heads at a time
     const uint32_t ng = min(64u, gq - g0);
+    const float* sc = a.scores + (size_t(row) * a.H + kvh * gq + g0) * a.score_stride + (in ? i : 0u);
     __syncthreads();
     for (uint32_t g = wave; g < ng; g += kWaves) {
       float M, L;
@@ -534,22 +553,17 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
       }
     }
     __syncthreads();
+#pragma unroll 8
     for (uint32_t g = 0; g < ng; ++g) {
-      const float* sc = a.scores + (size_t(row) * a.H + kvh * gq + g0 + g) * a.score_stride;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t j = first + k * 256 + tid;
-        if (j >= lo && j < len) w[k] += __builtin_amdgcn_exp2f(gld(sc + (j - lo)) - s_ml[g][0]) * s_ml[g][1];
-      }
+      const float4 s = ld_f4(sc + size_t(g) * a.score_stride);
+      const float M = s_ml[g][0], f = s_ml[g][1];
+      w += f4_t{__builtin_amdgcn_exp2f(s.x - M), __builtin_amdgcn_exp2f(s.y - M), __builtin_amdgcn_exp2f(s.z - M),
+                __builtin_amdgcn_exp2f(s.w - M)} * f;
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t j = first + k * 256 + tid;
-    if (j >= len) continue;
-    const size_t at = (size_t(row) * a.c.KV + kvh) * a.weight_stride + j;
-    a.weight_out[at] = (a.weight_in ? a.weight_in[at] : 0.0f) + w[k];
-  }
+  for (int k = 0; k < 4; ++k)
+    if (lo + i + k < len) a.weight_out[base + lo + i + k] = (a.weight_in ? a.weight_in[base + lo + i + k] : 0.0f) + w[k];
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
