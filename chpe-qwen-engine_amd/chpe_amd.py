@@ -392,22 +392,27 @@ class KvPages:
         self.k, self.v, self.table, self.device = k, v, table, k.device
         self.rows, self.kv_heads, self.page_size, self.head_dim = table.shape[0], k.shape[1], k.shape[2], k.shape[3]
         self.capacity = table.shape[1] * self.page_size
-        self._c = _KvPages(k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[1], k.shape[3], k.shape[2], k.shape[0],
-                           k.stride(0), k.stride(1), k.stride(2), table.data_ptr(), table.shape[0], table.shape[1],
-                           table.stride(0) if table.shape[0] > 1 else table.shape[1])
+        self._c = ctypes.byref(_KvPages(
+            k.data_ptr(), v.data_ptr(), types[k.dtype], k.shape[1], k.shape[3], k.shape[2], k.shape[0], k.stride(0), k.stride(1),
+            k.stride(2), table.data_ptr(), table.shape[0], table.shape[1],
+            table.stride(0) if table.shape[0] > 1 else table.shape[1]))
+        self._f32, self._i32, self._index = torch.float32, torch.int32, k.device.index
+        # (torch.cuda.current_stream builds an object for every call; a step of one token is a few us)
+        self._stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
 
     def _call(self, name, *args):
-        t = self._torch
-        if t.cuda.current_device() != self.device.index:
-            with t.cuda.device(self.device):
+        cuda = self._torch.cuda
+        if cuda.current_device() != self._index:
+            with cuda.device(self._index):
                 return self._call(name, *args)
-        rc = getattr(self.lib, name)(self._c, *args, t.cuda.current_stream(self.device).cuda_stream)
+        rc = getattr(self.lib, name)(self._c, *args, self._stream(self._index))
         if rc:
             raise EngineError(f"{name} failed: {rc}")
 
     def _take(self, t, name, dtype, shape):
         """The address of a contiguous tensor of this type and shape on the cache's device."""
-        if t.dtype != dtype or t.shape != shape or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
             raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}")
         return t.data_ptr()
 
@@ -417,48 +422,55 @@ class KvPages:
             raise ValueError(f"{name}: [rows, kv_heads, at least {least}]")
         return self._take(t, name, dtype, (self.rows, self.kv_heads, t.shape[2]))
 
+    def _heads(self, t, name, tokens, heads):
+        """Address and first two strides of a [tokens, heads, head_dim] f32 tensor whose last stride is 1."""
+        if t.dtype is not self._f32 or t.shape != (tokens, heads, self.head_dim) or t.get_device() != self._index:
+            raise ValueError(f"{name}: [{tokens}, {heads}, {self.head_dim}] f32 on {self.device}")
+        st, sh, sd = t.stride()
+        if heads <= 1:
+            sh = self.head_dim
+        if tokens <= 1:
+            st = heads * sh
+        if sd != 1 and t.numel():
+            raise ValueError(f"{name}: the last stride 1")
+        return t.data_ptr(), st, sh
+
     def append(self, k, v, rows, slots, positions, q=None, q_norm=None, k_norm=None, eps=1e-6, rope=None,
                interleaved=False, q_out=None, slot_pos=None, slot_weight=None):
         """chpe_paged_append: k, v [tokens, kv_heads, head_dim] f32 at slot slots[t] of row rows[t], rotated by
         positions[t] (int32); rope = (cos, sin), each [n, rot_dim / 2].  q [tokens, heads, head_dim] f32 (its
         first two strides free) gives the rotated queries, which are returned (q_out, or a new tensor)."""
-        f32, i32, t = self._torch.float32, self._torch.int32, k.shape[0]
-        for x, name in ((k, "k"), (v, "v")):
-            if x.dtype != f32 or x.shape != (t, self.kv_heads, self.head_dim) or x.device != self.device:
-                raise ValueError(f"{name}: [tokens, {self.kv_heads}, {self.head_dim}] f32 on {self.device}")
-            if t and (x.stride(2) != 1 or (self.kv_heads > 1 and x.stride(1) != self.head_dim)):
-                raise ValueError(f"{name}: contiguous within a token")
-        width = self.kv_heads * self.head_dim
-        heads = qs = qh = qp = qo = 0
+        take, f32, i32, t, hd = self._take, self._f32, self._i32, k.shape[0], self.head_dim
+        kp, ks, kh = self._heads(k, "k", t, self.kv_heads)
+        vp, vs, vh = self._heads(v, "v", t, self.kv_heads)
+        if kh != hd or vh != hd:
+            raise ValueError("k and v: contiguous within a token")
+        heads = qp = qs = qh = qo = 0
         if q is not None:
-            if q.dim() != 3 or q.dtype != f32 or q.shape[0] != t or q.shape[2] != self.head_dim or q.device != self.device:
-                raise ValueError(f"q: [tokens, heads, {self.head_dim}] f32 on {self.device}")
-            if q.numel() and q.stride(2) != 1:
-                raise ValueError("q: the last stride 1")
-            heads, qp = q.shape[1], q.data_ptr()
-            qh = q.stride(1) if heads > 1 else self.head_dim
-            qs = q.stride(0) if t > 1 else heads * qh
+            heads = q.shape[1] if q.dim() == 3 else 0
+            qp, qs, qh = self._heads(q, "q", t, heads)
             if q_out is None:
                 q_out = self._torch.empty(q.shape, dtype=f32, device=self.device)
-            qo = self._take(q_out, "q_out", f32, q.shape)
-        gains = [None if g is None else self._take(g, "a norm's gains", f32, (self.head_dim,)) for g in (q_norm, k_norm)]
+            qo = take(q_out, "q_out", f32, q.shape)
+        gq = None if q_norm is None else take(q_norm, "q_norm", f32, (hd,))
+        gk = None if k_norm is None else take(k_norm, "k_norm", f32, (hd,))
         cos = sin = None
         n = half = 0
         if rope is not None:
-            n, half = rope[0].shape
-            cos, sin = (self._take(x, "rope", f32, (n, half)) for x in rope)
-        idx = [self._take(x, "rows, slots, positions", i32, (t,)) for x in (rows, slots, positions)]
+            shape = rope[0].shape
+            n, half = shape
+            cos, sin = take(rope[0], "rope's cosines", f32, shape), take(rope[1], "rope's sines", f32, shape)
         track, sp, sw = 0, None, None
         if slot_pos is not None:
             sp, track = self._slots(slot_pos, "slot_pos", i32, 1), slot_pos.shape[2]
         if slot_weight is not None:
-            sw = self._slots(slot_weight, "slot_weight", f32, 1)
+            sw = self._slots(slot_weight, "slot_weight", f32, track or 1)
             if track and slot_weight.shape[2] != track:
                 raise ValueError("slot_pos and slot_weight: the same shape")
             track = slot_weight.shape[2]
-        self._call("chpe_paged_append", t, heads, qp, qs, qh, k.data_ptr(), k.stride(0) if t > 1 else width,
-                   v.data_ptr(), v.stride(0) if t > 1 else width, *gains, eps, cos, sin, 2 * half, n, int(interleaved),
-                   *idx, qo, sp, sw, track)
+        self._call("chpe_paged_append", t, heads, qp, qs, qh, kp, ks, vp, vs, gq, gk, eps, cos, sin, 2 * half, n,
+                   1 if interleaved else 0, take(rows, "rows", i32, (t,)), take(slots, "slots", i32, (t,)),
+                   take(positions, "positions", i32, (t,)), qo, sp, sw, track)
         return q_out
 
     def attention_workspace(self, heads, max_len, weights=False):
@@ -472,7 +484,7 @@ class KvPages:
                   workspace=None):
         """chpe_paged_attention: q [rows, heads, head_dim] f32 over the first lens[r] <= max_len slots of row r.
         weight_out [rows, kv_heads, >= max_len] receives weight_in (or 0) plus what each slot was given."""
-        f32 = self._torch.float32
+        f32 = self._f32
         if q.dim() != 3:
             raise ValueError("q: [rows, heads, head_dim]")
         heads, width = q.shape[1], q.shape[1] * self.head_dim
@@ -491,7 +503,7 @@ class KvPages:
         if workspace is None:
             workspace = self._torch.empty(self.attention_workspace(heads, max_len, wo is not None),
                                           dtype=self._torch.uint8, device=self.device)
-        lp = self._take(lens, "lens", self._torch.int32, (self.rows,))
+        lp = self._take(lens, "lens", self._i32, (self.rows,))
         ws = self._take(workspace, "workspace", self._torch.uint8, (workspace.numel(),))
         self._call("chpe_paged_attention", heads, lp, max_len, qp, width,
                    1.0 / self.head_dim ** 0.5 if scale is None else scale, window, op, width, wi, wo, stride, ws,
@@ -509,7 +521,7 @@ class KvPages:
               pos_out=None, slot_src=None, workspace=None):
         """chpe_paged_evict: every row and kv head down to `budget` slots.  lens_out, weight_out and pos_out
         default to the inputs themselves; returns lens_out."""
-        f32, i32 = self._torch.float32, self._torch.int32
+        f32, i32 = self._f32, self._i32
         lens_out, weight_out, pos_out = (i if o is None else o for o, i in
                                          ((lens_out, lens), (weight_out, slot_weight), (pos_out, slot_pos)))
         w = self._slots(slot_weight, "slot_weight", f32, max_len)
