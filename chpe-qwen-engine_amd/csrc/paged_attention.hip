@@ -45,49 +45,55 @@ __device__ __forceinline__ bool row_range(const PagedAttnArgs& a, uint32_t row, 
 // K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
 // The running maximum is in units of log2 (scores times scale * log2 e).
 constexpr int kWaves = 4;
+constexpr uint32_t kMaxSplits = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// 16-bit elements with f32 queries and weights: x is taken apart into parts that the products hold exactly.
-// fp16: two parts, 22 bits, in columns h and h + 8 of one operand; x is brought near 2^14 by a power of two
-// first, so that the second part does not fall below fp16's range.  bf16: three parts, 24 bits, the third in
-// an operand of its own.  Both columns' results are added at the end: no precision of the f32 queries or
-// weights is lost to the cache's type.
-template <class T>
+// 16-bit elements with f32 queries and weights: x is taken apart into parts that the products hold exactly,
+// part p of head h in column h + p * W of the 16; all columns' results are added at the end (sum_parts), so no
+// precision of the f32 queries or weights is lost to the cache's type.  fp16: two parts, 22 bits; x is brought
+// near 2^14 by a power of two first, so that the second part does not fall below fp16's range.  bf16: three
+// parts, 24 bits; of up to 4 heads they fit the 16 columns, of 8 the third is an operand of its own.
+template <class T, int W>
 struct Parts;
 template <>
-struct Parts<_Float16> {
+struct Parts<_Float16, 8> {
   using Vec = h8_t;
   static constexpr int kOps = 1, kScaleExp = 15;  // (weights <= 1 times 2^15)
-  static __device__ void split(const float (&x)[8], bool second, Vec (&out)[1]) {
+  static __device__ void split(const float (&x)[8], int part, Vec (&out)[1]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const _Float16 hi = _Float16(x[e]);
-      out[0][e] = second ? _Float16(x[e] - float(hi)) : hi;
+      out[0][e] = part != 0 ? _Float16(x[e] - float(hi)) : hi;
     }
   }
   static __device__ f4_t mfma(Vec a, Vec b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
-template <>
-struct Parts<Bf16> {
+template <int W>
+struct Parts<Bf16, W> {
   using Vec = b8_t;
-  static constexpr int kOps = 2, kScaleExp = 0;
-  static __device__ void split(const float (&x)[8], bool second, Vec (&out)[2]) {
+  static constexpr int kOps = W == 8 ? 2 : 1, kScaleExp = 0;
+  static __device__ void split(const float (&x)[8], int part, Vec (&out)[kOps]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const __bf16 hi = __bf16(x[e]);
       const float r = x[e] - float(hi);
       const __bf16 mid = __bf16(r);
-      const __bf16 lo = __bf16(r - float(mid));
-      out[0][e] = second ? mid : hi;
-      out[1][e] = second ? __bf16(0.0f) : lo;
+      const __bf16 lo = __bf16(r - float(mid)), zero = __bf16(0.0f);
+      out[0][e] = part == 0 ? hi : part == 1 ? mid : part == 2 ? lo : zero;
+      if constexpr (W == 8) out[1][e] = part == 0 ? lo : zero;
     }
   }
   static __device__ f4_t mfma(Vec a, Vec b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
+template <int W>
+__device__ __forceinline__ float sum_parts(float v) {
+  if constexpr (W == 4) v = pair_sum(v, 4);
+  return pair_sum(v, 8);
+}
 
 // where a workgroup works
 struct Place {
@@ -107,24 +113,35 @@ __device__ __forceinline__ Place place_of(const PagedAttnArgs& a) {
   p.row = b / a.c.KV;
   p.h0 = p.kvh * gq + z * HT;
   p.nh = min(uint32_t(HT), gq - z * HT);
-  p.ok = row_range(a, p.row, &p.lo, &p.len);
-  p.begin = p.lo + p.split * a.chunk;
-  p.end = min(p.len, p.begin + a.chunk);
   return p;
+}
+__device__ __forceinline__ void place_slots(const PagedAttnArgs& a, Place* p) {
+  p->ok = row_range(a, p->row, &p->lo, &p->len);
+  p->begin = p->lo + p->split * a.chunk;
+  p->end = min(p->len, p->begin + a.chunk);
 }
 
 // The tile's row offsets (bytes from k or v): lane r of the wave finds row r's page and leaves the
-// offset in LDS for the lanes that load the row.  `next` requests the table entry ahead of its use.
+// offset in LDS for the lanes that load the row.  `next` requests the table entry ahead of its use; for the
+// first tile of a range that starts at slot 0 it does not wait for the row's length (entries behind it may
+// hold anything).  Rows behind the split's end are its last row.
 template <int ROWS, int ES>
 struct TileRows {
   uint64_t (*s)[ROWS];
-  uint32_t id, slot;
+  uint32_t id = 0, slot = 0;
   bool bad = false;
-  __device__ void next(const PagedAttnArgs& a, const Place& p, uint32_t t, int lane) {
-    slot = min(t + uint32_t(lane % ROWS), p.end - 1);
-    id = uint32_t(gld(a.c.table + size_t(p.row) * a.c.table_stride + (slot >> a.c.shift)));
+  __device__ void next(const PagedAttnArgs& a, uint32_t row, uint32_t t, uint32_t last, int lane) {
+    slot = min(t + uint32_t(lane % ROWS), last);
+    id = uint32_t(gld(a.c.table + size_t(row) * a.c.table_stride + (slot >> a.c.shift)));
   }
   __device__ void put(const PagedAttnArgs& a, const Place& p, int buf, int lane) {
+    // a row behind the end, which `next` did not know yet: the last one's, which is in the tile too
+    const uint32_t first = __builtin_amdgcn_readfirstlane(slot);
+    const uint32_t id_last = uint32_t(__builtin_amdgcn_readlane(int(id), min(p.end - 1 - first, uint32_t(ROWS - 1))));
+    if (slot >= p.end) {
+      slot = p.end - 1;
+      id = id_last;
+    }
     const bool in = id < a.c.n_pages;
     bad |= !in;
     if (lane < ROWS) s[buf][lane] = a.c.at(in ? id : 0u, p.kvh, slot) * ES;
@@ -192,20 +209,22 @@ __device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& 
   for (uint32_t i = threadIdx.x; i < p.nh * HD; i += kWaves * 64) a.out[p.row * a.out_stride + size_t(p.h0) * HD + i] = v;
 }
 
-template <int HD, class T, int NT>
+template <int HD, class T, int W, int NT>
 __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
-  using P = Parts<T>;
+  using P = Parts<T, W>;
   using Vec = typename P::Vec;
-  constexpr int HT = 8 * NT, KS = HD / 32, VD = HD / 16, E = VD < 8 ? 4 : 8, VP = VD / E;
+  constexpr int HT = W * NT, KS = HD / 32, VD = HD / 16, E = VD < 8 ? 4 : 8, VP = VD / E;
   __shared__ uint64_t s_off[kWaves][2][32];
   __shared__ Vec s_q[NT][KS][P::kOps][64];  // the query operands, the same for every wave
-  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 32];
-  const Place p = place_of<HT>(a);
-  if (p.begin >= p.end) return leave_none<HD, HT>(a, p);  // (the whole workgroup)
+  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 4 * W];
+  Place p = place_of<HT>(a);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
-  const bool second = n >= 8;
-
   TileRows<32, 2> rows{s_off[wave]};
+  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 32 * wave, a.c.capacity - 1, lane);
+  place_slots(a, &p);
+  if (p.begin >= p.end) return leave_none<HD, HT>(a, p);  // (the whole workgroup)
+  const int part = n / W, col = n % W;  // the column's part and head
+
   uint32_t t = p.begin + 32 * wave;
   uint4 kf[2][KS], vf[8][VP];
   auto load_k = [&](int buf) {
@@ -231,14 +250,14 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
       }
     }
   };
-  rows.next(a, p, t, lane);
+  if (a.window != 0) rows.next(a, p.row, t, p.end - 1, lane);
 
-  // the queries of the columns' heads: dims (G + 4 s) * 8 .. + 7 of head n % 8 of each tile of heads
+  // the queries of the columns' heads: dims (G + 4 s) * 8 .. + 7 of head n % W of each tile of heads
   float mult[NT], m[NT], l[NT];
   f4_t o[NT][VD];
 #pragma unroll
   for (int ht = 0; ht < NT; ++ht) {
-    const uint32_t h = ht * 8 + (n & 7);
+    const uint32_t h = ht * W + col;
     const float* src = a.q + p.row * a.q_stride + size_t(p.h0 + (h < p.nh ? h : 0)) * HD + G * 8;
     float x[KS][8], top = 0.0f;
 #pragma unroll
@@ -266,7 +285,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
     for (int s = 0; s < KS; ++s) {
       if (s % kWaves != wave) continue;
       Vec q[P::kOps];
-      P::split(x[s], second, q);
+      P::split(x[s], part, q);
 #pragma unroll
       for (int op = 0; op < P::kOps; ++op) s_q[ht][s][op][lane] = q[op];
     }
@@ -281,7 +300,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
     rows.put(a, p, 0, lane);
     load_k(0);
     load_v(0);
-    rows.next(a, p, t + 32 * kWaves, lane);
+    rows.next(a, p.row, t + 32 * kWaves, p.end - 1, lane);
   }
   __syncthreads();  // (the query operands)
   for (; t < p.end; t += 32 * kWaves) {
@@ -304,7 +323,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p, t + 64 * kWaves, lane);
+      rows.next(a, p.row, t + 64 * kWaves, p.end - 1, lane);
     }
     Vec pb[NT][P::kOps];
 #pragma unroll
@@ -313,12 +332,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t j = t + (e >> 2) * 16 + 4 * G + (e & 3);
-        const float s = pair_sum(sc[ht][e >> 2][e & 3], 8) * mult[ht];
+        const float s = sum_parts<W>(sc[ht][e >> 2][e & 3]) * mult[ht];
         s8[e] = j < p.end ? s : -INFINITY;
         mx = fmaxf(mx, s8[e]);
       }
-      if (a.scores && n < 8 && ht * 8 + n < p.nh) {
-        float* d = a.scores + (size_t(p.row) * a.H + p.h0 + ht * 8 + n) * a.score_stride + (t - p.lo) + 4 * G;
+      if (a.scores && part == 0 && ht * W + col < p.nh) {
+        float* d = a.scores + (size_t(p.row) * a.H + p.h0 + ht * W + col) * a.score_stride + (t - p.lo) + 4 * G;
         *reinterpret_cast<float4*>(d) = make_float4(s8[0], s8[1], s8[2], s8[3]);
         *reinterpret_cast<float4*>(d + 16) = make_float4(s8[4], s8[5], s8[6], s8[7]);
       }
@@ -336,7 +355,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
         l[ht] += s8[e];
         s8[e] *= float(1 << P::kScaleExp);
       }
-      P::split(s8, second, pb[ht]);
+      P::split(s8, part, pb[ht]);
     }
 #pragma unroll
     for (int j = 0; j < VD; ++j) {
@@ -366,9 +385,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
 #pragma unroll
     for (int j = 0; j < VD; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[ht][j][i] = pair_sum(o[ht][j][i], 8) * (1.0f / float(1 << P::kScaleExp));
-    join_waves<VD, 32>(s_join, wave, G * 8 + (n & 7), !second, &m[ht], &l[ht], o[ht]);
-    if (wave == 0 && !second && ht * 8 + n < p.nh) leave<HD, VD, E>(a, p, p.h0 + ht * 8 + n, G, m[ht], l[ht], o[ht]);
+      for (int i = 0; i < 4; ++i) o[ht][j][i] = sum_parts<W>(o[ht][j][i]) * (1.0f / float(1 << P::kScaleExp));
+    join_waves<VD, 4 * W>(s_join, wave, G * W + col, part == 0, &m[ht], &l[ht], o[ht]);
+    if (wave == 0 && part == 0 && ht * W + col < p.nh) leave<HD, VD, E>(a, p, p.h0 + ht * W + col, G, m[ht], l[ht], o[ht]);
   }
 }
 
@@ -379,11 +398,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
   __shared__ uint64_t s_off[kWaves][2][16];
   __shared__ f4_t s_q[KP][64];
   __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 64];
-  const Place p = place_of<16>(a);
-  if (p.begin >= p.end) return leave_none<HD, 16>(a, p);  // (the whole workgroup)
+  Place p = place_of<16>(a);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
-
   TileRows<16, 4> rows{s_off[wave]};
+  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 16 * wave, a.c.capacity - 1, lane);
+  place_slots(a, &p);
+  if (p.begin >= p.end) return leave_none<HD, 16>(a, p);  // (the whole workgroup)
+
   uint32_t t = p.begin + 16 * wave;
   float4 kf[KP], vf[4][VP];
   auto load_k = [&](int buf) {
@@ -399,7 +420,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
       for (int c = 0; c < VP; ++c) vf[r][c] = ld_f4(reinterpret_cast<const float*>(src + 256 * c));
     }
   };
-  rows.next(a, p, t, lane);
+  if (a.window != 0) rows.next(a, p.row, t, p.end - 1, lane);
   const bool head = uint32_t(n) < p.nh;
 #pragma unroll
   for (int c = 0; c < KP; ++c) {  // dims (G + 4 c) * 4 .. + 3 of head n
@@ -418,7 +439,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
     rows.put(a, p, 0, lane);
     load_k(0);
     load_v(0);
-    rows.next(a, p, t + 16 * kWaves, lane);
+    rows.next(a, p.row, t + 16 * kWaves, p.end - 1, lane);
   }
   __syncthreads();  // (the queries)
   for (; t < p.end; t += 16 * kWaves) {
@@ -437,7 +458,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p, t + 32 * kWaves, lane);
+      rows.next(a, p.row, t + 32 * kWaves, p.end - 1, lane);
     }
     float s4[4], mx = m;
 #pragma unroll
@@ -485,12 +506,16 @@ __device__ __forceinline__ uint32_t splits_of(const PagedAttnArgs& a, uint32_t l
 
 // maximum and sum over a head's splits, by one wave
 __device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, uint32_t ns, int lane, float* M, float* L) {
-  const float* ml = a.part_ml + size_t(item) * a.splits * 2;
-  float m = -INFINITY, l = 0.0f;
-  for (uint32_t s = lane; s < ns; s += 64) m = fmaxf(m, gld(ml + 2 * s));
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + size_t(item) * a.splits;
+  const uint32_t mine = min(uint32_t(lane), a.splits - 1);
+  float2 x = ml[mine];  // (does not wait for the row's length)
+  if (uint32_t(lane) >= ns) x = make_float2(-INFINITY, 0.0f);
+  float m = x.x;
+  for (uint32_t s = lane + 64; s < ns; s += 64) m = fmaxf(m, ml[s].x);
   m = wave_max(m);
   if (m == -INFINITY) m = 0.0f;  // (no score above -inf)
-  for (uint32_t s = lane; s < ns; s += 64) l += gld(ml + 2 * s + 1) * __builtin_amdgcn_exp2f(gld(ml + 2 * s) - m);
+  float l = x.y * __builtin_amdgcn_exp2f(x.x - m);
+  for (uint32_t s = lane + 64; s < ns; s += 64) l += ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - m);
   *M = m;
   *L = wave_sum(l);
 }
@@ -505,17 +530,32 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
   if (blockIdx.x < joins) {
     const uint32_t item = blockIdx.x, h = item % a.H, row = item / a.H;
     const bool ok = row_range(a, row, &lo, &len);
-    const uint32_t ns = splits_of(a, lo, len);
     __shared__ __align__(16) float s_o[GR][HD];
-    float M, L;
-    join_ml(a, item, ns, lane, &M, &L);  // (every wave for itself)
+    __shared__ float s_f[kMaxSplits];
     const float* ml = a.part_ml + size_t(item) * a.splits * 2;
     const float* acc = a.part_acc + size_t(item) * a.splits * HD + (tid % D4) * 4;
+    // the first sums of every group of threads are requested before the statistics say what they count for
+    constexpr int U = 4;
+    f4_t x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t s = tid / D4 + u * GR;
+      const float4 v = ld_f4(acc + size_t(min(s, a.splits - 1)) * HD);
+      x[u] = f4_t{v.x, v.y, v.z, v.w};
+    }
+    const uint32_t ns = splits_of(a, lo, len);
+    float M, L;
+    join_ml(a, item, ns, lane, &M, &L);  // (every wave for itself)
+    for (uint32_t s = tid; s < ns; s += 256) s_f[s] = __builtin_amdgcn_exp2f(gld(ml + 2 * s) - M);
+    __syncthreads();
     f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (tid / D4 + u * GR < ns) o += x[u] * s_f[tid / D4 + u * GR];
 #pragma unroll 4
-    for (uint32_t s = tid / D4; s < ns; s += GR) {
-      const float4 x = ld_f4(acc + size_t(s) * HD);
-      o += f4_t{x.x, x.y, x.z, x.w} * __builtin_amdgcn_exp2f(gld(ml + 2 * s) - M);
+    for (uint32_t s = tid / D4 + U * GR; s < ns; s += GR) {
+      const float4 v = ld_f4(acc + size_t(s) * HD);
+      o += f4_t{v.x, v.y, v.z, v.w} * s_f[s];
     }
     *reinterpret_cast<f4_t*>(&s_o[tid / D4][(tid % D4) * 4]) = o;
     __syncthreads();
@@ -576,16 +616,18 @@ struct AttnPlan {
   size_t off_acc = 0, off_scores = 0, bytes = 0;
 };
 
-// query heads a workgroup serves: 16 columns, of which two hold one head with a 16-bit cache; two such tiles
-// of heads where the accumulators of both fit the registers
+// query heads a workgroup serves: of the 16 columns one holds a head of an f32 cache, two or (bf16, up to 4
+// heads) four one of a 16-bit cache; two such tiles of heads where the accumulators of both fit the registers
 uint32_t heads_per_group(const chpe_kv_pages* c, uint32_t heads) {
-  return c->type == 0 || (heads / c->kv_heads > 8 && c->head_dim <= 128) ? 16 : 8;
+  const uint32_t gq = heads / c->kv_heads;
+  if (c->type == 0 || (gq > 8 && c->head_dim <= 128)) return 16;
+  return c->type == 2 && gq <= 4 ? 4 : 8;
 }
 
 void split_range(uint64_t groups, uint32_t range, uint32_t step, uint32_t* splits, uint32_t* chunk) {
   const uint64_t n = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step);  // steps in all
   uint64_t want = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(range) + 1023) / 1024);
-  want = std::min<uint64_t>(std::min<uint64_t>(want, n), 512);
+  want = std::min<uint64_t>(std::min<uint64_t>(want, n), kMaxSplits);
   const uint64_t per = (n + want - 1) / want;
   *chunk = uint32_t(per * step);
   *splits = uint32_t((n + per - 1) / per);
@@ -601,7 +643,7 @@ AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uin
   // wanted number bounds
   const uint64_t n = std::max<uint64_t>(1, (uint64_t(max_len) + step - 1) / step);
   uint64_t room = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(max_len) + 1023) / 1024);
-  room = std::min<uint64_t>(std::min<uint64_t>(room, n), 512);
+  room = std::min<uint64_t>(std::min<uint64_t>(room, n), kMaxSplits);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   p.off_acc = up(items * room * 8);
   p.off_scores = p.off_acc + up(items * room * c->head_dim * 4);
@@ -611,20 +653,17 @@ AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uin
 }
 
 template <int HD>
-bool launch_attn(const PagedAttnArgs& a, int type, uint64_t groups, hipStream_t st) {
-  const uint64_t blocks = groups * a.splits;
+bool launch_partial(const PagedAttnArgs& a, int type, uint32_t ht, uint64_t blocks, hipStream_t st) {
   const uint32_t thr = kWaves * 64;
-  bool ok;
-  if (type == 0) ok = launch(&k_paged_32<HD>, blocks, thr, st, a);
-  else if (type == 1) ok = launch(&k_paged_16<HD, _Float16, 1>, blocks, thr, st, a);
-  else ok = launch(&k_paged_16<HD, Bf16, 1>, blocks, thr, st, a);
-  return ok;
-}
-template <int HD>
-bool launch_attn2(const PagedAttnArgs& a, int type, uint64_t groups, hipStream_t st) {  // two tiles of heads
-  const uint64_t blocks = groups * a.splits;
-  return type == 1 ? launch(&k_paged_16<HD, _Float16, 2>, blocks, kWaves * 64, st, a)
-                   : launch(&k_paged_16<HD, Bf16, 2>, blocks, kWaves * 64, st, a);
+  if (type == 0) return launch(&k_paged_32<HD>, blocks, thr, st, a);
+  if (type == 2 && ht == 4) return launch(&k_paged_16<HD, Bf16, 4, 1>, blocks, thr, st, a);
+  if (ht == 8)
+    return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1>, blocks, thr, st, a)
+                     : launch(&k_paged_16<HD, Bf16, 8, 1>, blocks, thr, st, a);
+  if constexpr (HD <= 128)
+    return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2>, blocks, thr, st, a)
+                     : launch(&k_paged_16<HD, Bf16, 8, 2>, blocks, thr, st, a);
+  return false;
 }
 
 bool attn_shape_ok(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len) {
@@ -683,11 +722,10 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   a.score_stride = p.score_stride;
   const int type = cache->type;
   const uint32_t hd = cache->head_dim, ht = heads_per_group(cache, heads);
-  bool ok;
-  if (type != 0 && ht == 16) ok = hd == 64 ? launch_attn2<64>(a, type, p.groups, st) : launch_attn2<128>(a, type, p.groups, st);
-  else ok = hd == 64    ? launch_attn<64>(a, type, p.groups, st)
-            : hd == 128 ? launch_attn<128>(a, type, p.groups, st)
-                        : launch_attn<256>(a, type, p.groups, st);
+  const uint64_t blocks = p.groups * p.splits;
+  bool ok = hd == 64    ? launch_partial<64>(a, type, ht, blocks, st)
+            : hd == 128 ? launch_partial<128>(a, type, ht, blocks, st)
+                        : launch_partial<256>(a, type, ht, blocks, st);
   if (ok && joined != 0)
     ok = hd == 64    ? launch(&k_paged_join<64>, joined, 256, st, a, joins, parts)
          : hd == 128 ? launch(&k_paged_join<128>, joined, 256, st, a, joins, parts)
