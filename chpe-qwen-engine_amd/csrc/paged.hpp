@@ -85,6 +85,24 @@ inline bool launch(void (*kernel)(P...), uint64_t blocks, uint32_t threads, hipS
   return false;
 }
 
+// inclusive prefix sum over the wave on the vector ALU: row_shr 1, 2, 4, 8 within rows of 16 lanes, then the
+// last lane of row 0 / 2 to row 1 / 3 (row_bcast 15) and lane 31 to the upper half (row_bcast 31)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xa, 0xf, false));
+  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xc, 0xf, false));
+  return v;
+}
+// the value of lane `at`, which is the same in all lanes
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int at) { return uint32_t(__builtin_amdgcn_readlane(int(v), at)); }
+
+// a value that is the same in all lanes, as a scalar
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) { return uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)); }
+
 // element types of the cache
 struct Bf16 {
   uint16_t bits;

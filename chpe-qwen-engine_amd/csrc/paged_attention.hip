@@ -1,7 +1,7 @@
 // paged_attention.hip -- chpe_paged_attention: the attention of one new token per row over the paged
 // cache.  s_j = scale q.k_j over the row's slots lo <= j < len, p = softmax(s), out = sum_j p_j v_j, and,
 // for a cache that is kept to a budget, each slot's p summed over the query heads of its kv head.
-// The slots are split over workgroups: each leaves its maximum, sum of 2^(s - max) and so weighted sum of V
+// A row's slots are split over workgroups: each leaves its maximum, sum of 2^(s - max) and so weighted sum of V
 // rows, and a second launch rescales and joins them (and turns the scores into weights).
 #include <algorithm>
 #include <cmath>
@@ -11,6 +11,8 @@
 namespace chpe {
 namespace {
 using namespace dev;
+
+constexpr int kWaves = 4;  // of a workgroup
 
 struct PagedAttnArgs {
   Pages c;
@@ -22,7 +24,8 @@ struct PagedAttnArgs {
   const float* weight_in;
   float* weight_out;
   uint64_t q_stride, out_stride, weight_stride;
-  uint32_t rows, H, max_len, window, splits, chunk, score_stride;
+  uint32_t rows, H, max_len, window, score_stride;
+  uint32_t hz, splits, chunk;     // groups of HT query heads of a kv head; splits of `chunk` slots
   float scale;
 };
 
@@ -34,9 +37,46 @@ __device__ __forceinline__ bool row_range(const PagedAttnArgs& a, uint32_t row, 
   return n <= a.max_len;
 }
 
-// ---- the partial sums of one split -----------------------------------------------------------------------
-// One workgroup of 4 waves per (row, kv head, group of HT query heads, split); wave w takes the tiles w, w + 4,
-// .. of the split.  A tile's scores are S^T = K . Q^T on the matrix cores (rows: slots, columns: query heads),
+// ---- the splits ------------------------------------------------------------------------------------------------
+// a workgroup's place: slots begin .. end - 1 of row `row`, whose range is lo .. len - 1, for query heads
+// h0 .. h0 + nh - 1
+struct Place {
+  uint32_t row, kvh, h0, nh, split, begin, end, lo, len;
+  bool ok;
+};
+template <int HT>
+__device__ __forceinline__ Place place_of(const PagedAttnArgs& a) {
+  Place p;
+  const uint32_t gq = a.H / a.c.KV;
+  uint32_t b = blockIdx.x;
+  // the rows' last splits, which short rows do not have, on other XCDs for other items (workgroup i runs on
+  // XCD i % 8: with 8 splits one XCD had all of them, and f32 rows of up to 2304 slots took 47 us instead of 33)
+  p.split = (b + b / a.splits) % a.splits;
+  b /= a.splits;
+  const uint32_t z = b % a.hz;
+  b /= a.hz;
+  p.kvh = b % a.c.KV;
+  p.row = b / a.c.KV;
+  p.h0 = p.kvh * gq + z * HT;
+  p.nh = min(uint32_t(HT), gq - z * HT);
+  return p;
+}
+__device__ __forceinline__ void place_slots(const PagedAttnArgs& a, Place* p) {
+  p->ok = row_range(a, p->row, &p->lo, &p->len);
+  p->begin = p->lo + p->split * a.chunk;
+  p->end = min(p->len, p->begin + a.chunk);
+}
+// a split without slots: nothing for the join (it goes by the row's length); the output of a row of one
+// split at most
+template <int HD>
+__device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& p) {
+  if (a.splits != 1) return;
+  const float v = p.ok ? 0.0f : __builtin_nanf("");
+  for (uint32_t i = threadIdx.x; i < p.nh * HD; i += kWaves * 64) a.out[p.row * a.out_stride + size_t(p.h0) * HD + i] = v;
+}
+
+// ---- the sums of a split ------------------------------------------------------------------------------------
+// 4 waves; wave w takes the tiles w, w + 4, .. of the split.  A tile's scores are S^T = K . Q^T on the matrix cores (rows: slots, columns: query heads),
 // its output O^T = V^T . P^T (rows: dims, columns: heads): with the heads as columns of both, a lane (G, n) =
 // (lane / 16, lane % 16) keeps the running maximum and sum of column n in scalars of its own, and the result
 // layout of the first product (slots 4 G + i of column n) is the operand layout of the second, so the weights
@@ -44,7 +84,11 @@ __device__ __forceinline__ bool row_range(const PagedAttnArgs& a, uint32_t row, 
 // second is free as long as both operands agree, which is what lets every lane load 16 bytes in a row:
 // K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
 // The running maximum is in units of log2 (scores times scale * log2 e).
-constexpr int kWaves = 4;
+// A wave holds at most 128 dims of a tile's rows and of the accumulators (its registers then allow three waves a
+// SIMD); at head dim 256 two waves share a tile, half of the dims each, and add their scores through LDS.
+constexpr int kWaveDims = 128;
+constexpr int dim_shares(int hd) { return hd > kWaveDims ? hd / kWaveDims : 1; }
+constexpr int tiles_at_once(int hd) { return kWaves / dim_shares(hd); }
 constexpr uint32_t kMaxSplits = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -79,12 +123,9 @@ struct Parts<Bf16, W> {
   static __device__ void split(const float (&x)[8], int part, Vec (&out)[kOps]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const __bf16 hi = __bf16(x[e]);
-      const float r = x[e] - float(hi);
-      const __bf16 mid = __bf16(r);
-      const __bf16 lo = __bf16(r - float(mid)), zero = __bf16(0.0f);
-      out[0][e] = part == 0 ? hi : part == 1 ? mid : part == 2 ? lo : zero;
-      if constexpr (W == 8) out[1][e] = part == 0 ? lo : zero;
+      const float r = x[e] - float(__bf16(x[e])), r2 = r - float(__bf16(r));
+      out[0][e] = __bf16(part == 0 ? x[e] : part == 1 ? r : part == 2 && W == 4 ? r2 : 0.0f);
+      if constexpr (W == 8) out[1][e] = __bf16(part == 0 ? r2 : 0.0f);
     }
   }
   static __device__ f4_t mfma(Vec a, Vec b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -95,32 +136,6 @@ __device__ __forceinline__ float sum_parts(float v) {
   return pair_sum(v, 8);
 }
 
-// where a workgroup works
-struct Place {
-  uint32_t row, kvh, h0, nh, begin, end, lo, len, split;  // query heads h0 .. h0 + nh - 1, slots begin .. end - 1
-  bool ok;
-};
-template <int HT>
-__device__ __forceinline__ Place place_of(const PagedAttnArgs& a) {
-  Place p;
-  const uint32_t gq = a.H / a.c.KV, hz = (gq + HT - 1) / HT;
-  uint32_t b = blockIdx.x;
-  p.split = b % a.splits;
-  b /= a.splits;
-  const uint32_t z = b % hz;
-  b /= hz;
-  p.kvh = b % a.c.KV;
-  p.row = b / a.c.KV;
-  p.h0 = p.kvh * gq + z * HT;
-  p.nh = min(uint32_t(HT), gq - z * HT);
-  return p;
-}
-__device__ __forceinline__ void place_slots(const PagedAttnArgs& a, Place* p) {
-  p->ok = row_range(a, p->row, &p->lo, &p->len);
-  p->begin = p->lo + p->split * a.chunk;
-  p->end = min(p->len, p->begin + a.chunk);
-}
-
 // The tile's row offsets (bytes from k or v): lane r of the wave finds row r's page and leaves the
 // offset in LDS for the lanes that load the row.  `next` requests the table entry ahead of its use; for the
 // first tile of a range that starts at slot 0 it does not wait for the row's length (entries behind it may
@@ -128,16 +143,16 @@ __device__ __forceinline__ void place_slots(const PagedAttnArgs& a, Place* p) {
 template <int ROWS, int ES>
 struct TileRows {
   uint64_t (*s)[ROWS];
-  uint32_t id = 0, slot = 0;
-  bool bad = false;
+  uint32_t id, slot;
+  bool bad;
   __device__ void next(const PagedAttnArgs& a, uint32_t row, uint32_t t, uint32_t last, int lane) {
     slot = min(t + uint32_t(lane % ROWS), last);
     id = uint32_t(gld(a.c.table + size_t(row) * a.c.table_stride + (slot >> a.c.shift)));
   }
   __device__ void put(const PagedAttnArgs& a, const Place& p, int buf, int lane) {
     // a row behind the end, which `next` did not know yet: the last one's, which is in the tile too
-    const uint32_t first = __builtin_amdgcn_readfirstlane(slot);
-    const uint32_t id_last = uint32_t(__builtin_amdgcn_readlane(int(id), min(p.end - 1 - first, uint32_t(ROWS - 1))));
+    const uint32_t first = uniform(slot);
+    const uint32_t id_last = lane_of(id, min(p.end - 1 - first, uint32_t(ROWS - 1)));
     if (slot >= p.end) {
       slot = p.end - 1;
       id = id_last;
@@ -149,88 +164,86 @@ struct TileRows {
   }
 };
 
-// joins waves 1 .. 3 into wave 0: each lane's maximum, sum and N accumulators, through LDS
-template <int N, int LANES>
-__device__ __forceinline__ void join_waves(float* s, int wave, int slot, bool mine, float* m, float* l, f4_t* o) {
+// The split's result from the waves' maxima, sums and accumulators: every wave leaves its own in LDS, then all
+// threads join them, 4 dims of a head at a time, and write them out, for the join or, where a row has one split
+// at most, as the output.  LANES = 4 * columns lanes of a wave hold something, lane
+// slot = G * columns + column; o[j][i] is dim (j / E) * 16 E + (4 G + i) E + j % E of the wave's dims.
+template <int LANES>
+struct WaveSums {
+  f4_t o[kWaves][kWaveDims / 16][LANES];
+  float2 ml[kWaves][LANES / 4];
+};
+template <int HD, int E, int LANES, int VD>
+__device__ __forceinline__ void leave(const PagedAttnArgs& a, const Place& p, WaveSums<LANES>& s, int tid, int wave, int G,
+                                      int col, bool mine, uint32_t head0, float m, float l, const f4_t (&o)[VD]) {
+  constexpr int DS = dim_shares(HD), TW = kWaves / DS, COLS = LANES / 4;
+  if (mine) {
 #pragma unroll
-  for (int half = kWaves / 2; half >= 1; half /= 2) {
-    __syncthreads();
-    if (wave >= half && wave < 2 * half && mine) {
-      float* d = s + (wave - half) * (N * 4 + 4) * LANES;
-#pragma unroll
-      for (int i = 0; i < N; ++i) *reinterpret_cast<f4_t*>(d + (i * LANES + slot) * 4) = o[i];
-      d[N * 4 * LANES + slot] = *m;
-      d[(N * 4 + 1) * LANES + slot] = *l;
+    for (int r = 0; r < VD; ++r) {  // (j / 4) * 4 + i: dims j .. j + 3 of row i
+      const int j = r / 4 * 4, i = r % 4;
+      s.o[wave][r][G * COLS + col] = f4_t{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]};
     }
-    __syncthreads();
-    if (wave < half && mine) {
-      const float* d = s + wave * (N * 4 + 4) * LANES;
-      const float m2 = d[N * 4 * LANES + slot], l2 = d[(N * 4 + 1) * LANES + slot];
-      const float M = fmaxf(*m, m2), base = M == -INFINITY ? 0.0f : M;
-      const float f = __builtin_amdgcn_exp2f(*m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = o[i] * f + *reinterpret_cast<const f4_t*>(d + (i * LANES + slot) * 4) * f2;
-      *l = *l * f + l2 * f2;
-      *m = M;
-    }
+    if (G == 0) s.ml[wave][col] = make_float2(m, l);
   }
-}
-
-// leaves a column's split for the join, or, where the row has one split at most, the output itself.
-// o[j][i] is dim dim_of(j, i) of the column's head.
-template <int HD, int N, int E>
-__device__ __forceinline__ void leave(const PagedAttnArgs& a, const Place& p, uint32_t head, int G, float m, float l,
-                                      const f4_t* o) {
-  const size_t item = size_t(p.row) * a.H + head, pt = item * a.splits + p.split;
-  float* dst = a.part_acc + pt * HD;
-  float f = 1.0f;
-  if (a.splits == 1) {
-    dst = a.out + p.row * a.out_stride + size_t(head) * HD;
-    f = l == 0.0f ? 0.0f : 1.0f / l;
-  }
-  if (G == 0) {
-    a.part_ml[pt * 2] = m;
-    a.part_ml[pt * 2 + 1] = l;
-  }
+  __syncthreads();
+  const int at = tid % LANES, tG = at / COLS;  // (256 is a multiple of LANES)
+  const uint32_t head = head0 + at % COLS;
+  if (head >= p.nh) return;
+  float M = -INFINITY, L = 0.0f, f[TW];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int w = 0; w < TW; ++w) M = fmaxf(M, s.ml[w * DS][at % COLS].x);
+  const float base = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-    for (int j = 0; j < N; j += 4)
-      *reinterpret_cast<float4*>(dst + (j / E) * 16 * E + (4 * G + i) * E + j % E) =
-          make_float4(o[j][i] * f, o[j + 1][i] * f, o[j + 2][i] * f, o[j + 3][i] * f);
-}
-
-// a split without slots: nothing for the join (it goes by the row's length); the output of a row of one
-// split at most
-template <int HD, int HT>
-__device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& p) {
-  if (a.splits != 1) return;
-  const float v = p.ok ? 0.0f : __builtin_nanf("");
-  for (uint32_t i = threadIdx.x; i < p.nh * HD; i += kWaves * 64) a.out[p.row * a.out_stride + size_t(p.h0) * HD + i] = v;
+  for (int w = 0; w < TW; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(s.ml[w * DS][at % COLS].x - base);
+    L += s.ml[w * DS][at % COLS].y * f[w];
+  }
+  const size_t pt = (size_t(p.row) * a.H + p.h0 + head) * a.splits + p.split;
+  const bool whole = a.splits == 1;
+  float* dst = whole ? a.out + p.row * a.out_stride + size_t(p.h0 + head) * HD : a.part_acc + pt * HD;
+  const float g = !whole ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+  if (tid < COLS) reinterpret_cast<float2*>(a.part_ml)[pt] = make_float2(M, L);
+#pragma unroll
+  for (int k = 0; k < (DS * VD * LANES + 255) / 256; ++k) {
+    const int i0 = k * (256 / LANES) + tid / LANES, share = i0 / VD, r = i0 % VD;
+    if (DS * VD * LANES % 256 != 0 && i0 >= DS * VD) break;
+    f4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < TW; ++w) v += s.o[w * DS + share][r][at] * f[w];
+    v *= g;
+    const int j = r / 4 * 4, i = r % 4;
+    *reinterpret_cast<f4_t*>(dst + share * kWaveDims + (j / E) * 16 * E + (4 * tG + i) * E + j % E) = v;
+  }
 }
 
 template <int HD, class T, int W, int NT>
-__global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (HD == 64 ? 3 : 2)) k_paged_16(PagedAttnArgs a) {
   using P = Parts<T, W>;
   using Vec = typename P::Vec;
-  constexpr int HT = W * NT, KS = HD / 32, VD = HD / 16, E = VD < 8 ? 4 : 8, VP = VD / E;
+  constexpr int DS = dim_shares(HD), HW = HD / DS, UNIT = 32 * tiles_at_once(HD);
+  constexpr int HT = W * NT, KS = HW / 32, VD = HW / 16, E = VD < 8 ? 4 : 8;
   __shared__ uint64_t s_off[kWaves][2][32];
-  __shared__ Vec s_q[NT][KS][P::kOps][64];  // the query operands, the same for every wave
-  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 4 * W];
-  Place p = place_of<HT>(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
-  TileRows<32, 2> rows{s_off[wave]};
-  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 32 * wave, a.c.capacity - 1, lane);
-  place_slots(a, &p);
-  if (p.begin >= p.end) return leave_none<HD, HT>(a, p);  // (the whole workgroup)
+  __shared__ Vec s_q[NT][HD / 32][P::kOps][64];  // the query operands, the same for every wave
+  __shared__ float s_mult[HT];
+  // a share's scores for the other one; after the tiles the waves' sums
+  __shared__ union {
+    WaveSums<4 * W> sums;
+    f4_t share[DS > 1 ? 2 * kWaves * NT * 2 * 64 : 1];
+  } s_u;
+  const int wave = uniform(threadIdx.x >> 6), share = wave % DS;
+  const int tid = threadIdx.x, lane = tid & 63, G = lane >> 4, n = lane & 15;
   const int part = n / W, col = n % W;  // the column's part and head
-
-  uint32_t t = p.begin + 32 * wave;
-  uint4 kf[2][KS], vf[8][VP];
+  Place p = place_of<HT>(a);
+  TileRows<32, 2> rows{s_off[wave], 0, 0, false};
+  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 32 * (wave / DS), a.c.capacity - 1, lane);
+  place_slots(a, &p);
+  if (p.begin >= p.end) return leave_none<HD>(a, p);  // (the whole workgroup)
+  uint32_t t = p.begin + 32 * (wave / DS);
+  uint4 kf[2][KS], vf[8];
   auto load_k = [&](int buf) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint8_t* src = a.c.k + rows.s[buf][16 * u + n] + G * 16;
+      const uint8_t* src = a.c.k + rows.s[buf][16 * u + n] + G * 16 + share * (HW * 2);
 #pragma unroll
       for (int s = 0; s < KS; ++s) kf[u][s] = ld_u128(src + 64 * s);
     }
@@ -238,92 +251,108 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
   auto load_v = [&](int buf) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      const uint8_t* src = a.c.v + rows.s[buf][(r >> 2) * 16 + 4 * G + (r & 3)] + n * (2 * E);
-#pragma unroll
-      for (int c = 0; c < VP; ++c) {
-        if constexpr (E == 8) {
-          vf[r][c] = ld_u128(src + 256 * c);
-        } else {
-          const uint2 w = ld_u64(src);
-          vf[r][c] = make_uint4(w.x, w.y, 0, 0);
-        }
+      const uint8_t* src = a.c.v + rows.s[buf][(r >> 2) * 16 + 4 * G + (r & 3)] + n * (2 * E) + share * (HW * 2);
+      if constexpr (E == 8) {
+        vf[r] = ld_u128(src);
+      } else {
+        const uint2 w = ld_u64(src);
+        vf[r] = make_uint4(w.x, w.y, 0, 0);
       }
     }
   };
   if (a.window != 0) rows.next(a, p.row, t, p.end - 1, lane);
-
-  // the queries of the columns' heads: dims (G + 4 s) * 8 .. + 7 of head n % W of each tile of heads
+  // the queries: HD / 8 threads a head take 8 dims each (dims (G + 4 s) * 8 .. + 7 are what lanes of group G
+  // need in step s); they are taken apart while the first tile's rows are on their way
+  constexpr int TH = HD / 8;
+  const int qh = tid / TH, qc = tid % TH;
+  float x[8];
+  if (qh < HT) {
+    const float* src = a.q + p.row * a.q_stride + size_t(p.h0 + (qh < int(p.nh) ? qh : 0)) * HD + qc * 8;
+    const float4 u = ld_f4(src), v = ld_f4(src + 4);
+    const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = w[e];
+  }
+  int buf = 0;
+  if (t < p.end) {
+    rows.put(a, p, 0, lane);
+    load_k(0);
+    load_v(0);
+    rows.next(a, p.row, t + UNIT, p.end - 1, lane);
+  }
+  if (qh < HT) {  // (whole groups of TH lanes)
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (qh >= int(p.nh)) x[e] = 0.0f;
+      top = fmaxf(top, fabsf(x[e]));
+    }
+    int ex = 0;
+    if constexpr (P::kScaleExp != 0) {
+#pragma unroll
+      for (int o = 1; o < TH; o <<= 1) top = pair_max(top, o);
+      if (top > 0.0f && top < INFINITY) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_ldexpf(x[e], ex);
+    }
+    if (qc == 0) s_mult[qh] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -ex);
+#pragma unroll
+    for (int pt = 0; pt < 16 / W; ++pt) {
+      Vec q[P::kOps];
+      P::split(x, pt, q);
+#pragma unroll
+      for (int op = 0; op < P::kOps; ++op) s_q[qh / W][qc / 4][op][(qc % 4) * 16 + pt * W + qh % W] = q[op];
+    }
+  }
+  __syncthreads();  // (the query operands)
   float mult[NT], m[NT], l[NT];
   f4_t o[NT][VD];
 #pragma unroll
   for (int ht = 0; ht < NT; ++ht) {
-    const uint32_t h = ht * W + col;
-    const float* src = a.q + p.row * a.q_stride + size_t(p.h0 + (h < p.nh ? h : 0)) * HD + G * 8;
-    float x[KS][8], top = 0.0f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const float4 u = ld_f4(src + 32 * s), v = ld_f4(src + 32 * s + 4);
-      const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[s][e] = h < p.nh ? w[e] : 0.0f;
-        top = fmaxf(top, fabsf(x[s][e]));
-      }
-    }
-    mult[ht] = a.scale * kLog2e;
-    if constexpr (P::kScaleExp != 0) {
-      top = pair_max(pair_max(top, 16), 32);
-      int ex = 0;
-      if (top > 0.0f && top < INFINITY) ex = 14 - __builtin_amdgcn_frexp_expf(top);
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(x[s][e], ex);
-      mult[ht] = __builtin_amdgcn_ldexpf(mult[ht], -ex);
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (s % kWaves != wave) continue;
-      Vec q[P::kOps];
-      P::split(x[s], part, q);
-#pragma unroll
-      for (int op = 0; op < P::kOps; ++op) s_q[ht][s][op][lane] = q[op];
-    }
+    mult[ht] = s_mult[ht * W + col];
     m[ht] = -INFINITY;
     l[ht] = 0.0f;
 #pragma unroll
     for (int j = 0; j < VD; ++j) o[ht][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  int buf = 0;
-  if (t < p.end) {
-    rows.put(a, p, 0, lane);
-    load_k(0);
-    load_v(0);
-    rows.next(a, p.row, t + 32 * kWaves, p.end - 1, lane);
-  }
-  __syncthreads();  // (the query operands)
-  for (; t < p.end; t += 32 * kWaves) {
-    const bool more = t + 32 * kWaves < p.end;
+  // (where waves share a tile, all waves of the workgroup take the same number of steps)
+  for (uint32_t t0 = p.begin; (DS > 1 ? t0 : t) < p.end; t0 += UNIT, t += UNIT) {
+    const bool here = DS == 1 || t < p.end, more = t + UNIT < p.end;
     asm volatile("" ::: "memory");  // (the query operands are read from LDS anew: they would fill the registers)
     // scores; the K registers are free after them and take the next tile's rows
     f4_t sc[NT][2];
+    if (here) {
 #pragma unroll
-    for (int ht = 0; ht < NT; ++ht)
+      for (int ht = 0; ht < NT; ++ht)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < 2; ++u) {
+          f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+          for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int op = 0; op < P::kOps; ++op) acc = P::mfma(__builtin_bit_cast(Vec, kf[u][s]), s_q[ht][s][op][lane], acc);
-        sc[ht][u] = acc;
-      }
+            for (int op = 0; op < P::kOps; ++op)
+              acc = P::mfma(__builtin_bit_cast(Vec, kf[u][s]), s_q[ht][share * KS + s][op][lane], acc);
+          sc[ht][u] = acc;
+          if constexpr (DS > 1) s_u.share[(((buf * kWaves + wave) * NT + ht) * 2 + u) * 64 + lane] = acc;
+        }
+    }
     buf ^= 1;
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p.row, t + 64 * kWaves, p.end - 1, lane);
+      rows.next(a, p.row, t + 2 * UNIT, p.end - 1, lane);
+    }
+    if constexpr (DS > 1) {
+      // (written anew two steps later, past the next step's barrier)
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      if (!here) continue;
+#pragma unroll
+      for (int ht = 0; ht < NT; ++ht)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sc[ht][u] += s_u.share[((((buf ^ 1) * kWaves + (wave ^ 1)) * NT + ht) * 2 + u) * 64 + lane];
     }
     Vec pb[NT][P::kOps];
 #pragma unroll
@@ -336,7 +365,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
         s8[e] = j < p.end ? s : -INFINITY;
         mx = fmaxf(mx, s8[e]);
       }
-      if (a.scores && part == 0 && ht * W + col < p.nh) {
+      if (a.scores && share == 0 && part == 0 && ht * W + col < p.nh) {
         float* d = a.scores + (size_t(p.row) * a.H + p.h0 + ht * W + col) * a.score_stride + (t - p.lo) + 4 * G;
         *reinterpret_cast<float4*>(d) = make_float4(s8[0], s8[1], s8[2], s8[3]);
         *reinterpret_cast<float4*>(d + 16) = make_float4(s8[4], s8[5], s8[6], s8[7]);
@@ -362,10 +391,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
       uint32_t w[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint4 x = vf[2 * r][j / E], y = vf[2 * r + 1][j / E];
-        const int wi = (j % E) / 2;
-        const uint32_t lo = wi == 0 ? x.x : wi == 1 ? x.y : wi == 2 ? x.z : x.w;
-        const uint32_t hi = wi == 0 ? y.x : wi == 1 ? y.y : wi == 2 ? y.z : y.w;
+        const uint4 x = vf[2 * r], y = vf[2 * r + 1];
+        const uint32_t lo = j / 2 == 0 ? x.x : j / 2 == 1 ? x.y : j / 2 == 2 ? x.z : x.w;
+        const uint32_t hi = j / 2 == 0 ? y.x : j / 2 == 1 ? y.y : j / 2 == 2 ? y.z : y.w;
         w[r] = __builtin_amdgcn_perm(hi, lo, (j & 1) ? 0x07060302u : 0x05040100u);
       }
       const Vec vv = __builtin_bit_cast(Vec, make_uint4(w[0], w[1], w[2], w[3]));
@@ -386,79 +414,96 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_16(PagedAttnArgs a) {
     for (int j = 0; j < VD; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[ht][j][i] = sum_parts<W>(o[ht][j][i]) * (1.0f / float(1 << P::kScaleExp));
-    join_waves<VD, 4 * W>(s_join, wave, G * W + col, part == 0, &m[ht], &l[ht], o[ht]);
-    if (wave == 0 && part == 0 && ht * W + col < p.nh) leave<HD, VD, E>(a, p, p.h0 + ht * W + col, G, m[ht], l[ht], o[ht]);
+    if (ht != 0 || DS > 1) __syncthreads();  // (s_u)
+    leave<HD, E, 4 * W>(a, p, s_u.sums, tid, wave, G, col, part == 0, ht * W, m[ht], l[ht], o[ht]);
   }
 }
 
 // The f32 cache: 16 query heads as columns, tiles of 16 slots, v_mfma_f32_16x16x4f32 (exact f32 products).
 template <int HD>
-__global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
-  constexpr int KP = HD / 16, VP = HD / 64, VD = HD / 16;
+__global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(PagedAttnArgs a) {
+  constexpr int DS = dim_shares(HD), HW = HD / DS, UNIT = 16 * tiles_at_once(HD);
+  constexpr int KP = HW / 16, VP = HW / 64, VD = HW / 16;
   __shared__ uint64_t s_off[kWaves][2][16];
-  __shared__ f4_t s_q[KP][64];
-  __shared__ __align__(16) float s_join[2 * (VD * 4 + 4) * 64];
+  __shared__ f4_t s_q[HD / 16][64];  // dims (G + 4 c) * 4 .. + 3 of head n
+  // a share's scores for the other one; after the tiles the waves' sums
+  __shared__ union {
+    WaveSums<64> sums;
+    f4_t share[DS > 1 ? 2 * kWaves * 64 : 1];
+  } s_u;
+  const int wave = uniform(threadIdx.x >> 6), share = wave % DS;
+  const int tid = threadIdx.x, lane = tid & 63, G = lane >> 4, n = lane & 15;
   Place p = place_of<16>(a);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
-  TileRows<16, 4> rows{s_off[wave]};
-  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 16 * wave, a.c.capacity - 1, lane);
+  TileRows<16, 4> rows{s_off[wave], 0, 0, false};
+  if (a.window == 0) rows.next(a, p.row, p.split * a.chunk + 16 * (wave / DS), a.c.capacity - 1, lane);
   place_slots(a, &p);
-  if (p.begin >= p.end) return leave_none<HD, 16>(a, p);  // (the whole workgroup)
-
-  uint32_t t = p.begin + 16 * wave;
-  float4 kf[KP], vf[4][VP];
+  if (p.begin >= p.end) return leave_none<HD>(a, p);  // (the whole workgroup)
+  uint32_t t = p.begin + 16 * (wave / DS);
+  f4_t kf[KP], vf[4][VP];
   auto load_k = [&](int buf) {
-    const uint8_t* src = a.c.k + rows.s[buf][n] + G * 16;
+    const uint8_t* src = a.c.k + rows.s[buf][n] + G * 16 + share * (HW * 4);
 #pragma unroll
-    for (int c = 0; c < KP; ++c) kf[c] = ld_f4(reinterpret_cast<const float*>(src + 64 * c));
+    for (int c = 0; c < KP; ++c) kf[c] = gld(reinterpret_cast<const f4_t*>(src + 64 * c));
   };
   auto load_v = [&](int buf) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint8_t* src = a.c.v + rows.s[buf][4 * G + r] + n * 16;
+      const uint8_t* src = a.c.v + rows.s[buf][4 * G + r] + n * 16 + share * (HW * 4);
 #pragma unroll
-      for (int c = 0; c < VP; ++c) vf[r][c] = ld_f4(reinterpret_cast<const float*>(src + 256 * c));
+      for (int c = 0; c < VP; ++c) vf[r][c] = gld(reinterpret_cast<const f4_t*>(src + 256 * c));
     }
   };
   if (a.window != 0) rows.next(a, p.row, t, p.end - 1, lane);
   const bool head = uint32_t(n) < p.nh;
+  constexpr int QW = HD / 16 / kWaves;
+  f4_t x[QW];  // the wave's share of the queries
 #pragma unroll
-  for (int c = 0; c < KP; ++c) {  // dims (G + 4 c) * 4 .. + 3 of head n
-    if (c % kWaves != wave) continue;
-    const float4 q = ld_f4(a.q + p.row * a.q_stride + size_t(p.h0 + (head ? n : 0)) * HD + G * 4 + 16 * c);
-    s_q[c][lane] = head ? f4_t{q.x, q.y, q.z, q.w} : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < QW; ++i) {
+    const float4 q = ld_f4(a.q + p.row * a.q_stride + size_t(p.h0 + (head ? n : 0)) * HD + G * 4 + 16 * (i * kWaves + wave));
+    x[i] = f4_t{q.x, q.y, q.z, q.w};
   }
+  int buf = 0;
+  if (t < p.end) {
+    rows.put(a, p, 0, lane);
+    load_k(0);
+    load_v(0);
+    rows.next(a, p.row, t + UNIT, p.end - 1, lane);
+  }
+#pragma unroll
+  for (int i = 0; i < QW; ++i) s_q[i * kWaves + wave][lane] = head ? x[i] : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  __syncthreads();  // (the queries)
   const float mult = a.scale * kLog2e;
   float m = -INFINITY, l = 0.0f;
   f4_t o[VD];
 #pragma unroll
   for (int j = 0; j < VD; ++j) o[j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  int buf = 0;
-  if (t < p.end) {
-    rows.put(a, p, 0, lane);
-    load_k(0);
-    load_v(0);
-    rows.next(a, p.row, t + 16 * kWaves, p.end - 1, lane);
-  }
-  __syncthreads();  // (the queries)
-  for (; t < p.end; t += 16 * kWaves) {
-    const bool more = t + 16 * kWaves < p.end;
+  // (where waves share a tile, all waves of the workgroup take the same number of steps)
+  for (uint32_t t0 = p.begin; (DS > 1 ? t0 : t) < p.end; t0 += UNIT, t += UNIT) {
+    const bool here = DS == 1 || t < p.end, more = t + UNIT < p.end;
     asm volatile("" ::: "memory");  // (the queries are read from LDS anew: they would fill the registers)
     f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (here) {
 #pragma unroll
-    for (int c = 0; c < KP; ++c) {
-      const f4_t q = s_q[c][lane];
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].x, q[0], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].y, q[1], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].z, q[2], sc, 0, 0, 0);
-      sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].w, q[3], sc, 0, 0, 0);
+      for (int c = 0; c < KP; ++c) {
+        const f4_t q = s_q[share * KP + c][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][e], q[e], sc, 0, 0, 0);
+      }
+      if constexpr (DS > 1) s_u.share[(buf * kWaves + wave) * 64 + lane] = sc;
     }
     buf ^= 1;
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p.row, t + 32 * kWaves, p.end - 1, lane);
+      rows.next(a, p.row, t + 2 * UNIT, p.end - 1, lane);
+    }
+    if constexpr (DS > 1) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+      if (!here) continue;
+      sc += s_u.share[((buf ^ 1) * kWaves + (wave ^ 1)) * 64 + lane];
     }
     float s4[4], mx = m;
 #pragma unroll
@@ -466,7 +511,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
       s4[i] = t + 4 * G + i < p.end ? sc[i] * mult : -INFINITY;
       mx = fmaxf(mx, s4[i]);
     }
-    if (a.scores && head)
+    if (a.scores && share == 0 && head)
       *reinterpret_cast<float4*>(a.scores + (size_t(p.row) * a.H + p.h0 + n) * a.score_stride + (t - p.lo) + 4 * G) =
           make_float4(s4[0], s4[1], s4[2], s4[3]);
     mx = pair_max(pair_max(mx, 16), 32);
@@ -483,19 +528,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) k_paged_32(PagedAttnArgs a) {
       l += s4[i];
     }
 #pragma unroll
-    for (int j = 0; j < VD; ++j)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 x = vf[i][j / 4];
-        const float v = j % 4 == 0 ? x.x : j % 4 == 1 ? x.y : j % 4 == 2 ? x.z : x.w;
-        o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s4[i], o[j], 0, 0, 0);
-      }
+      for (int j = 0; j < VD; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][j / 4][j % 4], s4[i], o[j], 0, 0, 0);
     if (more) load_v(buf);
   }
   l = pair_sum(pair_sum(l, 16), 32);
   if (__ballot(rows.bad) != 0) l = __builtin_nanf("");
-  join_waves<VD, 64>(s_join, wave, lane, true, &m, &l, o);
-  if (wave == 0 && head) leave<HD, VD, 4>(a, p, p.h0 + n, G, m, l, o);
+  if (DS > 1) __syncthreads();  // (s_u)
+  leave<HD, 4, 64>(a, p, s_u.sums, tid, wave, G, n, true, 0, m, l, o);
 }
 
 // ---- joining the splits, and the slots' weights -------------------------------------------------------------
@@ -507,8 +548,7 @@ __device__ __forceinline__ uint32_t splits_of(const PagedAttnArgs& a, uint32_t l
 // maximum and sum over a head's splits, by one wave
 __device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, uint32_t ns, int lane, float* M, float* L) {
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + size_t(item) * a.splits;
-  const uint32_t mine = min(uint32_t(lane), a.splits - 1);
-  float2 x = ml[mine];  // (does not wait for the row's length)
+  float2 x = ml[min(uint32_t(lane), a.splits - 1)];  // (does not wait for the row's length)
   if (uint32_t(lane) >= ns) x = make_float2(-INFINITY, 0.0f);
   float m = x.x;
   for (uint32_t s = lane + 64; s < ns; s += 64) m = fmaxf(m, ml[s].x);
@@ -520,7 +560,7 @@ __device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, u
   *L = wave_sum(l);
 }
 
-// blocks 0 .. joins - 1: the output of one (row, head) each, its splits in 256 / (HD / 4) groups;
+// blocks 0 .. joins - 1: the output of one (row, query head) each, 256 / (HD / 4) splits at a time;
 // the others: the weights of 1024 slots of one (row, kv head)
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t joins, uint32_t weight_parts) {
@@ -539,8 +579,7 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
     f4_t x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t s = tid / D4 + u * GR;
-      const float4 v = ld_f4(acc + size_t(min(s, a.splits - 1)) * HD);
+      const float4 v = ld_f4(acc + size_t(min(uint32_t(tid / D4 + u * GR), a.splits - 1)) * HD);
       x[u] = f4_t{v.x, v.y, v.z, v.w};
     }
     const uint32_t ns = splits_of(a, lo, len);
@@ -567,14 +606,13 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
     }
     return;
   }
-  const uint32_t b = blockIdx.x - joins, part = b % weight_parts, item = b / weight_parts;
-  const uint32_t kvh = item % a.c.KV, row = item / a.c.KV, gq = a.H / a.c.KV;
+  const uint32_t b = blockIdx.x - joins, part = b % weight_parts, kv = b / weight_parts;
+  const uint32_t kvh = kv % a.c.KV, row = kv / a.c.KV, gq = a.H / a.c.KV;
   row_range(a, row, &lo, &len);
   const uint32_t first = part * 1024, i = first + tid * 4;  // slots lo + i .. + 3
   const size_t base = (size_t(row) * a.c.KV + kvh) * a.weight_stride;
   // slots before the window were given nothing
-  for (uint32_t j = first + tid; j < lo; j += weight_parts * 1024)
-    for (uint32_t k = 0; k < 1024 && j + k < lo; k += 256) a.weight_out[base + j + k] = a.weight_in ? a.weight_in[base + j + k] : 0.0f;
+  for (uint32_t j = first + tid; j < min(first + 1024, lo); j += 256) a.weight_out[base + j] = a.weight_in ? a.weight_in[base + j] : 0.0f;
   if (lo + first >= len) return;
   const uint32_t ns = splits_of(a, lo, len);
   __shared__ float s_ml[64][2];
@@ -607,48 +645,51 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
-// How the rows are split: a workgroup's slots (`chunk`) are a multiple of its tiles; about 4 workgroups per CU
-// where there are few rows, at most 1024 slots a workgroup where there are many (rows of different lengths
-// then still spread evenly: the chip takes the next workgroup where one ends), at most 512 splits.
-struct AttnPlan {
-  uint32_t splits = 1, chunk = 1, score_stride = 0;
-  uint64_t groups = 0;  // (row, kv head, group of query heads)
-  size_t off_acc = 0, off_scores = 0, bytes = 0;
-};
-
 // query heads a workgroup serves: of the 16 columns one holds a head of an f32 cache, two or (bf16, up to 4
 // heads) four one of a 16-bit cache; two such tiles of heads where the accumulators of both fit the registers
 uint32_t heads_per_group(const chpe_kv_pages* c, uint32_t heads) {
   const uint32_t gq = heads / c->kv_heads;
-  if (c->type == 0 || (gq > 8 && c->head_dim <= 128)) return 16;
+  if (c->type == 0 || (gq > 8 && c->head_dim <= kWaveDims)) return 16;
   return c->type == 2 && gq <= 4 ? 4 : 8;
 }
 
-void split_range(uint64_t groups, uint32_t range, uint32_t step, uint32_t* splits, uint32_t* chunk) {
-  const uint64_t n = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step);  // steps in all
-  uint64_t want = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(range) + 1023) / 1024);
-  want = std::min<uint64_t>(std::min<uint64_t>(want, n), kMaxSplits);
-  const uint64_t per = (n + want - 1) / want;
-  *chunk = uint32_t(per * step);
-  *splits = uint32_t((n + per - 1) / per);
-}
+struct AttnPlan {
+  uint32_t ht = 0, hz = 0, splits = 1, chunk = 1, score_stride = 0;
+  uint64_t blocks = 0;
+  size_t off_acc = 0, off_scores = 0, bytes = 0;
+};
 
+// How the rows are split: into about 1024 workgroups where the rows are few (4 a CU: a long row alone takes
+// 32.6 us over 32771 slots of 4 KB; with 2048 workgroups 34.8), and into splits of at most 512 KB where they
+// are many, so that rows of different lengths keep the chip busy to the end (64 rows of up to 8320 slots: 211 us
+// with 512 KB, 223 with 256 KB).  A row's split depends on max_len and the number of rows,
+// not on the other rows' lengths.  (Dealing all rows' tiles out in equal runs over the workgroups that the chip
+// holds took as long on f32 and 5 to 25 % longer on 16-bit caches: finding the place costs 2 us and the slowest
+// run ends the launch.)
 AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uint32_t window, bool weights) {
   AttnPlan p;
-  const uint32_t gq = heads / c->kv_heads, ht = heads_per_group(c, heads), step = (c->type == 0 ? 16 : 32) * kWaves;
-  p.groups = uint64_t(c->rows) * c->kv_heads * ((gq + ht - 1) / ht);
-  const uint64_t groups = std::max<uint64_t>(1, p.groups), items = uint64_t(c->rows) * heads;
-  split_range(groups, window != 0 && window < max_len ? window : max_len, step, &p.splits, &p.chunk);
-  // the workspace does not depend on the window: room for the most splits of any shorter range, which the
-  // wanted number bounds
-  const uint64_t n = std::max<uint64_t>(1, (uint64_t(max_len) + step - 1) / step);
-  uint64_t room = std::max<uint64_t>((1024 + groups - 1) / groups, (uint64_t(max_len) + 1023) / 1024);
-  room = std::min<uint64_t>(std::min<uint64_t>(room, n), kMaxSplits);
+  const uint32_t gq = heads / c->kv_heads, step = (c->type == 0 ? 16 : 32) * tiles_at_once(c->head_dim);
+  p.ht = heads_per_group(c, heads);
+  p.hz = (gq + p.ht - 1) / p.ht;
+  const uint64_t items = uint64_t(c->rows) * c->kv_heads * p.hz, some = std::max<uint64_t>(1, items);
+  const uint64_t large = (512 << 10) / (2 * c->head_dim * (c->type == 0 ? 4 : 2));  // slots
+  auto most = [&](uint32_t range) {
+    const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step);
+    const uint64_t want = std::max<uint64_t>((1024 + some - 1) / some, (uint64_t(range) + large - 1) / large);
+    return std::min<uint64_t>(std::min<uint64_t>(want, steps), kMaxSplits);
+  };
+  const uint32_t range = window != 0 && window < max_len ? window : max_len;
+  const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step), per = (steps + most(range) - 1) / most(range);
+  p.chunk = uint32_t(per * step);
+  p.splits = uint32_t((steps + per - 1) / per);
+  p.blocks = items * p.splits;
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  p.off_acc = up(items * room * 8);
-  p.off_scores = p.off_acc + up(items * room * c->head_dim * 4);
+  // the workspace does not depend on the window: `most` grows with the range
+  const size_t places = size_t(c->rows) * heads * most(max_len);
+  p.off_acc = up(places * 8);
+  p.off_scores = p.off_acc + up(places * c->head_dim * 4);
   p.score_stride = uint32_t((max_len + 63) / 64 * 64);
-  p.bytes = p.off_scores + (weights ? up(items * p.score_stride * 4) : 0);
+  p.bytes = p.off_scores + (weights ? up(size_t(c->rows) * heads * p.score_stride * 4) : 0);
   return p;
 }
 
@@ -696,9 +737,10 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   if (q_stride % 4 || out_stride % 4 || (cache->rows > 1 && (q_stride < width || out_stride < width))) return -1;
   if ((weight_in && !weight_out) || (weight_out && weight_stride < max_len)) return -1;
   const AttnPlan p = attn_plan(cache, heads, max_len, window, weight_out != nullptr);
-  const uint32_t parts = weight_out ? (max_len + 1023) / 1024 : 0, joins = p.splits > 1 ? cache->rows * heads : 0;
-  const uint64_t joined = uint64_t(joins) + uint64_t(cache->rows) * cache->kv_heads * parts;
-  if (uint64_t(cache->rows) * heads > kMaxBlocks || p.groups * p.splits > kMaxBlocks || joined > kMaxBlocks) return -1;
+  const uint32_t parts = weight_out ? (max_len + 1023) / 1024 : 0;
+  const uint64_t heads_in_all = uint64_t(cache->rows) * heads, joins = p.splits > 1 ? heads_in_all : 0;
+  const uint64_t joined = joins + uint64_t(cache->rows) * cache->kv_heads * parts;
+  if (heads_in_all > kMaxBlocks || p.blocks > kMaxBlocks || joined > kMaxBlocks) return -1;
   if (workspace_bytes < p.bytes) return -2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.q = q;
@@ -716,19 +758,19 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   a.H = heads;
   a.max_len = max_len;
   a.window = window;
+  a.hz = p.hz;
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.scale = scale;
   a.score_stride = p.score_stride;
   const int type = cache->type;
-  const uint32_t hd = cache->head_dim, ht = heads_per_group(cache, heads);
-  const uint64_t blocks = p.groups * p.splits;
-  bool ok = hd == 64    ? launch_partial<64>(a, type, ht, blocks, st)
-            : hd == 128 ? launch_partial<128>(a, type, ht, blocks, st)
-                        : launch_partial<256>(a, type, ht, blocks, st);
+  const uint32_t hd = cache->head_dim;
+  bool ok = hd == 64    ? launch_partial<64>(a, type, p.ht, p.blocks, st)
+            : hd == 128 ? launch_partial<128>(a, type, p.ht, p.blocks, st)
+                        : launch_partial<256>(a, type, p.ht, p.blocks, st);
   if (ok && joined != 0)
-    ok = hd == 64    ? launch(&k_paged_join<64>, joined, 256, st, a, joins, parts)
-         : hd == 128 ? launch(&k_paged_join<128>, joined, 256, st, a, joins, parts)
-                     : launch(&k_paged_join<256>, joined, 256, st, a, joins, parts);
+    ok = hd == 64    ? launch(&k_paged_join<64>, joined, 256, st, a, uint32_t(joins), parts)
+         : hd == 128 ? launch(&k_paged_join<128>, joined, 256, st, a, uint32_t(joins), parts)
+                     : launch(&k_paged_join<256>, joined, 256, st, a, uint32_t(joins), parts);
   return ok ? 0 : -3;
 }

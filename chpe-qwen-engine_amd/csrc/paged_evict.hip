@@ -47,17 +47,6 @@ __device__ __forceinline__ int32_t block_max(int32_t v, int32_t* s) {
   return v;
 }
 
-// inclusive prefix sum over the wave on the vector ALU: row_shr 1, 2, 4, 8 within rows of 16 lanes, then the
-// last lane of row 0 / 2 to row 1 / 3 (row_bcast 15) and lane 31 to the upper half (row_bcast 31)
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x111, 0xf, 0xf, false));
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x112, 0xf, 0xf, false));
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x114, 0xf, 0xf, false));
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x118, 0xf, 0xf, false));
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x142, 0xa, 0xf, false));
-  v += uint32_t(__builtin_amdgcn_update_dpp(0, int(v), 0x143, 0xc, 0xf, false));
-  return v;
-}
 // the sum over the waves before this one, and over all, of what every wave's last lane holds
 __device__ __forceinline__ uint32_t waves_before(uint32_t last, uint32_t* s, uint32_t* all) {
   const uint32_t wave = threadIdx.x >> 6;
