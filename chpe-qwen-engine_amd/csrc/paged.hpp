@@ -99,6 +99,16 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // the value of lane `at`, which is the same in all lanes
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int at) { return uint32_t(__builtin_amdgcn_readlane(int(v), at)); }
 
+// Loads and stores of what a launch touches once and in bulk: keys, values, activations.  Marked as not to be
+// kept, they leave the caches to the rest (1.1 GB read once: 7.1 TB/s, without the mark 6.3).
+template <class T>
+__device__ __forceinline__ T ld_once(const T* p) {
+  return __builtin_nontemporal_load(dev::as_global(p));
+}
+template <class T>
+__device__ __forceinline__ void st_once(T* p, T v) {
+  __builtin_nontemporal_store(v, (__attribute__((address_space(1))) T*)p);
+}
 // a value that is the same in all lanes, as a scalar
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) { return uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)); }

@@ -41,14 +41,14 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, uint32_t par
   uint32_t page = 0;
   const bool writes = turns && row >= 0 && uint32_t(row) < a.rows && slot >= 0 && uint32_t(slot) < a.c.capacity &&
                       a.c.page_of(row, slot, &page);
-  float4 x[U];
-  auto load = [&](uint32_t at, float4& v) {
-    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  f32x4_t x[U];
+  auto load = [&](uint32_t at, f32x4_t& v) {
+    v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= n_rows) return;
     const float* src = at < a.H ? a.q + t * a.q_stride + at * a.q_head_stride
                        : at < a.H + a.c.KV ? a.k + t * a.k_stride + size_t(at - a.H) * HD
                                            : a.v + t * a.v_stride + size_t(at - a.H - a.c.KV) * HD;
-    v = ld_f4(src + d);
+    v = ld_once(reinterpret_cast<const f32x4_t*>(src + d));
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) load(r + u * step, x[u]);
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, uint32_t par
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t at = r + u * step;
-      float4 y = x[u];
+      f32x4_t y = x[u];
       load(at + U * step, x[u]);
       if (at - threadIdx.x / L >= n_rows) return;  // (the whole workgroup)
       const bool is_q = at < a.H, is_v = at >= a.H + a.c.KV;
@@ -87,19 +87,19 @@ __global__ void __launch_bounds__(256) k_paged_append(AppendArgs a, uint32_t par
         for (int o = 1; o < L; o <<= 1) s2 += __shfl_xor(s2, o);
         const float inv = 1.0f / sqrtf(s2 / float(HD) + a.eps);
         const float4 g = is_q ? gq : gk;
-        y = make_float4(y.x * inv * g.x, y.y * inv * g.y, y.z * inv * g.z, y.w * inv * g.w);
+        y = f32x4_t{y.x * inv * g.x, y.y * inv * g.y, y.z * inv * g.z, y.w * inv * g.w};
       }
       if (a.rot != 0) {
         float4 z;  // the pairs' other halves
         if (a.interleaved) z = make_float4(y.y, y.x, y.w, y.z);
         else z = make_float4(__shfl(y.x, other), __shfl(y.y, other), __shfl(y.z, other), __shfl(y.w, other));
         if (in_rot && !is_v)
-          y = make_float4(y.x * cs.x + z.x * sn.x, y.y * cs.y + z.y * sn.y, y.z * cs.z + z.z * sn.z, y.w * cs.w + z.w * sn.w);
+          y = f32x4_t{y.x * cs.x + z.x * sn.x, y.y * cs.y + z.y * sn.y, y.z * cs.z + z.z * sn.z, y.w * cs.w + z.w * sn.w};
       }
       if (at >= n_rows) continue;
       if (is_q) {
         if (!turns) y.x = y.y = y.z = y.w = __builtin_nanf("");
-        *reinterpret_cast<float4*>(a.q_out + (size_t(t) * a.H + at) * HD + d) = y;
+        st_once(reinterpret_cast<f32x4_t*>(a.q_out + (size_t(t) * a.H + at) * HD + d), y);
       } else if (writes) {
         const uint32_t h = is_v ? at - a.H - a.c.KV : at - a.H;
         T* dst = reinterpret_cast<T*>(is_v ? a.c.v : a.c.k) + a.c.at(page, h, slot) + d;

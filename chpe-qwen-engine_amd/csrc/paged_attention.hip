@@ -239,13 +239,13 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
   place_slots(a, &p);
   if (p.begin >= p.end) return leave_none<HD>(a, p);  // (the whole workgroup)
   uint32_t t = p.begin + 32 * (wave / DS);
-  uint4 kf[2][KS], vf[8];
+  u32x4_t kf[2][KS], vf[8];
   auto load_k = [&](int buf) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint8_t* src = a.c.k + rows.s[buf][16 * u + n] + G * 16 + share * (HW * 2);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kf[u][s] = ld_u128(src + 64 * s);
+      for (int s = 0; s < KS; ++s) kf[u][s] = gld(reinterpret_cast<const u32x4_t*>(src + 64 * s));
     }
   };
   auto load_v = [&](int buf) {
@@ -253,10 +253,10 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
     for (int r = 0; r < 8; ++r) {
       const uint8_t* src = a.c.v + rows.s[buf][(r >> 2) * 16 + 4 * G + (r & 3)] + n * (2 * E) + share * (HW * 2);
       if constexpr (E == 8) {
-        vf[r] = ld_u128(src);
+        vf[r] = ld_once(reinterpret_cast<const u32x4_t*>(src));
       } else {
-        const uint2 w = ld_u64(src);
-        vf[r] = make_uint4(w.x, w.y, 0, 0);
+        const u32x2_t w = ld_once(reinterpret_cast<const u32x2_t*>(src));
+        vf[r] = u32x4_t{w.x, w.y, 0, 0};
       }
     }
   };
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
       uint32_t w[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const uint4 x = vf[2 * r], y = vf[2 * r + 1];
+        const u32x4_t x = vf[2 * r], y = vf[2 * r + 1];
         const uint32_t lo = j / 2 == 0 ? x.x : j / 2 == 1 ? x.y : j / 2 == 2 ? x.z : x.w;
         const uint32_t hi = j / 2 == 0 ? y.x : j / 2 == 1 ? y.y : j / 2 == 2 ? y.z : y.w;
         w[r] = __builtin_amdgcn_perm(hi, lo, (j & 1) ? 0x07060302u : 0x05040100u);
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Page
     for (int r = 0; r < 4; ++r) {
       const uint8_t* src = a.c.v + rows.s[buf][4 * G + r] + n * 16 + share * (HW * 4);
 #pragma unroll
-      for (int c = 0; c < VP; ++c) vf[r][c] = gld(reinterpret_cast<const f4_t*>(src + 256 * c));
+      for (int c = 0; c < VP; ++c) vf[r][c] = ld_once(reinterpret_cast<const f4_t*>(src + 256 * c));
     }
   };
   if (a.window != 0) rows.next(a, p.row, t, p.end - 1, lane);

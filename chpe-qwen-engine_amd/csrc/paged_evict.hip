@@ -140,9 +140,10 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, uint32_t row, uint
     uint32_t pd, ps;
     if (!a.c.page_of(row, d, &pd) || !a.c.page_of(row, s, &ps)) continue;
     const size_t od = a.c.at(pd, h, d) * a.elem + lane * 16, os = a.c.at(ps, h, s) * a.elem + lane * 16;
-    const uint4 kk = ld_u128(a.c.k + os), vv = ld_u128(a.c.v + os);
-    *reinterpret_cast<uint4*>(a.c.k + od) = kk;
-    *reinterpret_cast<uint4*>(a.c.v + od) = vv;
+    const u32x4_t kk = ld_once(reinterpret_cast<const u32x4_t*>(a.c.k + os));
+    const u32x4_t vv = ld_once(reinterpret_cast<const u32x4_t*>(a.c.v + os));
+    st_once(reinterpret_cast<u32x4_t*>(a.c.k + od), kk);
+    st_once(reinterpret_cast<u32x4_t*>(a.c.v + od), vv);
   }
 }
 
