@@ -487,6 +487,8 @@ class KvPages:
         f32 = self._f32
         if q.dim() != 3:
             raise ValueError("q: [rows, heads, head_dim]")
+        if max_len < 0 or window < 0:
+            raise ValueError("max_len and window: not negative")
         heads, width = q.shape[1], q.shape[1] * self.head_dim
         qp = self._take(q, "q", f32, (self.rows, heads, self.head_dim))
         if out is None:
@@ -522,6 +524,8 @@ class KvPages:
         """chpe_paged_evict: every row and kv head down to `budget` slots.  lens_out, weight_out and pos_out
         default to the inputs themselves; returns lens_out."""
         f32, i32 = self._f32, self._i32
+        if min(max_len, budget, recent, sinks) < 0:
+            raise ValueError("max_len, budget, recent and sinks: not negative")
         lens_out, weight_out, pos_out = (i if o is None else o for o, i in
                                          ((lens_out, lens), (weight_out, slot_weight), (pos_out, slot_pos)))
         w = self._slots(slot_weight, "slot_weight", f32, max_len)

@@ -23,6 +23,7 @@ struct EvictArgs {
   uint64_t stride;
   uint32_t rows, max_len, budget, recent, sinks, half, fused;
   uint32_t elem, row16;  // bytes of an element; 16-byte pieces of a row
+  uint32_t in_place;     // lens_out is lens: written after the selection, whose workgroups all read the lengths
 };
 
 constexpr int kSelect = 1024, kSelWaves = kSelect / 64;  // threads of the selection
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
   const uint32_t raw = uint32_t(gld(a.lens + row));
   const bool bad = raw > a.max_len;
   const uint32_t len = bad ? 0u : raw, keep = min(len, a.budget);
-  if (tid == 0 && item % a.c.KV == 0) a.lens_out[row] = bad ? int32_t(raw) : int32_t(keep);
+  if (tid == 0 && item % a.c.KV == 0 && !a.in_place) a.lens_out[row] = bad ? int32_t(raw) : int32_t(keep);
   const size_t base = size_t(item) * a.stride;
   const float* weight = a.weight + base;
   const int32_t* pos = a.pos + base;
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kSelect) k_evict_select_long(EvictArgs a) {
   const uint32_t raw = uint32_t(gld(a.lens + row));
   const bool bad = raw > a.max_len;
   const uint32_t len = bad ? 0u : raw, keep = min(len, a.budget);
-  if (tid == 0 && item % a.c.KV == 0) a.lens_out[row] = bad ? int32_t(raw) : int32_t(keep);
+  if (tid == 0 && item % a.c.KV == 0 && !a.in_place) a.lens_out[row] = bad ? int32_t(raw) : int32_t(keep);
   const size_t base = size_t(item) * a.stride;
   const float* weight = a.weight + base;
   const int32_t* pos = a.pos + base;
@@ -330,6 +331,13 @@ __global__ void __launch_bounds__(256) k_evict_move(EvictArgs a, uint32_t parts)
   const uint32_t *to = a.moves + size_t(item) * a.half * 2, *from = to + a.half;
   move_rows(a, item / a.c.KV, item % a.c.KV, to, from, gld(a.n_moves + item), part * per + threadIdx.x / a.row16,
             parts * per, threadIdx.x % a.row16);
+}
+
+__global__ void __launch_bounds__(256) k_evict_lens(EvictArgs a) {
+  const uint32_t row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  const uint32_t len = uint32_t(a.lens_out[row]);
+  if (len <= a.max_len) a.lens_out[row] = int32_t(min(len, a.budget));
 }
 
 size_t evict_bytes(const chpe_kv_pages* c, uint32_t max_len, size_t* off) {
@@ -386,6 +394,7 @@ extern "C" int chpe_paged_evict(const chpe_kv_pages* cache, const int32_t* lens,
   a.row16 = cache->head_dim * a.elem / 16;
   // a (row, kv head) has at most this many moves
   const uint32_t most = max_len > budget ? std::min(budget, max_len - budget) : 0;
+  a.in_place = lens_out == lens ? 1 : 0;
   a.fused = most <= kFusedMoves && max_len <= kLongest ? 1 : 0;
   const uint64_t items = uint64_t(cache->rows) * cache->kv_heads;
   const uint32_t parts = std::max(1u, std::min(8u, most / 64));
@@ -397,5 +406,6 @@ extern "C" int chpe_paged_evict(const chpe_kv_pages* cache, const int32_t* lens,
                   : max_len <= kLongest     ? launch(&k_evict_select<32>, items, kSelect, st, a)
                                             : launch(&k_evict_select_long, items, kSelect, st, a);
   if (!ok || (most != 0 && !a.fused && !launch(&k_evict_move, items * parts, 256, st, a, parts))) return -3;
+  if (a.in_place && max_len > budget && !launch(&k_evict_lens, (cache->rows + 255) / 256, 256, st, a)) return -3;
   return 0;
 }

@@ -237,13 +237,13 @@ typedef struct chpe_kv_pages {
  * token_slot[t] of row token_row[t].  The rotation goes by token_pos[t]: after an eviction the slot is
  * not the position.  q [tokens] rows of q_stride floats, its heads q_head_stride apart (a model with
  * output gates has them between the queries); k, v [tokens][kv_heads][head_dim] in rows of k_stride /
- * v_stride floats; q_out [tokens][heads][head_dim], not overlapping q.  heads 0: no queries.
+ * v_stride floats; q_out [tokens][heads][head_dim], q itself where q has that layout, else not overlapping it.  heads 0: no queries.
  * slot_pos / slot_weight (optional) [rows][kv_heads][track_stride]: receive the position and 0 at the
  * written slot, if it is below track_stride (chpe_paged_evict's inputs).
  * Float arrays at 16-byte boundaries, their strides multiples of 4.  A token whose row is not one of the
  * table's, whose slot is past the row's pages or whose page id is outside the pool is not written (a row
  * of -1 pads a batch); one whose position is outside the tables is not written and its queries are NaN.
- * Two tokens of one call at the same slot of the same row: either may stay.
+ * Two tokens of one call at the same slot of the same row leave a mixture there.
  * Returns 0, -1 bad arguments, -3 device error. */
 int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t heads, const float *q, uint64_t q_stride,
                       uint64_t q_head_stride, const float *k, uint64_t k_stride, const float *v, uint64_t v_stride,
@@ -256,8 +256,8 @@ int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t head
  * the last `window` of them), softmax((q . k) * scale) . V, every head over kv head h / (heads / kv_heads).
  * q and out: `heads` x head_dim floats per row, rows q_stride / out_stride apart.  lens is read on the
  * device; max_len bounds it (and sizes the launch).  A row of length 0 gives zeros; one of a length
- * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN, and so may an
- * infinite value among a head's keys or queries.  What lies in slots outside the range is never used.
+ * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN (in the latter case in its
+ * weights too), and so may an infinite value among a head's keys or queries.  What lies in slots outside the range is never used.
  * weight_out (optional) [rows][kv_heads][weight_stride]: at each slot below the length, weight_in (null:
  * 0) plus the slot's softmax weights summed over the query heads of its kv head; weight_in may be
  * weight_out.  Rows may share pages (a common prefix, or one sequence's drafts as rows of growing length).

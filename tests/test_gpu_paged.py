@@ -109,6 +109,25 @@ def test_attention_layouts(H, KV, hd, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_many_heads_a_kv_head(hd, dtype):
+    """More query heads on one kv head than a workgroup serves, and than the weights' launch takes at a time."""
+    pool = Pool(2, 400, 1, hd, 16, dtype, seed=14)
+    q = torch.randn(2, 130, hd, generator=torch.Generator().manual_seed(14)) * 2
+    check_attention(pool, q, [400, 63], 400, weights=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_attention_does_not_depend_on_the_other_rows(dtype):
+    """A row's bits are the same whatever the other rows' lengths are."""
+    pool = Pool(5, 3000, 2, 128, 16, dtype, seed=15)
+    q = torch.randn(5, 16, 128, generator=torch.Generator().manual_seed(15)).cuda()
+    got = [pool.p.attention(q, dev(np.array([1234, *rest], np.int32)), 3000)[0]
+           for rest in ((0, 0, 0, 0), (3000, 3000, 3000, 3000), (1, 2999, 17, 640))]
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("ps", [1, 2, 8, 64, 256])
 def test_attention_page_sizes_and_orders(ps, dtype):
     """Pages that end inside a tile, one slot a page, and heads as the inner dimension."""
@@ -362,6 +381,18 @@ def test_append(H, KV, hd, rot, norm, inter, gate, tokens, dtype):
     assert torch.equal(sp.cpu(), want_sp) and torch.equal(sw.cpu(), want_sw)
 
 
+def test_append_queries_in_place():
+    pool = Pool(2, 32, 2, 128, 16, "f16", seed=4)
+    g = torch.Generator().manual_seed(4)
+    x, q = torch.randn(50, 2, 128, generator=g).cuda(), torch.randn(50, 7, 128, generator=g).cuda()
+    z = torch.zeros(50, dtype=torch.int32, device="cuda")
+    pos = torch.arange(50, dtype=torch.int32, device="cuda")
+    rope = tuple(t.cuda() for t in rope_tables(64, 96))
+    want = pool.p.append(x, x, z - 1, z, pos, q=q, q_norm=q[0, 0] * 1, rope=rope)
+    gain = q[0, 0] * 1
+    assert pool.p.append(x, x, z - 1, z, pos, q=q, q_norm=gain, rope=rope, q_out=q) is q and torch.equal(q, want)
+
+
 def test_append_roundings_and_special_values():
     """Values, infinities and NaN in the cache's types as torch rounds them; keys unrotated."""
     x = torch.tensor([0.0, -0.0, 1.0, 65504.0, 65519.9, 65520.0, 1e30, -1e30, 3.4e38, 1e-8, 2.98e-8, 6e-8, 1e-40, math.inf,
@@ -491,6 +522,22 @@ def test_evict_ties_and_special_weights():
     check_evict(pool, w, np.full_like(p, 5), [n], n, 350, 1, 0)  # (all of them are the newest: the lowest slots stay)
     check_evict(pool, w, np.full_like(p, -2 ** 31), [n], n, 350, 0, 1)
     check_evict(pool, w, np.where(p % 2, 2 ** 31 - 1, -2 ** 31).astype(np.int32), [n], n, 350, 300, 1)
+
+
+@pytest.mark.parametrize("n,budget", [(70, 66), (300, 150)])
+def test_evict_in_place_over_many_workgroups(n, budget):
+    """lens_out is lens, and a row's heads are spread over more workgroups than the chip holds at once: all of
+    them see the length before the call."""
+    rows, KV = 700, 3
+    pool = Pool(rows, n, KV, 64, 16, "f16", seed=8)
+    w, p = evict_inputs(rows, KV, n, 8)
+    check_evict(pool, w, p, [n] * rows, n, budget, 5, 1, in_place=True)
+
+
+def test_evict_to_nothing_in_place():
+    pool = Pool(300, 33, 2, 64, 16, "bf16", seed=9)
+    w, p = evict_inputs(300, 2, 33, 9)
+    check_evict(pool, w, p, [33] * 299 + [-4], 33, 0, 0, 0, in_place=True)
 
 
 def test_evict_one_slot_of_many():
@@ -692,7 +739,9 @@ def test_python_refusals():
                  lambda: p.append(x, x, lens, lens, lens[:1]), lambda: p.append(x, x, lens, lens, lens, q=q.transpose(1, 2)),
                  lambda: p.append(x, x, lens, lens, lens, q_norm=q[0, 0, :32]),
                  lambda: p.evict(lens, 32, 16, w[..., :31].contiguous(), s), lambda: p.evict(lens, 32, 16, w, s.long()),
-                 lambda: p.evict(lens, 32, 16, w, s, lens_out=lens[:1])):
+                 lambda: p.evict(lens, 32, 16, w, s, lens_out=lens[:1]), lambda: p.evict(lens, 32, -1, w, s),
+                 lambda: p.evict(lens, 32, 16, w, s, recent=-1), lambda: p.attention(q, lens, 32, window=-1),
+                 lambda: p.attention(q, lens, -1)):
         with pytest.raises(ValueError):
             call()
     with pytest.raises(ca.EngineError):
