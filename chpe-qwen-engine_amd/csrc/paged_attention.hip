@@ -357,18 +357,18 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
     Vec pb[NT][P::kOps];
 #pragma unroll
     for (int ht = 0; ht < NT; ++ht) {
-      float s8[8], mx = m[ht];
+      float s8[8], top[8], mx = m[ht];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t j = t + (e >> 2) * 16 + 4 * G + (e & 3);
-        const float s = sum_parts<W>(sc[ht][e >> 2][e & 3]) * mult[ht];
-        s8[e] = j < p.end ? s : -INFINITY;
-        mx = fmaxf(mx, s8[e]);
+        s8[e] = sum_parts<W>(sc[ht][e >> 2][e & 3]);
+        top[e] = j < p.end ? s8[e] * mult[ht] : -INFINITY;
+        mx = fmaxf(mx, top[e]);
       }
       if (a.scores && share == 0 && part == 0 && ht * W + col < p.nh) {
         float* d = a.scores + (size_t(p.row) * a.H + p.h0 + ht * W + col) * a.score_stride + (t - p.lo) + 4 * G;
-        *reinterpret_cast<float4*>(d) = make_float4(s8[0], s8[1], s8[2], s8[3]);
-        *reinterpret_cast<float4*>(d + 16) = make_float4(s8[4], s8[5], s8[6], s8[7]);
+        *reinterpret_cast<float4*>(d) = make_float4(top[0], top[1], top[2], top[3]);
+        *reinterpret_cast<float4*>(d + 16) = make_float4(top[4], top[5], top[6], top[7]);
       }
       mx = pair_max(pair_max(mx, 16), 32);
       const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m[ht] - base);
@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
       m[ht] = mx;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s8[e] = __builtin_amdgcn_exp2f(s8[e] - base);
+        // (the product again inside the fma: rounded once, as small as the difference is)
+        s8[e] = __builtin_amdgcn_exp2f(top[e] > -INFINITY ? fmaf(s8[e], mult[ht], -base) : top[e]);
         l[ht] += s8[e];
         s8[e] *= float(1 << P::kScaleExp);
       }
@@ -484,12 +485,15 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Page
     asm volatile("" ::: "memory");  // (the queries are read from LDS anew: they would fill the registers)
     f4_t sc = {0.0f, 0.0f, 0.0f, 0.0f};
     if (here) {
+      // four sums, added in pairs: one sum of all dims in turn was off by three times as much
+      f4_t part[4] = {sc, sc, sc, sc};
 #pragma unroll
       for (int c = 0; c < KP; ++c) {
         const f4_t q = s_q[share * KP + c][lane];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][e], q[e], sc, 0, 0, 0);
+        for (int e = 0; e < 4; ++e) part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][e], q[e], part[e], 0, 0, 0);
       }
+      sc = (part[0] + part[1]) + (part[2] + part[3]);
       if constexpr (DS > 1) s_u.share[(buf * kWaves + wave) * 64 + lane] = sc;
     }
     buf ^= 1;
@@ -505,15 +509,15 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Page
       if (!here) continue;
       sc += s_u.share[((buf ^ 1) * kWaves + (wave ^ 1)) * 64 + lane];
     }
-    float s4[4], mx = m;
+    float s4[4], top[4], mx = m;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s4[i] = t + 4 * G + i < p.end ? sc[i] * mult : -INFINITY;
-      mx = fmaxf(mx, s4[i]);
+      top[i] = t + 4 * G + i < p.end ? sc[i] * mult : -INFINITY;
+      mx = fmaxf(mx, top[i]);
     }
     if (a.scores && share == 0 && head)
       *reinterpret_cast<float4*>(a.scores + (size_t(p.row) * a.H + p.h0 + n) * a.score_stride + (t - p.lo) + 4 * G) =
-          make_float4(s4[0], s4[1], s4[2], s4[3]);
+          make_float4(top[0], top[1], top[2], top[3]);
     mx = pair_max(pair_max(mx, 16), 32);
     const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - base);
     if (__ballot(f != 1.0f) != 0) {
@@ -524,7 +528,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Page
     m = mx;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s4[i] = __builtin_amdgcn_exp2f(s4[i] - base);
+      s4[i] = __builtin_amdgcn_exp2f(top[i] > -INFINITY ? fmaf(sc[i], mult, -base) : top[i]);
       l += s4[i];
     }
 #pragma unroll
