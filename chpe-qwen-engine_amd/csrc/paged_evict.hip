@@ -28,6 +28,7 @@ struct EvictArgs {
 
 constexpr int kSelect = 1024, kSelWaves = kSelect / 64;  // threads of the selection
 constexpr uint32_t kFusedMoves = 64;                     // at most this many moves: made by the selection itself
+constexpr uint32_t kFew = 8;                             // at most this many slots to drop: one after the other
 
 // the order of the weights as unsigned integers: NaN 0, then -inf .. +inf (-0 as +0)
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -154,6 +155,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, uint32_t row, uint
 template <int KPT>
 __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
   __shared__ uint32_t s_tab[KPT * kSelWaves], s_red[kSelWaves], s_found[3], s_moves[2 * kFusedMoves], s_hist[kBins];
+  __shared__ uint64_t s_least[2][kSelWaves];
   const uint32_t item = blockIdx.x, row = item / a.c.KV, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
   const uint32_t raw = uint32_t(gld(a.lens + row));
@@ -194,34 +196,57 @@ __global__ void __launch_bounds__(kSelect) k_evict_select(EvictArgs a) {
     key[k] = k * kSelect + tid < len ? slot_key(a, wk, pk, newest) : 0u;
   }
 
-  const Threshold th = find_threshold(len, keep, s_hist, s_red, s_found, [&](auto f) {
-#pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      if (uint32_t(k) * kSelect >= len) break;
-      f(k * kSelect + tid < len, key[k]);
-    }
-  });
-
-  // of the keys equal to the threshold the first `ties` slots stay
   uint32_t kept = 0;  // bit k: slot k * kSelect + tid
-#pragma unroll
-  for (int k = 0; k < KPT; ++k)
-    if (k * kSelect + tid < len && key[k] >= th.T) kept |= 1u << k;
   auto is_kept = [&](int k) { return (kept >> k & 1) != 0; };
-  if (!th.all) {
+  if (len - keep <= kFew) {
+    // (the same in all threads.)  A cache that is full drops a slot or a few at every step: one after the other the
+    // slot that goes first, 0.35 us each, where the threshold and the ranks of its ties take 4.5 us
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const uint64_t eq = __ballot(is_kept(k) && key[k] == th.T);
-      if (lane == 0) s_tab[k * kSelWaves + wave] = __popcll(eq);
-    }
-    block_scan(s_tab, KPT * kSelWaves, s_red);
+    for (int k = 0; k < KPT; ++k)
+      if (k * kSelect + tid < len) kept |= 1u << k;
+    for (uint32_t i = 0; i < len - keep; ++i) {
+      uint64_t least = ~uint64_t(0);  // (the key, then the higher slot first)
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const bool eq = is_kept(k) && key[k] == th.T;
-      const uint32_t rank = s_tab[k * kSelWaves + wave] + below(__ballot(eq), lane);
-      if (eq && rank >= th.ties) kept &= ~(1u << k);
+      for (int k = 0; k < KPT; ++k)
+        if (is_kept(k)) least = min(least, uint64_t(key[k]) << 32 | ~(k * kSelect + tid));
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1)
+        least = min(least, uint64_t(pair_u(uint32_t(least >> 32), o)) << 32 | pair_u(uint32_t(least), o));
+      if (lane == 0) s_least[i & 1][wave] = least;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kSelWaves; ++w) least = min(least, s_least[i & 1][w]);
+      const uint32_t slot = ~uint32_t(least);
+      if (slot % kSelect == tid) kept &= ~(1u << slot / kSelect);
     }
-    __syncthreads();
+  } else {
+    const Threshold th = find_threshold(len, keep, s_hist, s_red, s_found, [&](auto f) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) {
+        if (uint32_t(k) * kSelect >= len) break;
+        f(k * kSelect + tid < len, key[k]);
+      }
+    });
+
+    // of the keys equal to the threshold the first `ties` slots stay
+#pragma unroll
+    for (int k = 0; k < KPT; ++k)
+      if (k * kSelect + tid < len && key[k] >= th.T) kept |= 1u << k;
+    if (!th.all) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) {
+        const uint64_t eq = __ballot(is_kept(k) && key[k] == th.T);
+        if (lane == 0) s_tab[k * kSelWaves + wave] = __popcll(eq);
+      }
+      block_scan(s_tab, KPT * kSelWaves, s_red);
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) {
+        const bool eq = is_kept(k) && key[k] == th.T;
+        const uint32_t rank = s_tab[k * kSelWaves + wave] + below(__ballot(eq), lane);
+        if (eq && rank >= th.ties) kept &= ~(1u << k);
+      }
+      __syncthreads();
+    }
   }
   // holes in the lower, movers in the upper half of a count (either is at most half of kLongest)
 #pragma unroll

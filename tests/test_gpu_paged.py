@@ -540,6 +540,20 @@ def test_evict_to_nothing_in_place():
     check_evict(pool, w, p, [33] * 299 + [-4], 33, 0, 0, 0, in_place=True)
 
 
+@pytest.mark.parametrize("n", [9, 64, 1000, 1024, 1025, 4097, 17000])
+def test_evict_a_few(n):
+    """One to ten slots go: the smallest weights, their ties from the highest slot on, protected ones last."""
+    pool = Pool(2, n, 3, 64, 16, "bf16", seed=n)
+    w, p = evict_inputs(2, 3, n, n, zeros=0.3)
+    w[:, 1] = np.random.default_rng(n).choice(np.array([math.nan, -1.0, -0.0, 0.0, math.inf, -math.inf], np.float32), (2, n))
+    w[1, 2] = 1.0
+    for drop in range(1, 11):
+        if drop < n:
+            check_evict(pool, w, p, [n, max(0, n - 3)], n, n - drop, min(3, n - drop), 0)
+    check_evict(pool, w, np.full_like(p, 7), [n, n], n, n - 4, 1, 0)  # (every position the newest: the highest slots go)
+    check_evict(pool, w, np.full_like(p, 7), [n, n - 1], n, n - 8, 0, 0)
+
+
 def test_evict_one_slot_of_many():
     """Every step of a full cache: the one that goes, wherever it is."""
     n = 2049
