@@ -51,7 +51,7 @@ inline bool pages_from(const chpe_kv_pages* c, Pages* out) {
   uint64_t extent = c->head_dim;
   for (int i = 0; i < 3; ++i) {
     if (n[i] == 1) continue;
-    if (st[i] < extent || st[i] % per16 != 0 || st[i] > (uint64_t(1) << 40)) return false;
+    if (st[i] < extent || st[i] % per16 != 0 || st[i] > (uint64_t(1) << 60) / n[i]) return false;
     extent = st[i] * n[i];
   }
   int shift = 0;
@@ -64,7 +64,7 @@ inline bool pages_from(const chpe_kv_pages* c, Pages* out) {
 
 // false for a stream of another device than the current one, whose kernels would run there
 inline bool stream_here(hipStream_t st) {
-  if (st == nullptr || st == hipStreamPerThread) return true;
+  if (st == nullptr || st == hipStreamLegacy || st == hipStreamPerThread) return true;
   int cur = 0;
   hipDevice_t dev = 0;
   if (hipGetDevice(&cur) == hipSuccess && hipStreamGetDevice(st, &dev) == hipSuccess) return dev == cur;

@@ -25,6 +25,7 @@ BAD_PAGES = [
     dict(head_stride=1024),                    # heads in each other's slots
     dict(page_stride=8192),                    # pages in each other
     dict(slot_stride=132, head_stride=132 * 16, page_stride=132 * 128),  # rows that start between 16-byte boundaries
+    dict(page_stride=1 << 62), dict(head_stride=(1 << 64) - 8, page_stride=2048),
     dict(page_size=1 << 20, pages_per_row=4096, table_stride=4096, head_stride=128 << 20, page_stride=1024 << 20),
 ]
 
