@@ -9,7 +9,6 @@ Tolerances count roundings to f32 (u = 2^-24 relative) in the worst case, no two
   count 16 u) and the divisions, all relative; the output by that times sum p |v|.
 * the norm of hd dims is off by (hd / 2 + 8) u relative, a rotation by 3 u of |x0| + |x1|; a cached key by
   half a step of its type more."""
-import ctypes
 import math
 
 import numpy as np
@@ -713,6 +712,48 @@ def test_graph_of_a_step():
         assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
         junk = torch.randn(1 << 20, device="cuda").sum()  # eager work between the replays
         assert torch.isfinite(junk)
+
+
+def test_two_graphs_one_workspace():
+    """Graphs of other sizes that use one workspace, replayed in turn."""
+    pools = [Pool(4, 2000, 2, 128, 16, "f16", seed=21), Pool(1, 700, 4, 64, 32, "bf16", seed=22)]
+    qs = [torch.randn(4, 16, 128, generator=torch.Generator().manual_seed(21)).cuda(),
+          torch.randn(1, 12, 64, generator=torch.Generator().manual_seed(22)).cuda()]
+    lens = [dev(np.array([2000, 3, 0, 1111], np.int32)), dev(np.array([700], np.int32))]
+    tops = (2000, 700)
+    ws = torch.zeros(max(p.p.attention_workspace(q.shape[1], n, True) for p, q, n in zip(pools, qs, tops)),
+                     dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros_like(q) for q in qs]
+    gots = [torch.zeros(p.p.rows, p.p.kv_heads, n, device="cuda") for p, n in zip(pools, tops)]
+    wants = [torch.zeros_like(w) for w in gots]
+    want = [p.p.attention(q, n, t, weight_out=w) for p, q, n, t, w in zip(pools, qs, lens, tops, wants)]
+    graphs = []
+    for p, q, n, t, o, w in zip(pools, qs, lens, tops, outs, gots):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            p.p.attention(q, n, t, out=o, weight_out=w, workspace=ws)
+    for i in (0, 1, 0, 0, 1, 1, 0):
+        outs[i].fill_(5.0)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i]) and torch.equal(gots[i], wants[i])
+
+
+def test_stream_handles():
+    """The default stream by its handles, and a stream that is none of torch's current ones."""
+    lib, pool = ca.load_engine_lib(), Pool(2, 64, 2, 64, 16, "f32", seed=23)
+    x = torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(23)).cuda()
+    row, slot = dev(np.array([0, 1], np.int32)), dev(np.array([5, 60], np.int32))
+    for i, stream in enumerate((None, 1, 2, torch.cuda.Stream().cuda_stream)):
+        torch.cuda.synchronize()
+        y = x * (i + 2)
+        torch.cuda.synchronize()
+        rc = lib.chpe_paged_append(pool.p._c, 2, 0, None, 0, 0, y.data_ptr(), 128, y.data_ptr(), 128, None, None, 1e-6, None,
+                                   None, 0, 0, 0, row.data_ptr(), slot.data_ptr(), slot.data_ptr(), None, None, None, 0, stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        for r, s in ((0, 5), (1, 60)):
+            assert torch.equal(pool.k[int(pool.table[r, s // 16]), :, s % 16], y[r])
 
 
 def test_workspace_content_does_not_matter():
