@@ -76,14 +76,17 @@ __device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& 
 }
 
 // ---- the sums of a split ------------------------------------------------------------------------------------
-// 4 waves; wave w takes the tiles w, w + 4, .. of the split.  A tile's scores are S^T = K . Q^T on the matrix cores (rows: slots, columns: query heads),
-// its output O^T = V^T . P^T (rows: dims, columns: heads): with the heads as columns of both, a lane (G, n) =
-// (lane / 16, lane % 16) keeps the running maximum and sum of column n in scalars of its own, and the result
-// layout of the first product (slots 4 G + i of column n) is the operand layout of the second, so the weights
-// never leave the registers.  The order of the dims inside the first product and of the slots inside the
-// second is free as long as both operands agree, which is what lets every lane load 16 bytes in a row:
-// K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
+// 4 waves; wave w takes the tiles w, w + 4, .. of the split.  A tile's scores are S^T = K . Q^T on the matrix
+// cores (rows: slots, columns: query heads), its output O^T = V^T . P^T (rows: dims, columns: heads): with the
+// heads as columns of both, a lane (G, n) = (lane / 16, lane % 16) keeps the running maximum and sum of column n
+// in scalars of its own, and the result layout of the first product (slots 4 G + i of column n) is the operand
+// layout of the second, so the weights never leave the registers.  The order of the dims inside the first product
+// and of the slots inside the second is free as long as both operands agree, which is what lets every lane load
+// 16 bytes in a row: K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
 // The running maximum is in units of log2 (scores times scale * log2 e).
+// Bound by memory: each K and V row is read once, the next tile's K rows while the weights are formed, its V rows
+// while the scores are.  64 rows of 8320 slots with 8 kv heads of 128 (2.2 GB, fp16 or bf16) take 370 us with the
+// join, 5.9 TB/s, as do 32 such rows in f32; plain reads of the card reach 6.3.
 // A wave holds at most 128 dims of a tile's rows and of the accumulators (its registers then allow three waves a
 // SIMD); at head dim 256 two waves share a tile, half of the dims each, and add their scores through LDS.
 constexpr int kWaveDims = 128;
@@ -420,7 +423,9 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
   }
 }
 
-// The f32 cache: 16 query heads as columns, tiles of 16 slots, v_mfma_f32_16x16x4f32 (exact f32 products).
+// The same for the f32 cache: 16 query heads as columns, tiles of 16 slots, v_mfma_f32_16x16x4f32 (exact f32
+// products).  The order of the second product's loops is the one that compiles right: with the four slots of a
+// lane inside, the compiler put a result over V values that were still to be read.
 template <int HD>
 __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(PagedAttnArgs a) {
   constexpr int DS = dim_shares(HD), HW = HD / DS, UNIT = 16 * tiles_at_once(HD);
@@ -564,6 +569,8 @@ __device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, u
   *L = wave_sum(l);
 }
 
+// Bound by latency: the lengths, the statistics and the sums, one after the other (64 heads of 86 splits 4.8 us,
+// 4096 heads of 9 splits 9.6 us; with the weights of 24 rows of up to 4097 slots 8.7 us).
 // blocks 0 .. joins - 1: the output of one (row, query head) each, 256 / (HD / 4) splits at a time;
 // the others: the weights of 1024 slots of one (row, kv head)
 template <int HD>
@@ -664,10 +671,10 @@ struct AttnPlan {
 };
 
 // How the rows are split: into about 1024 workgroups where the rows are few (4 a CU: a long row alone takes
-// 32.6 us over 32771 slots of 4 KB; with 2048 workgroups 34.8), and into splits of at most 512 KB where they
-// are many, so that rows of different lengths keep the chip busy to the end (64 rows of up to 8320 slots: 211 us
-// with 512 KB, 223 with 256 KB).  A row's split depends on max_len and the number of rows,
-// not on the other rows' lengths.  (Dealing all rows' tiles out in equal runs over the workgroups that the chip
+// 28.6 us over 32771 slots of 4 KB; with 1536 workgroups 30.8), and into splits of at most 512 KB where they
+// are many, so that rows of different lengths keep the chip busy to the end (64 rows of up to 8320 slots: 205 us
+// with 512 KB, 200 with 768 KB, 235 with 256 KB).  A row's split depends on max_len and the number of rows, not
+// on the other rows' lengths.  (Dealing all rows' tiles out in equal runs over the workgroups that the chip
 // holds took as long on f32 and 5 to 25 % longer on 16-bit caches: finding the place costs 2 us and the slowest
 // run ends the launch.)
 AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uint32_t window, bool weights) {

@@ -253,7 +253,8 @@ int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t head
                       float *slot_weight, uint64_t track_stride, void *stream);
 
 /* The attention of one new token per row: row r's query heads over its slots 0 .. lens[r] - 1 (window > 0:
- * the last `window` of them, by slot: after an eviction that is not the order of their positions), softmax((q . k) * scale) . V, every head over kv head h / (heads / kv_heads).
+ * the last `window` of them, by slot: after an eviction that is not the order of their positions),
+ * softmax((q . k) * scale) . V, every head over kv head h / (heads / kv_heads).
  * q and out: `heads` x head_dim floats per row, rows q_stride / out_stride apart.  lens is read on the
  * device; max_len bounds it (and sizes the launch).  A row of length 0 gives zeros; one of a length
  * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN (in the latter case in its
