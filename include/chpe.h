@@ -237,7 +237,8 @@ typedef struct chpe_kv_pages {
  * token_slot[t] of row token_row[t].  The rotation goes by token_pos[t]: after an eviction the slot is
  * not the position.  q [tokens] rows of q_stride floats, its heads q_head_stride apart (a model with
  * output gates has them between the queries); k, v [tokens][kv_heads][head_dim] in rows of k_stride /
- * v_stride floats; q_out [tokens][heads][head_dim], q itself where q has that layout, else not overlapping it.  heads 0: no queries.
+ * v_stride floats; q_out [tokens][heads][head_dim], q itself where q has that layout, else not
+ * overlapping it.  heads 0: no queries.
  * slot_pos / slot_weight (optional) [rows][kv_heads][track_stride]: receive the position and 0 at the
  * written slot, if it is below track_stride (chpe_paged_evict's inputs).
  * Float arrays at 16-byte boundaries, their strides multiples of 4.  A token whose row is not one of the
@@ -258,7 +259,8 @@ int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t head
  * q and out: `heads` x head_dim floats per row, rows q_stride / out_stride apart.  lens is read on the
  * device; max_len bounds it (and sizes the launch).  A row of length 0 gives zeros; one of a length
  * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN (in the latter case in its
- * weights too), and so may an infinite value among a head's keys or queries.  What lies in slots outside the range is never used.
+ * weights too), and so may an infinite value among a head's keys or queries.  What lies in slots outside the
+ * range is never used.
  * weight_out (optional) [rows][kv_heads][weight_stride]: at each slot below the length, weight_in (null:
  * 0) plus the slot's softmax weights summed over the query heads of its kv head; weight_in may be
  * weight_out.  Rows may share pages (a common prefix, or one sequence's drafts as rows of growing length).
