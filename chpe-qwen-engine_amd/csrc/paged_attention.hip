@@ -167,6 +167,32 @@ struct TileRows {
   }
 };
 
+// An infinite V element makes its dim's sum infinite whatever its slot's weight, but the products give NaN where
+// they meet it with a 0: a padding row's weight, a part of a weight that has no bits left, a weight that 32 bits
+// hold as 0.  So a sum of dims dim .. dim + 3 that came out infinite or NaN is told again from the split's values
+// that are not finite themselves: their sum, or v where there are none (a sum past f32's range).
+__device__ __forceinline__ bool all_finite(f4_t v) {
+  return fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
+}
+template <class T>
+__device__ __forceinline__ f4_t non_finite_sum(const PagedAttnArgs& a, const Place& p, uint32_t dim, f4_t v) {
+  f4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t j = p.begin; j < p.end; ++j) {
+    uint32_t page;
+    a.c.page_of(p.row, j, &page);  // (a bad one: the head's sum of weights is NaN and nothing comes here)
+    const T* src = reinterpret_cast<const T*>(a.c.v) + a.c.at(page, p.kvh, j) + dim;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = Elem<T>::get(src + e);
+      s[e] += fabsf(x) < INFINITY ? 0.0f : x;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = s[e] == 0.0f ? v[e] : s[e];
+  return v;
+}
+
 // The split's result from the waves' maxima, sums and accumulators: every wave leaves its own in LDS, then all
 // threads join them, 4 dims of a head at a time, and write them out, for the join or, where a row has one split
 // at most, as the output.  LANES = 4 * columns lanes of a wave hold something, lane
@@ -176,7 +202,7 @@ struct WaveSums {
   f4_t o[kWaves][kWaveDims / 16][LANES];
   float2 ml[kWaves][LANES / 4];
 };
-template <int HD, int E, int LANES, int VD>
+template <int HD, class T, int E, int LANES, int VD>
 __device__ __forceinline__ void leave(const PagedAttnArgs& a, const Place& p, WaveSums<LANES>& s, int tid, int wave, int G,
                                       int col, bool mine, uint32_t head0, float m, float l, const f4_t (&o)[VD]) {
   constexpr int DS = dim_shares(HD), TW = kWaves / DS, COLS = LANES / 4;
@@ -206,16 +232,32 @@ __device__ __forceinline__ void leave(const PagedAttnArgs& a, const Place& p, Wa
   float* dst = whole ? a.out + p.row * a.out_stride + size_t(p.h0 + head) * HD : a.part_acc + pt * HD;
   const float g = !whole ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
   if (tid < COLS) reinterpret_cast<float2*>(a.part_ml)[pt] = make_float2(M, L);
+  constexpr int PIECES = (DS * VD * LANES + 255) / 256;
+  // piece k of a thread: 4 dims from this one on
+  auto dim_of = [&](int k) {
+    const int i0 = k * (256 / LANES) + tid / LANES, r = i0 % VD, j = r / 4 * 4, i = r % 4;
+    return i0 / VD * kWaveDims + (j / E) * 16 * E + (4 * tG + i) * E + j % E;
+  };
+  auto none = [&](int k) { return DS * VD * LANES % 256 != 0 && k * (256 / LANES) + tid / LANES >= DS * VD; };
+  bool finite = true;
 #pragma unroll
-  for (int k = 0; k < (DS * VD * LANES + 255) / 256; ++k) {
+  for (int k = 0; k < PIECES; ++k) {
     const int i0 = k * (256 / LANES) + tid / LANES, share = i0 / VD, r = i0 % VD;
-    if (DS * VD * LANES % 256 != 0 && i0 >= DS * VD) break;
+    if (none(k)) break;
     f4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < TW; ++w) v += s.o[w * DS + share][r][at] * f[w];
     v *= g;
-    const int j = r / 4 * 4, i = r % 4;
-    *reinterpret_cast<f4_t*>(dst + share * kWaveDims + (j / E) * 16 * E + (4 * tG + i) * E + j % E) = v;
+    finite &= all_finite(v);
+    *reinterpret_cast<f4_t*>(dst + dim_of(k)) = v;
+  }
+  if (finite || L != L) return;
+#pragma unroll 1
+  for (int k = 0; k < PIECES; ++k) {
+    if (none(k)) break;
+    f4_t* d = reinterpret_cast<f4_t*>(dst + dim_of(k));
+    const f4_t v = *d;
+    if (!all_finite(v)) *d = non_finite_sum<T>(a, p, dim_of(k), v);
   }
 }
 
@@ -419,7 +461,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[ht][j][i] = sum_parts<W>(o[ht][j][i]) * (1.0f / float(1 << P::kScaleExp));
     if (ht != 0 || DS > 1) __syncthreads();  // (s_u)
-    leave<HD, E, 4 * W>(a, p, s_u.sums, tid, wave, G, col, part == 0, ht * W, m[ht], l[ht], o[ht]);
+    leave<HD, T, E, 4 * W>(a, p, s_u.sums, tid, wave, G, col, part == 0, ht * W, m[ht], l[ht], o[ht]);
   }
 }
 
@@ -545,7 +587,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Page
   l = pair_sum(pair_sum(l, 16), 32);
   if (__ballot(rows.bad) != 0) l = __builtin_nanf("");
   if (DS > 1) __syncthreads();  // (s_u)
-  leave<HD, 4, 64>(a, p, s_u.sums, tid, wave, G, n, true, 0, m, l, o);
+  leave<HD, float, 4, 64>(a, p, s_u.sums, tid, wave, G, n, true, 0, m, l, o);
 }
 
 // ---- joining the splits, and the slots' weights -------------------------------------------------------------
@@ -599,13 +641,20 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
     for (uint32_t s = tid; s < ns; s += 256) s_f[s] = __builtin_amdgcn_exp2f(gld(ml + 2 * s) - M);
     __syncthreads();
     f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    // a split far below the maximum still counts where its sum is infinite
+    auto add = [&](f4_t v, float f) {
+      if (f == 0.0f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fabsf(v[e]) < INFINITY ? 0.0f : v[e];
+      o += v * (f == 0.0f ? 1.0f : f);
+    };
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (tid / D4 + u * GR < ns) o += x[u] * s_f[tid / D4 + u * GR];
+      if (tid / D4 + u * GR < ns) add(x[u], s_f[tid / D4 + u * GR]);
 #pragma unroll 4
     for (uint32_t s = tid / D4 + U * GR; s < ns; s += GR) {
       const float4 v = ld_f4(acc + size_t(s) * HD);
-      o += f4_t{v.x, v.y, v.z, v.w} * s_f[s];
+      add(f4_t{v.x, v.y, v.z, v.w}, s_f[s]);
     }
     *reinterpret_cast<f4_t*>(&s_o[tid / D4][(tid % D4) * 4]) = o;
     __syncthreads();

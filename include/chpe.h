@@ -259,8 +259,9 @@ int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t head
  * q and out: `heads` x head_dim floats per row, rows q_stride / out_stride apart.  lens is read on the
  * device; max_len bounds it (and sizes the launch).  A row of length 0 gives zeros; one of a length
  * outside 0 .. max_len, or with a page id outside the pool among its slots, gives NaN (in the latter case in its
- * weights too), and so may an infinite value among a head's keys or queries.  What lies in slots outside the
- * range is never used.
+ * weights too), and so may an infinite value among a head's keys or queries.  An infinite element of V makes its
+ * dim infinite for the heads that read it, whatever its slot's weight; NaN where it meets a NaN or an infinity of the
+ * other sign.  What lies in slots outside the range is never used.
  * weight_out (optional) [rows][kv_heads][weight_stride]: at each slot below the length, weight_in (null:
  * 0) plus the slot's softmax weights summed over the query heads of its kv head; weight_in may be
  * weight_out.  Rows may share pages (a common prefix, or one sequence's drafts as rows of growing length).
