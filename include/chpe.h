@@ -284,7 +284,8 @@ size_t chpe_paged_attention_workspace(const chpe_kv_pages *cache, uint32_t heads
  * slot that each one held before) of the same layout receive the slots below lens_out[r], the others keep
  * what they hold.  weight_out may be weight, pos_out slot_pos, lens_out lens; they do not overlap
  * otherwise.  Rows whose length is outside 0 .. max_len are left as they are.  The pages of a row that is
- * cut belong to it alone; a move from or to a page id outside the pool is left out.
+ * cut belong to it alone.  A move to a page id outside the pool is left out; where a kept slot lay in one, its keys
+ * and values are lost and the slot that receives it holds NaN.
  * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
 int chpe_paged_evict(const chpe_kv_pages *cache, const int32_t *lens, uint32_t max_len, uint32_t budget,
                      uint32_t recent, uint32_t sinks, const float *weight, const int32_t *slot_pos, uint64_t stride,
