@@ -42,6 +42,9 @@ _engine_lib = None
 _pack_lib = None
 
 
+_U32_MAX = 0xffffffff  # (ctypes keeps the low 32 bits of what is larger, without a word)
+
+
 class _KvPages(ctypes.Structure):  # chpe_kv_pages
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int),
                 *[(n, ctypes.c_uint32) for n in ("kv_heads", "head_dim", "page_size", "n_pages")],
@@ -387,6 +390,8 @@ class KvPages:
             raise ValueError("table: [rows, pages_per_row] int32, the last stride 1")
         if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
             raise ValueError("table: rows that do not lie in each other")
+        if max(*k.shape, *table.shape, table.stride(0)) > _U32_MAX:
+            raise ValueError("k, v and table: sizes within 32 bits")
         if not k.is_cuda or v.device != k.device or table.device != k.device:
             raise ValueError("k, v and table: on one GPU")
         self.k, self.v, self.table, self.device = k, v, table, k.device
@@ -460,6 +465,8 @@ class KvPages:
             shape = rope[0].shape
             n, half = shape
             cos, sin = take(rope[0], "rope's cosines", f32, shape), take(rope[1], "rope's sines", f32, shape)
+        if max(t, n) > _U32_MAX:
+            raise ValueError("tokens and rope's rows: within 32 bits")
         track, sp, sw = 0, None, None
         if slot_pos is not None:
             sp, track = self._slots(slot_pos, "slot_pos", i32, 1), slot_pos.shape[2]
@@ -475,6 +482,8 @@ class KvPages:
 
     def attention_workspace(self, heads, max_len, weights=False):
         """Bytes that attention() needs for these sizes."""
+        if min(heads, max_len) < 0 or max(heads, max_len) > _U32_MAX:
+            raise ValueError("heads and max_len: from 0 to 2^32 - 1")
         n = self.lib.chpe_paged_attention_workspace(self._c, heads, max_len, int(weights))
         if n == 0 and self.rows:
             raise ValueError("chpe_paged_attention_workspace rejected the arguments")
@@ -487,8 +496,8 @@ class KvPages:
         f32 = self._f32
         if q.dim() != 3:
             raise ValueError("q: [rows, heads, head_dim]")
-        if max_len < 0 or window < 0:
-            raise ValueError("max_len and window: not negative")
+        if min(max_len, window) < 0 or max(max_len, window) > _U32_MAX:
+            raise ValueError("max_len and window: from 0 to 2^32 - 1")
         heads, width = q.shape[1], q.shape[1] * self.head_dim
         qp = self._take(q, "q", f32, (self.rows, heads, self.head_dim))
         if out is None:
@@ -514,6 +523,8 @@ class KvPages:
 
     def evict_workspace(self, max_len):
         """Bytes that evict() needs."""
+        if max_len < 0 or max_len > _U32_MAX:
+            raise ValueError("max_len: from 0 to 2^32 - 1")
         n = self.lib.chpe_paged_evict_workspace(self._c, max_len)
         if n == 0 and self.rows:
             raise ValueError("chpe_paged_evict_workspace rejected the arguments")
@@ -524,8 +535,8 @@ class KvPages:
         """chpe_paged_evict: every row and kv head down to `budget` slots.  lens_out, weight_out and pos_out
         default to the inputs themselves; returns lens_out."""
         f32, i32 = self._f32, self._i32
-        if min(max_len, budget, recent, sinks) < 0:
-            raise ValueError("max_len, budget, recent and sinks: not negative")
+        if min(max_len, budget, recent, sinks) < 0 or max(max_len, budget, recent, sinks) > _U32_MAX:
+            raise ValueError("max_len, budget, recent and sinks: from 0 to 2^32 - 1")
         lens_out, weight_out, pos_out = (i if o is None else o for o, i in
                                          ((lens_out, lens), (weight_out, slot_weight), (pos_out, slot_pos)))
         w = self._slots(slot_weight, "slot_weight", f32, max_len)
