@@ -139,17 +139,27 @@ __device__ __forceinline__ uint32_t below(uint64_t ballot, int lane) {
 // over it still says so.
 __device__ __forceinline__ void move_rows(const EvictArgs& a, uint32_t row, uint32_t h, const uint32_t* to,
                                           const uint32_t* from, uint32_t n, uint32_t first, uint32_t step, uint32_t lane) {
+  bool lost = false;
   for (uint32_t i = first; i < n; i += step) {
     const uint32_t d = to[i], s = from[i];
     uint32_t pd, ps;
     if (!a.c.page_of(row, d, &pd)) continue;
-    const bool held = a.c.page_of(row, s, &ps);
+    if (!a.c.page_of(row, s, &ps)) {
+      lost = true;
+      continue;
+    }
     const size_t od = a.c.at(pd, h, d) * a.elem + lane * 16, os = a.c.at(ps, h, s) * a.elem + lane * 16;
-    u32x4_t kk = ld_once(reinterpret_cast<const u32x4_t*>(a.c.k + os));
-    u32x4_t vv = ld_once(reinterpret_cast<const u32x4_t*>(a.c.v + os));
-    if (!held) kk = vv = u32x4_t{~0u, ~0u, ~0u, ~0u};
+    const u32x4_t kk = ld_once(reinterpret_cast<const u32x4_t*>(a.c.k + os));
+    const u32x4_t vv = ld_once(reinterpret_cast<const u32x4_t*>(a.c.v + os));
     st_once(reinterpret_cast<u32x4_t*>(a.c.k + od), kk);
     st_once(reinterpret_cast<u32x4_t*>(a.c.v + od), vv);
+  }
+  if (!lost) return;
+  for (uint32_t i = first; i < n; i += step) {
+    uint32_t pd, ps;
+    if (!a.c.page_of(row, to[i], &pd) || a.c.page_of(row, from[i], &ps)) continue;
+    const size_t od = a.c.at(pd, h, to[i]) * a.elem + lane * 16;
+    *reinterpret_cast<u32x4_t*>(a.c.k + od) = *reinterpret_cast<u32x4_t*>(a.c.v + od) = u32x4_t{~0u, ~0u, ~0u, ~0u};
   }
 }
 
