@@ -72,7 +72,8 @@ inline bool stream_here(hipStream_t st) {
   return false;
 }
 
-constexpr uint64_t kMaxBlocks = uint64_t(1) << 23;  // x 256 threads: below the grid's 2^32 work-items
+constexpr uint64_t kMaxItems = (uint64_t(1) << 32) - 1;  // work-items of a launch
+constexpr uint64_t kMaxBlocks = uint64_t(1) << 23;       // of 256 threads: half of that
 
 // one launch; its own error, not one that an earlier call of the program left
 template <class... P, class... A>

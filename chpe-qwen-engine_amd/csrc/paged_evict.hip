@@ -389,7 +389,8 @@ size_t evict_bytes(const chpe_kv_pages* c, uint32_t max_len, size_t* off) {
 }
 
 bool evict_shape_ok(const chpe_kv_pages* c, uint32_t max_len) {
-  return uint64_t(max_len) <= uint64_t(c->pages_per_row) * c->page_size && uint64_t(c->rows) * c->kv_heads <= kMaxBlocks;
+  return uint64_t(max_len) <= uint64_t(c->pages_per_row) * c->page_size &&
+         uint64_t(c->rows) * c->kv_heads <= kMaxItems / kSelect;
 }
 
 }  // namespace
@@ -439,8 +440,7 @@ extern "C" int chpe_paged_evict(const chpe_kv_pages* cache, const int32_t* lens,
   a.in_place = lens_out == lens ? 1 : 0;
   a.fused = most <= kFusedMoves && max_len <= kLongest ? 1 : 0;
   const uint64_t items = uint64_t(cache->rows) * cache->kv_heads;
-  const uint32_t parts = std::max(1u, std::min(8u, most / 64));
-  if (items * parts > kMaxBlocks) return -1;
+  const uint32_t parts = std::max(1u, std::min({8u, most / 64, uint32_t(kMaxBlocks / items)}));
   const bool ok = max_len == 0              ? launch(&k_evict_select_long, items, kSelect, st, a)  // (lens_out)
                   : max_len <= kSelect      ? launch(&k_evict_select<1>, items, kSelect, st, a)
                   : max_len <= 4 * kSelect  ? launch(&k_evict_select<4>, items, kSelect, st, a)
