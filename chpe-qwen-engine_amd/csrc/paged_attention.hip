@@ -714,8 +714,9 @@ uint32_t heads_per_group(const chpe_kv_pages* c, uint32_t heads) {
 }
 
 struct AttnPlan {
-  uint32_t ht = 0, hz = 0, splits = 1, chunk = 1, score_stride = 0;
-  uint64_t blocks = 0;
+  bool ok = false;  // the launches fit
+  uint32_t ht = 0, hz = 0, splits = 1, chunk = 1, score_stride = 0, joins = 0, weight_parts = 0;
+  uint64_t blocks = 0, joined = 0;
   size_t off_acc = 0, off_scores = 0, bytes = 0;
 };
 
@@ -738,11 +739,21 @@ AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uin
     const uint64_t want = std::max<uint64_t>((1024 + some - 1) / some, (uint64_t(range) + large - 1) / large);
     return std::min<uint64_t>(std::min<uint64_t>(want, steps), kMaxSplits);
   };
+  // (items <= heads_in_all)
+  const uint64_t heads_in_all = uint64_t(c->rows) * heads;
+  p.weight_parts = weights ? (max_len + 1023) / 1024 : 0;
+  const uint64_t weight_blocks = uint64_t(c->rows) * c->kv_heads * p.weight_parts;
+  if (heads_in_all > kMaxBlocks || weight_blocks > kMaxBlocks) return p;
   const uint32_t range = window != 0 && window < max_len ? window : max_len;
-  const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step), per = (steps + most(range) - 1) / most(range);
+  const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step), fit = kMaxBlocks / some;
+  uint64_t per = (steps + most(range) - 1) / most(range);
+  if ((steps + per - 1) / per > fit) per = (steps + fit - 1) / fit;  // (more than a launch holds: longer splits)
   p.chunk = uint32_t(per * step);
   p.splits = uint32_t((steps + per - 1) / per);
   p.blocks = items * p.splits;
+  p.joins = p.splits > 1 ? uint32_t(heads_in_all) : 0;
+  p.joined = p.joins + weight_blocks;
+  p.ok = p.joined <= kMaxItems / 256;
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   // the workspace does not depend on the window: `most` grows with the range
   const size_t places = size_t(c->rows) * heads * most(max_len);
@@ -781,7 +792,8 @@ extern "C" size_t chpe_paged_attention_workspace(const chpe_kv_pages* cache, uin
                                                  int weights) {
   Pages p;
   if (!pages_from(cache, &p) || !attn_shape_ok(cache, heads, max_len)) return 0;
-  return attn_plan(cache, heads, max_len, 0, weights != 0).bytes;
+  const AttnPlan plan = attn_plan(cache, heads, max_len, 0, weights != 0);
+  return plan.ok ? plan.bytes : 0;
 }
 
 extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, const int32_t* lens, uint32_t max_len,
@@ -797,10 +809,7 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   if (q_stride % 4 || out_stride % 4 || (cache->rows > 1 && (q_stride < width || out_stride < width))) return -1;
   if ((weight_in && !weight_out) || (weight_out && weight_stride < max_len)) return -1;
   const AttnPlan p = attn_plan(cache, heads, max_len, window, weight_out != nullptr);
-  const uint32_t parts = weight_out ? (max_len + 1023) / 1024 : 0;
-  const uint64_t heads_in_all = uint64_t(cache->rows) * heads, joins = p.splits > 1 ? heads_in_all : 0;
-  const uint64_t joined = joins + uint64_t(cache->rows) * cache->kv_heads * parts;
-  if (heads_in_all > kMaxBlocks || p.blocks > kMaxBlocks || joined > kMaxBlocks) return -1;
+  if (!p.ok) return -1;
   if (workspace_bytes < p.bytes) return -2;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   a.q = q;
@@ -828,9 +837,9 @@ extern "C" int chpe_paged_attention(const chpe_kv_pages* cache, uint32_t heads, 
   bool ok = hd == 64    ? launch_partial<64>(a, type, p.ht, p.blocks, st)
             : hd == 128 ? launch_partial<128>(a, type, p.ht, p.blocks, st)
                         : launch_partial<256>(a, type, p.ht, p.blocks, st);
-  if (ok && joined != 0)
-    ok = hd == 64    ? launch(&k_paged_join<64>, joined, 256, st, a, uint32_t(joins), parts)
-         : hd == 128 ? launch(&k_paged_join<128>, joined, 256, st, a, uint32_t(joins), parts)
-                     : launch(&k_paged_join<256>, joined, 256, st, a, uint32_t(joins), parts);
+  if (ok && p.joined != 0)
+    ok = hd == 64    ? launch(&k_paged_join<64>, p.joined, 256, st, a, p.joins, p.weight_parts)
+         : hd == 128 ? launch(&k_paged_join<128>, p.joined, 256, st, a, p.joins, p.weight_parts)
+                     : launch(&k_paged_join<256>, p.joined, 256, st, a, p.joins, p.weight_parts);
   return ok ? 0 : -3;
 }

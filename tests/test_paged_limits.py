@@ -15,3 +15,20 @@ def test_eviction_counts_its_own_workgroups(rows, kv, ok):
     c = pages(rows=rows, kv_heads=kv)
     assert (ca.load_engine_lib().chpe_paged_evict_workspace(c, 80) > 0) == ok
     assert evict(c, bytes=0) == (-2 if ok else -1)
+
+
+@pytest.mark.parametrize("rows,kv,heads,max_len,window,weights,ok", [
+    (131072, 1, 64, 80, 0, 0, True), (131073, 1, 64, 80, 0, 0, False), (200000, 8, 64, 80, 0, 0, False),
+    (200000, 8, 64, 80, 1, 0, False), ((1 << 32) - 1, 8, 65536, 80, 0, 0, False),
+    ((1 << 32) - 1, 8, 65536, 0x7ffffff0, 0, 1, False),
+    (1 << 20, 1, 1, 0x7ffffff0, 0, 0, True), (1 << 20, 1, 1, 0x7ffffff0, 99, 0, True),
+    (1 << 20, 8, 8, 0x7ffffff0, 0, 0, True),
+    (1 << 20, 1, 1, 8 * 1024, 0, 1, True), (1 << 20, 1, 1, 8 * 1024 + 1, 0, 1, False), (1 << 20, 1, 1, 8 * 1024 + 1, 1, 1, False),
+    (1 << 20, 1, 8, 8 * 1024, 0, 0, True)])
+def test_attention_workspace_is_0_where_the_call_refuses(rows, kv, heads, max_len, window, weights, ok):
+    per = (max_len + 15) // 16
+    c = pages(rows=rows, kv_heads=kv, pages_per_row=per, table_stride=per)
+    assert (ca.load_engine_lib().chpe_paged_attention_workspace(c, heads, max_len, weights) > 0) == ok
+    more = dict(wo=A, ws=max_len) if weights else {}
+    got = attention(c, heads=heads, max_len=max_len, window=window, qs=heads * 128, os=heads * 128, bytes=0, **more)
+    assert got == (-2 if ok else -1)
