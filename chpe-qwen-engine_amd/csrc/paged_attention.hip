@@ -641,20 +641,13 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
     for (uint32_t s = tid; s < ns; s += 256) s_f[s] = __builtin_amdgcn_exp2f(gld(ml + 2 * s) - M);
     __syncthreads();
     f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    // a split far below the maximum still counts where its sum is infinite
-    auto add = [&](f4_t v, float f) {
-      if (f == 0.0f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = fabsf(v[e]) < INFINITY ? 0.0f : v[e];
-      o += v * (f == 0.0f ? 1.0f : f);
-    };
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (tid / D4 + u * GR < ns) add(x[u], s_f[tid / D4 + u * GR]);
+      if (tid / D4 + u * GR < ns) o += x[u] * s_f[tid / D4 + u * GR];
 #pragma unroll 4
     for (uint32_t s = tid / D4 + U * GR; s < ns; s += GR) {
       const float4 v = ld_f4(acc + size_t(s) * HD);
-      add(f4_t{v.x, v.y, v.z, v.w}, s_f[s]);
+      o += f4_t{v.x, v.y, v.z, v.w} * s_f[s];
     }
     *reinterpret_cast<f4_t*>(&s_o[tid / D4][(tid % D4) * 4]) = o;
     __syncthreads();
@@ -662,7 +655,17 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnArgs a, uint32_t jo
       float v = 0.0f;
 #pragma unroll
       for (int g = 0; g < GR; ++g) v += s_o[g][tid];
-      a.out[row * a.out_stride + size_t(h) * HD + tid] = !ok ? __builtin_nanf("") : (L == 0.0f ? 0.0f : v / L);
+      v = !ok ? __builtin_nanf("") : (L == 0.0f ? 0.0f : v / L);
+      if (!(fabsf(v) < INFINITY) && ok && L == L) {
+        // an infinite sum counts whatever its split's factor, which may be 0
+        float inf = 0.0f;
+        for (uint32_t s = 0; s < ns; ++s) {
+          const float x = gld(a.part_acc + (size_t(item) * a.splits + s) * HD + tid);
+          inf += fabsf(x) < INFINITY ? 0.0f : x;
+        }
+        if (inf != 0.0f) v = inf;
+      }
+      a.out[row * a.out_stride + size_t(h) * HD + tid] = v;
     }
     return;
   }
