@@ -154,6 +154,7 @@ extern "C" int chpe_paged_append(const chpe_kv_pages* cache, uint32_t tokens, ui
   if (tokens == 0) return 0;
   if (!k || !v || !token_row || !token_slot || !token_pos || (heads != 0 && (!q || !q_out))) return -1;
   if (k_stride < uint64_t(cache->kv_heads) * hd || v_stride < uint64_t(cache->kv_heads) * hd) return -1;
+  if (heads > 1 && q_head_stride > (uint64_t(1) << 60) / heads) return -1;  // (their extent fits 64 bits, as the pool's)
   if (heads != 0 && (q_head_stride < hd || (tokens > 1 && q_stride < (heads - 1) * q_head_stride + hd))) return -1;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm) ||
       q_stride % 4 || q_head_stride % 4 || k_stride % 4 || v_stride % 4)

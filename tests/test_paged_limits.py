@@ -32,3 +32,10 @@ def test_attention_workspace_is_0_where_the_call_refuses(rows, kv, heads, max_le
     more = dict(wo=A, ws=max_len) if weights else {}
     got = attention(c, heads=heads, max_len=max_len, window=window, qs=heads * 128, os=heads * 128, bytes=0, **more)
     assert got == (-2 if ok else -1)
+
+
+@pytest.mark.parametrize("heads,head_stride", [(5, 1 << 62), (65, 1 << 58), (64, 0x0410410410410414), (2, (1 << 64) - 128)])
+def test_append_strides_whose_extent_wraps(heads, head_stride):
+    """(heads - 1) * q_head_stride past 64 bits does not pass for a small extent; nor without a second token."""
+    assert append(pages(), heads=heads, qh=head_stride, qs=64 * 128) == -1
+    assert append(pages(), heads=heads, qh=head_stride, qs=64 * 128, tokens=1) == -1
