@@ -84,9 +84,10 @@ __device__ __forceinline__ void leave_none(const PagedAttnArgs& a, const Place& 
 // and of the slots inside the second is free as long as both operands agree, which is what lets every lane load
 // 16 bytes in a row: K rows as pieces of 4 x 16 bytes, V rows as 16 lanes x 16 bytes.
 // The running maximum is in units of log2 (scores times scale * log2 e).
-// Bound by memory: each K and V row is read once, the next tile's K rows while the weights are formed, its V rows
-// while the scores are.  64 rows of 8320 slots with 8 kv heads of 128 (2.2 GB, fp16 or bf16) take 370 us with the
-// join, 5.9 TB/s, as do 32 such rows in f32; plain reads of the card reach 6.3.
+// Bound by memory: each K and V row is read once for the query heads of a workgroup (4, 8 or 16 of its kv head's,
+// heads_per_group; more query heads read it again), the next tile's K rows while the weights are formed, its V rows
+// while the scores are.  64 rows of 8320 slots with 8 kv heads of 128 (2.2 GB, fp16 or bf16) take 370 to 384 us with the
+// join, 5.7 to 5.9 TB/s, as do 32 such rows in f32; reads of the card reach 6.3, marked as made once (as V's are) 7.1.
 // A wave holds at most 128 dims of a tile's rows and of the accumulators (its registers then allow three waves a
 // SIMD); at head dim 256 two waves share a tile, half of the dims each, and add their scores through LDS.
 constexpr int kWaveDims = 128;
@@ -99,11 +100,13 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// 16-bit elements with f32 queries and weights: x is taken apart into parts that the products hold exactly,
-// part p of head h in column h + p * W of the 16; all columns' results are added at the end (sum_parts), so no
-// precision of the f32 queries or weights is lost to the cache's type.  fp16: two parts, 22 bits; x is brought
-// near 2^14 by a power of two first, so that the second part does not fall below fp16's range.  bf16: three
-// parts, 24 bits; of up to 4 heads they fit the 16 columns, of 8 the third is an operand of its own.
+// 16-bit elements with f32 queries and weights: x is taken apart into parts of the cache's type, part p of head h in
+// column h + p * W of the 16; all columns' results are added at the end (sum_parts).  bf16: three parts hold all 24
+// bits of x; of up to 4 heads they fit the 16 columns, of 8 the third is an operand of its own.  fp16: two parts hold
+// 22 bits, so that a query or weight enters the products rounded, off by up to 2^-23 of itself (one unit in the last
+// place of f32, which a quarter of all values are off by): as much as two of the roundings that the f32 sums of hd
+// products make anyway, and a third part would double the products.  x is brought near 2^14 by a power of two
+// first, so that the second part does not fall below fp16's range.
 template <class T, int W>
 struct Parts;
 template <>
@@ -466,8 +469,8 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
 }
 
 // The same for the f32 cache: 16 query heads as columns, tiles of 16 slots, v_mfma_f32_16x16x4f32 (exact f32
-// products).  The order of the second product's loops is the one that compiles right: with the four slots of a
-// lane inside, the compiler put a result over V values that were still to be read.
+// products).  The second product takes the four slots of a lane outside and the dims inside, so that products into
+// one accumulator are VD apart.
 template <int HD>
 __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(PagedAttnArgs a) {
   constexpr int DS = dim_shares(HD), HW = HD / DS, UNIT = 16 * tiles_at_once(HD);
@@ -612,7 +615,7 @@ __device__ __forceinline__ void join_ml(const PagedAttnArgs& a, uint32_t item, u
 }
 
 // Bound by latency: the lengths, the statistics and the sums, one after the other (64 heads of 86 splits 4.8 us,
-// 4096 heads of 9 splits 9.6 us; with the weights of 24 rows of up to 4097 slots 8.7 us).
+// 4096 heads of 9 splits 9.6 us; with the weights of 24 rows of up to 4097 slots 9.4 us).
 // blocks 0 .. joins - 1: the output of one (row, query head) each, 256 / (HD / 4) splits at a time;
 // the others: the weights of 1024 slots of one (row, kv head)
 template <int HD>
@@ -725,9 +728,11 @@ struct AttnPlan {
 
 // How the rows are split: into about 1024 workgroups where the rows are few (4 a CU: a long row alone takes
 // 28.6 us over 32771 slots of 4 KB; with 1536 workgroups 30.8), and into splits of at most 512 KB where they
-// are many, so that rows of different lengths keep the chip busy to the end (64 rows of up to 8320 slots: 205 us
-// with 512 KB, 200 with 768 KB, 235 with 256 KB).  A row's split depends on max_len and the number of rows, not
-// on the other rows' lengths.  (Dealing all rows' tiles out in equal runs over the workgroups that the chip
+// are many, so that rows of different lengths keep the chip busy to the end (64 rows of up to 8320 slots: 207 us
+// with 512 KB, 204 to 211 with 768 KB, 238 with 256 KB).  Between 512 and 768 KB neither wins everywhere: over twelve
+// batches of 24 to 200 rows of all types 768 took 0.82 to 1.17 of the time, 0.98 in the mean, by how the number of
+// splits meets that of the workgroups that the chip holds.  A row's split depends on max_len and the number of rows,
+// not on the other rows' lengths.  (Dealing all rows' tiles out in equal runs over the workgroups that the chip
 // holds took as long on f32 and 5 to 25 % longer on 16-bit caches: finding the place costs 2 us and the slowest
 // run ends the launch.)
 AttnPlan attn_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t max_len, uint32_t window, bool weights) {

@@ -27,7 +27,9 @@ struct EvictArgs {
 };
 
 constexpr int kSelect = 1024, kSelWaves = kSelect / 64;  // threads of the selection
-constexpr uint32_t kFusedMoves = 64;                     // at most this many moves: made by the selection itself
+// At most this many moves are made by the selection itself: 16 rows of 4 heads of 256 with 64 moves each 11.7 us a
+// call, with a launch for them 17.9.  The two meet at some 256 moves (22.1 us both ways; 512: 30.3 against 24.5).
+constexpr uint32_t kFusedMoves = 64;
 constexpr uint32_t kFew = 8;                             // at most this many slots to drop: one after the other
 
 // the order of the weights as unsigned integers: NaN 0, then -inf .. +inf (-0 as +0)
@@ -366,8 +368,8 @@ __global__ void __launch_bounds__(kSelect) k_evict_select_long(EvictArgs a) {
   }
 }
 
-// the moves that the selection left, `parts` workgroups per (row, kv head).  Bound by memory: 128 x 1560 moves of
-// 256-byte rows 42 to 48 us, 4.2 to 4.8 TB/s read and written.
+// the moves that the selection left, `parts` workgroups per (row, kv head).  128 x 1560 moves of 256-byte
+// rows 48.5 us, 4.2 TB/s read and written: a thread has one row in flight, behind its slots' and pages' numbers.
 __global__ void __launch_bounds__(256) k_evict_move(EvictArgs a, uint32_t parts) {
   const uint32_t item = blockIdx.x / parts, part = blockIdx.x % parts, per = 256 / a.row16;
   const uint32_t *to = a.moves + size_t(item) * a.half * 2, *from = to + a.half;
