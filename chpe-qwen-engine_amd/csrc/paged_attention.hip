@@ -106,7 +106,8 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 // 22 bits, so that a query or weight enters the products rounded, off by up to 2^-23 of itself (one unit in the last
 // place of f32, which a quarter of all values are off by): as much as two of the roundings that the f32 sums of hd
 // products make anyway, and a third part would double the products.  x is brought near 2^14 by a power of two
-// first, so that the second part does not fall below fp16's range.
+// first, so that the second part falls below fp16's range only where x is small beside the others: then it is off
+// by 2^-38 of the head's largest query, or by 2^-40 of the row's largest weight.
 template <class T, int W>
 struct Parts;
 template <>
@@ -173,7 +174,8 @@ struct TileRows {
 // An infinite V element makes its dim's sum infinite whatever its slot's weight, but the products give NaN where
 // they meet it with a 0: a padding row's weight, a part of a weight that has no bits left, a weight that 32 bits
 // hold as 0.  So a sum of dims dim .. dim + 3 that came out infinite or NaN is told again from the split's values
-// that are not finite themselves: their sum, or v where there are none (a sum past f32's range).
+// that are not finite themselves: their sum, or v where there are none (a sum past f32's range).  64 rows of up to
+// 8320 slots take 0.52 ms with one such element in every row, 1.4 ms where all are, 0.21 ms without.
 __device__ __forceinline__ bool all_finite(f4_t v) {
   return fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
 }

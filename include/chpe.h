@@ -266,7 +266,8 @@ int chpe_paged_append(const chpe_kv_pages *cache, uint32_t tokens, uint32_t head
  * 0) plus the slot's softmax weights summed over the query heads of its kv head; weight_in may be
  * weight_out.  Rows may share pages (a common prefix, or one sequence's drafts as rows of growing length).
  * Scores, sums and outputs are f32; queries and softmax weights enter the products with 24 bits, against an fp16
- * cache with 22.
+ * cache with 22.  The sums of V are divided by the weights' sum at the end, so that elements of V past 3e38 / lens[r]
+ * may come out infinite.
  * workspace: chpe_paged_attention_workspace bytes for the same cache, heads and max_len, at a 16-byte boundary, any
  * content; calls that may overlap need one each.
  * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
