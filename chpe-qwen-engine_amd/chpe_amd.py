@@ -32,6 +32,7 @@ ENGINE_SYMBOLS = [
     "chpe_debug_gemv", "chpe_debug_flat_tile_weights", "chpe_debug_gemv_flat", "chpe_debug_gemv_cells", "chpe_debug_gemv_poly", "chpe_debug_gemv_raw", "chpe_debug_embed_row_cell",
     "chpe_debug_attention", "chpe_debug_attention_block", "chpe_attention_noalloc", "chpe_paged_append",
     "chpe_paged_attention", "chpe_paged_attention_workspace", "chpe_paged_evict", "chpe_paged_evict_workspace",
+    "chpe_delta_step", "chpe_delta_prompt", "chpe_delta_prompt_workspace", "chpe_delta_conv",
     "chpe_debug_deltanet_conv", "chpe_debug_deltanet_step",
 ]
 
@@ -50,6 +51,18 @@ class _KvPages(ctypes.Structure):  # chpe_kv_pages
                 *[(n, ctypes.c_uint32) for n in ("kv_heads", "head_dim", "page_size", "n_pages")],
                 *[(n, ctypes.c_uint64) for n in ("page_stride", "head_stride", "slot_stride")],
                 ("table", ctypes.c_void_p), *[(n, ctypes.c_uint32) for n in ("rows", "pages_per_row", "table_stride")]]
+
+
+class _DeltaStates(ctypes.Structure):  # chpe_delta_states
+    _fields_ = [("state", ctypes.c_void_p), ("slot_stride", ctypes.c_uint64),
+                *[(n, ctypes.c_uint32) for n in ("n_slots", "v_heads", "k_heads", "head_dim")]]
+
+
+class _DeltaTokens(ctypes.Structure):  # chpe_delta_tokens
+    _fields_ = [("type", ctypes.c_int), *[(n, ctypes.c_void_p) for n in ("q", "k", "v", "z", "out")],
+                *[(n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "z_stride", "out_stride")],
+                ("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("a_stride", ctypes.c_uint64), ("b_stride", ctypes.c_uint64),
+                *[(n, ctypes.c_void_p) for n in ("A_log", "dt_bias", "norm_w")], ("eps", ctypes.c_float)]
 
 
 def _fp(a):
@@ -85,6 +98,7 @@ def load_engine_lib():
         V, S, I, U64, F, D = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint64,
                               ctypes.c_float, ctypes.c_double)
         U32, P = ctypes.c_uint32, ctypes.POINTER(_KvPages)
+        DS, DT = ctypes.POINTER(_DeltaStates), ctypes.POINTER(_DeltaTokens)
         sig = {
             "chpe_init": (V, [ctypes.c_char_p]),
             "chpe_forward_tokens": (I, [V, _c_u32_p, S, _c_float_p]),
@@ -137,6 +151,10 @@ def load_engine_lib():
             "chpe_paged_attention_workspace": (S, [P, U32, U32, I]),
             "chpe_paged_evict": (I, [P, V, U32, U32, U32, U32, V, V, U64, V, V, V, V, V, S, V]),
             "chpe_paged_evict_workspace": (S, [P, U32]),
+            "chpe_delta_step": (I, [DS, DT, U32, V, V, V]),
+            "chpe_delta_prompt": (I, [DS, DT, U32, U32, V, V, V, V, S, V]),
+            "chpe_delta_prompt_workspace": (S, [DS, U32, U32, I]),
+            "chpe_delta_conv": (I, [V, U64, U32, U32, U32, V, I, V, U64, V, U64, U32, U32, V, V, V, V]),
             "chpe_debug_deltanet_conv": (I, [ctypes.c_uint32, ctypes.c_uint32, _c_float_p, _c_float_p, _c_float_p,
                                              _c_float_p]),
             "chpe_debug_deltanet_step": (I, [ctypes.c_uint32] * 3 + [_c_float_p] * 9 + [F, _c_float_p, _c_float_p]),
@@ -550,6 +568,158 @@ class KvPages:
         self._call("chpe_paged_evict", self._take(lens, "lens", i32, (self.rows,)), max_len, budget, recent, sinks, w,
                    *args, ws, workspace.numel())
         return lens_out
+
+
+class _OnDevice:
+    """What the operators on torch tensors of one GPU share: types, streams, checks of tensors."""
+
+    def __init__(self, device):
+        import torch
+        self._torch, self.lib, self.device, self._index = torch, load_engine_lib(), device, device.index
+        self._f32, self._i32, self._types = torch.float32, torch.int32, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        # (torch.cuda.current_stream builds an object for every call)
+        self._stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+    def _call(self, name, *args):
+        cuda = self._torch.cuda
+        if cuda.current_device() != self._index:
+            with cuda.device(self._index):
+                return self._call(name, *args)
+        rc = getattr(self.lib, name)(*args, self._stream(self._index))
+        if rc:
+            raise EngineError(f"{name} failed: {rc}")
+
+    def _take(self, t, name, dtype, shape):
+        """The address of a contiguous tensor of this type and shape on the pool's device."""
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
+            raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {self.device}")
+        return t.data_ptr()
+
+    def _tokens(self, t, name, dtype, shape):
+        """Address and token stride of a [tokens, ..] tensor that is contiguous within a token."""
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index:
+            raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} on {self.device}")
+        width = 1
+        for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if n != 1 and st != width and t.numel():
+                raise ValueError(f"{name}: contiguous within a token")
+            width *= n
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+
+    def _rows(self, starts, slot_in, slot_out, rows):
+        """The addresses of a call's rows: starts [rows + 1] (or None), slot_in and slot_out [rows], int32."""
+        i32 = self._i32
+        return (None if starts is None else self._take(starts, "starts", i32, (rows + 1,)),
+                self._take(slot_in, "slot_in", i32, (rows,)),
+                self._take(slot_in if slot_out is None else slot_out, "slot_out", i32, (rows,)))
+
+
+class DeltaConv(_OnDevice):
+    """The convolution in front of the gated delta rule over a pool of its states (chpe_delta_conv, include/chpe.h):
+    state [n_slots, channels, taps - 1] f32 (contiguous within a slot), w [channels, taps] f32.  The tensors stay
+    the caller's; calls enqueue on torch's current stream of their device."""
+
+    def __init__(self, state, w):
+        if not state.is_cuda or state.dim() != 3 or w.dim() != 2:
+            raise ValueError("state: [n_slots, channels, taps - 1], w: [channels, taps], on one GPU")
+        super().__init__(state.device)
+        self.state, self.w = state, w
+        n, self.channels, past = state.shape
+        p, stride = self._tokens(state, "state", self._f32, state.shape)
+        if max(n, self.channels, past) >= _U32_MAX:
+            raise ValueError("state: sizes within 32 bits")
+        self._args = (p, stride, n, self.channels, past + 1, self._take(w, "w", self._f32, (self.channels, past + 1)))
+
+    def apply(self, x, starts, slot_in, slot_out=None, out=None):
+        """chpe_delta_conv: x [tokens, channels] (f32, fp16 or bf16); row r's tokens are starts[r] .. starts[r + 1] - 1
+        (starts None: token r is row r's).  slot_out defaults to slot_in.  Returns out (or a new tensor) of x's type."""
+        if x.dim() != 2 or x.dtype not in self._types:
+            raise ValueError("x: [tokens, channels], f32, fp16 or bf16")
+        rows, shape = slot_in.numel(), (x.shape[0], self.channels)
+        if starts is None and x.shape[0] != rows:
+            raise ValueError("without starts: one token per row")
+        if max(x.shape[0], rows) > _U32_MAX:
+            raise ValueError("tokens and rows: within 32 bits")
+        if out is None:
+            out = self._torch.empty(shape, dtype=x.dtype, device=self.device)
+        xp, xs = self._tokens(x, "x", x.dtype, shape)
+        op, os_ = self._tokens(out, "out", x.dtype, shape)
+        self._call("chpe_delta_conv", *self._args, self._types[x.dtype], xp, xs, op, os_, x.shape[0], rows,
+                   *self._rows(starts, slot_in, slot_out, rows))
+        return out
+
+
+class DeltaStates(_OnDevice):
+    """A pool of states of the gated delta rule and its operators (chpe_delta_*, include/chpe.h): state [n_slots, v_heads,
+    head_dim, head_dim] f32 (keys, values; contiguous within a slot), k_heads key heads.  The tensor stays the
+    caller's; calls enqueue on torch's current stream of its device."""
+
+    def __init__(self, state, k_heads):
+        if not state.is_cuda or state.dim() != 4 or state.shape[2] != state.shape[3]:
+            raise ValueError("state: [n_slots, v_heads, head_dim, head_dim] on a GPU")
+        super().__init__(state.device)
+        self.state, self.k_heads = state, k_heads
+        n, self.v_heads, self.head_dim, _ = state.shape
+        if max(n, self.v_heads, self.head_dim, k_heads) > _U32_MAX or k_heads < 0:
+            raise ValueError("state and k_heads: sizes within 32 bits")
+        p, stride = self._tokens(state, "state", self._f32, state.shape)
+        self._c = ctypes.byref(_DeltaStates(p, stride, n, self.v_heads, k_heads, self.head_dim))
+
+    def _layer(self, q, k, v, a, b, A_log, dt_bias, z, norm_w, eps, out):
+        f32, dt, n, nv, hd = self._f32, v.dtype, v.shape[0], self.v_heads, self.head_dim
+        if dt not in self._types:
+            raise ValueError("q, k, v, z and out: f32, fp16 or bf16")
+        if n > _U32_MAX:
+            raise ValueError("tokens: within 32 bits")
+        if (z is None) != (norm_w is None):
+            raise ValueError("z and norm_w: both or neither")
+        kshape, vshape = (n, self.k_heads, hd), (n, nv, hd)
+        if out is None:
+            out = self._torch.empty(vshape, dtype=dt, device=self.device)
+        qp, qs = self._tokens(q, "q", dt, kshape)
+        kp, ks = self._tokens(k, "k", dt, kshape)
+        vp, vs = self._tokens(v, "v", dt, vshape)
+        op, os_ = self._tokens(out, "out", dt, vshape)
+        zp, zs = (None, 0) if z is None else self._tokens(z, "z", dt, vshape)
+        ap, as_ = self._tokens(a, "a", f32, (n, nv))
+        bp, bs = self._tokens(b, "b", f32, (n, nv))
+        return out, ctypes.byref(_DeltaTokens(
+            self._types[dt], qp, kp, vp, zp, op, qs, ks, vs, zs, os_, ap, bp, as_, bs, self._take(A_log, "A_log", f32, (nv,)),
+            self._take(dt_bias, "dt_bias", f32, (nv,)), None if norm_w is None else self._take(norm_w, "norm_w", f32, (hd,)),
+            eps))
+
+    def step(self, q, k, v, a, b, A_log, dt_bias, slot_in, slot_out=None, z=None, norm_w=None, eps=1e-6, out=None):
+        """chpe_delta_step: one token per row.  q, k [rows, k_heads, head_dim], v [rows, v_heads, head_dim] (f32, fp16
+        or bf16, parts of wider rows as they come), a, b [rows, v_heads] f32; slot_out defaults to slot_in.
+        Returns out [rows, v_heads, head_dim] (or a new tensor)."""
+        out, t = self._layer(q, k, v, a, b, A_log, dt_bias, z, norm_w, eps, out)
+        rows = v.shape[0]
+        self._call("chpe_delta_step", self._c, t, rows, *self._rows(None, slot_in, slot_out, rows)[1:])
+        return out
+
+    def prompt_workspace(self, tokens, rows, norm=False):
+        """Bytes that prompt() needs; norm: with z and norm_w."""
+        if min(tokens, rows) < 0 or max(tokens, rows) > _U32_MAX:
+            raise ValueError("tokens and rows: from 0 to 2^32 - 1")
+        n = self.lib.chpe_delta_prompt_workspace(self._c, tokens, rows, int(norm))
+        if n == 0 and rows:
+            raise ValueError("chpe_delta_prompt_workspace rejected the arguments")
+        return n
+
+    def prompt(self, q, k, v, a, b, A_log, dt_bias, starts, slot_in, slot_out=None, z=None, norm_w=None, eps=1e-6, out=None,
+               workspace=None):
+        """chpe_delta_prompt: row r's tokens are starts[r] .. starts[r + 1] - 1 of q, k, v, a, b; the rest as step()."""
+        out, t = self._layer(q, k, v, a, b, A_log, dt_bias, z, norm_w, eps, out)
+        rows = slot_in.numel()
+        if rows > _U32_MAX:
+            raise ValueError("rows: within 32 bits")
+        u8 = self._torch.uint8
+        if workspace is None:
+            workspace = self._torch.empty(self.prompt_workspace(v.shape[0], rows, z is not None), dtype=u8, device=self.device)
+        self._call("chpe_delta_prompt", self._c, t, v.shape[0], rows, *self._rows(starts, slot_in, slot_out, rows),
+                   self._take(workspace, "workspace", u8, (workspace.numel(),)), workspace.numel())
+        return out
 
 
 def gpu_flat_tile_weights(cell):

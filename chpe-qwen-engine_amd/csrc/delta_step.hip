@@ -1,0 +1,166 @@
+// delta_step.hip -- chpe_delta_step: one token per row of the gated delta rule over a pool of states.
+// Per value head, with q, k l2-normalised, q over sqrt(head_dim) too, d the token's decay and b its beta:
+//   S' = d S,  S = S' + k (b (v - S'^T k))^T,  o = S^T q,  and optionally w * o / rms(o) * silu(z).
+#include "delta.hpp"
+
+namespace chpe {
+namespace {
+using namespace dev;
+
+// A workgroup takes one value head of one row: 256 threads hold its state, 4 columns of D / RG rows each (RG groups of
+// rows), 16 bytes a lane, read once and written once.  The column sums (S^T k before the update, S^T q after it) meet
+// over the groups of a wave, then over the waves in LDS, in a fixed order.
+// Bound by memory: 2 x 64 KB a head of 128.
+template <int D, class T>
+__global__ void __launch_bounds__(256) k_delta_step(DeltaArgs a) {
+  constexpr int LPR = D / 4, RG = 256 / LPR, RPT = D / RG, PL = D / 64;
+  const uint32_t h = blockIdx.x % a.NV, row = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR * 4, rg = tid / LPR;
+  __shared__ float s_q[D], s_k[D];
+  __shared__ __align__(16) float s_sum[2][4][D];
+  uint32_t lo, hi;
+  float fill;
+  const bool there = a.r.range(row, &lo, &hi);
+  const int slot = a.r.before(row, &fill), to = a.r.after(row);
+  if (!there) return;
+  float s[RPT][4];
+  const size_t at = size_t(h) * D * D + size_t(rg) * D + c;
+  if (slot >= 0) {
+    const float* S = a.state + uint64_t(slot) * a.slot_stride + at;
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) {
+      const f32x4_t v = ld_once(reinterpret_cast<const f32x4_t*>(S + size_t(r) * RG * D));
+      s[r][0] = v.x, s[r][1] = v.y, s[r][2] = v.z, s[r][3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < RPT; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[r][e] = fill;
+  }
+  // a column's total over the row groups, in every thread
+  auto total = [&](float (&p)[4], int buf) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (LPR == 16) p[e] = pair_sum(p[e], 16);
+      p[e] = pair_sum(p[e], 32);
+    }
+    if (lane < LPR) *reinterpret_cast<float4*>(&s_sum[buf][wave][c]) = make_float4(p[0], p[1], p[2], p[3]);
+    __syncthreads();
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(&s_sum[buf][w][c]);
+      t.x += x.x, t.y += x.y, t.z += x.z, t.w += x.w;
+    }
+    p[0] = t.x, p[1] = t.y, p[2] = t.z, p[3] = t.w;
+  };
+  const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
+  for (uint32_t t = lo; t < hi; ++t) {
+    float v[4], x[PL], y[PL], z[4], w[4];
+    ld_row(static_cast<const T*>(a.q) + t * a.q_stride + kh * D + lane * PL, x);
+    ld_row(static_cast<const T*>(a.k) + t * a.k_stride + kh * D + lane * PL, y);
+    ld_row(static_cast<const T*>(a.v) + t * a.v_stride + h * D + c, v);
+    if (a.z) {
+      ld_row(static_cast<const T*>(a.z) + t * a.z_stride + h * D + c, z);
+      ld_row(a.norm_w + c, w);
+    }
+    const float decay = expf(delta_log_decay(A_log, gld(a.a + t * a.a_stride + h) + dt));
+    const float beta = delta_beta(gld(a.b + t * a.b_stride + h));
+    float q2 = 0.0f, k2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      q2 = fmaf(x[i], x[i], q2);
+      k2 = fmaf(y[i], y[i], k2);
+    }
+    const float qi = 1.0f / sqrtf(wave_sum(q2) + 1e-6f) * (1.0f / sqrtf(float(D))), ki = 1.0f / sqrtf(wave_sum(k2) + 1e-6f);
+    if (t != lo) __syncthreads();  // (s_q, s_k)
+    if (wave == 0) {
+#pragma unroll
+      for (int i = 0; i < PL; ++i) {
+        s_q[lane * PL + i] = x[i] * qi;
+        s_k[lane * PL + i] = y[i] * ki;
+      }
+    }
+    __syncthreads();
+    float p[4] = {0.0f, 0.0f, 0.0f, 0.0f}, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) {
+      const float k = s_k[rg + r * RG];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[r][e] *= decay;
+        p[e] = fmaf(s[r][e], k, p[e]);
+      }
+    }
+    total(p, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = (v[e] - p[e]) * beta;
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) {
+      const float k = s_k[rg + r * RG], q = s_q[rg + r * RG];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[r][e] = fmaf(k, p[e], s[r][e]);
+        o[e] = fmaf(s[r][e], q, o[e]);
+      }
+    }
+    total(o, 1);
+    if (a.z) {  // (every group of D / 4 lanes holds the head's outputs)
+      float s2 = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s2 = fmaf(o[e], o[e], s2);
+#pragma unroll
+      for (int m = 1; m < LPR; m <<= 1) s2 = pair_sum(s2, m);
+      const float rr = 1.0f / sqrtf(s2 / float(D) + a.eps);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = w[e] * (o[e] * rr) * delta_silu(z[e]);
+    }
+    if (rg == 0) st_row(static_cast<T*>(a.out) + t * a.out_stride + h * D + c, o);
+  }
+  if (to >= 0) {
+    float* S = a.state + uint64_t(to) * a.slot_stride + at;
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) st_row(S + size_t(r) * RG * D, s[r]);
+  }
+}
+
+template <int D>
+bool launch_step(const DeltaArgs& a, int type, hipStream_t st) {
+  const uint64_t blocks = uint64_t(a.r.rows) * a.NV;
+  return type == 0   ? launch(&k_delta_step<D, float>, blocks, 256, st, a)
+         : type == 1 ? launch(&k_delta_step<D, _Float16>, blocks, 256, st, a)
+                     : launch(&k_delta_step<D, Bf16>, blocks, 256, st, a);
+}
+
+}  // namespace
+}  // namespace chpe
+
+using namespace chpe;
+
+extern "C" int chpe_delta_step(const chpe_delta_states* states, const chpe_delta_tokens* t, uint32_t rows,
+                               const int32_t* slot_in, const int32_t* slot_out, void* stream) {
+  DeltaArgs a{};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!delta_from(states, t, rows, rows, nullptr, slot_in, slot_out, &a) || !stream_here(st)) return -1;
+  if (uint64_t(rows) * a.NV > kMaxItems / 256) return -1;
+  if (rows == 0) return 0;
+  return (states->head_dim == 128 ? launch_step<128>(a, t->type, st) : launch_step<64>(a, t->type, st)) ? 0 : -3;
+}
+
+extern "C" size_t chpe_delta_prompt_workspace(const chpe_delta_states* states, uint32_t tokens, uint32_t rows, int norm) {
+  if (!delta_states_ok(states) || tokens > kMaxTokens || uint64_t(rows) * states->v_heads > kMaxItems / 256) return 0;
+  return 256;
+}
+
+extern "C" int chpe_delta_prompt(const chpe_delta_states* states, const chpe_delta_tokens* t, uint32_t tokens,
+                                 uint32_t rows, const int32_t* starts, const int32_t* slot_in, const int32_t* slot_out,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  DeltaArgs a{};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!delta_from(states, t, tokens, rows, starts, slot_in, slot_out, &a) || !stream_here(st)) return -1;
+  if (rows == 0) return 0;
+  if (!starts || !workspace || !aligned16(workspace) || uint64_t(rows) * a.NV > kMaxItems / 256) return -1;
+  if (workspace_bytes < chpe_delta_prompt_workspace(states, tokens, rows, t->z != nullptr)) return -2;
+  return (states->head_dim == 128 ? launch_step<128>(a, t->type, st) : launch_step<64>(a, t->type, st)) ? 0 : -3;
+}

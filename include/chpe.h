@@ -297,6 +297,65 @@ int chpe_paged_evict(const chpe_kv_pages *cache, const int32_t *lens, uint32_t m
 /* bytes; 0 for arguments that the call refuses */
 size_t chpe_paged_evict_workspace(const chpe_kv_pages *cache, uint32_t max_len);
 
+/* ---- the gated delta rule over a pool of states (no counterpart in the reference) ----
+ * For serving loops with many sequences of the hybrid model: its linear-attention layers beside the paged cache,
+ * on caller device buffers, under the rules of the paged cache's calls (nothing is allocated or kept, the calls only
+ * enqueue on `stream`).  The arithmetic is chpe_debug_deltanet_conv's and chpe_debug_deltanet_step's.
+ *
+ * A sequence's state lies in a slot of a pool.  Row r of a call reads slot slot_in[r] and leaves slot slot_out[r] (device
+ * arrays): the same one, or another where the program may have to go back (drafts that are rejected: run the accepted
+ * ones again from the state before) or starts many sequences from one prompt's state.  slot_in -1: a new sequence, all
+ * zeros; another id outside the pool: the state before is NaN.  A slot_out outside the pool (-1): the state is not kept.
+ * No slot that one row of a call writes is read or written by another row.
+ * Row r's tokens are starts[r] .. starts[r + 1] - 1 of `tokens` (starts [rows + 1], device, ascending); a row without
+ * tokens keeps its state (copied if the slots differ), a row whose range does not lie in the tokens is left out, and
+ * so are tokens of no row. */
+typedef struct chpe_delta_states {
+  float *state;              /* slot s at s * slot_stride: [v_heads][head_dim (keys)][head_dim (values)] */
+  uint64_t slot_stride;      /* floats */
+  uint32_t n_slots, v_heads, k_heads, head_dim;   /* v_heads a multiple of k_heads; head_dim 64 or 128 */
+} chpe_delta_states;
+
+/* Tokens of a linear-attention layer behind its convolution: q, k [k_heads][head_dim] before the l2 norm, v and out
+ * [v_heads][head_dim], a, b [v_heads] (f32) per token; strides in elements between tokens, so that q, k and v may be parts
+ * of the convolution's rows.  type (of q, k, v, z, out): 0 f32, 1 fp16, 2 bf16.  z and norm_w (both or neither): out
+ * is norm_w * o / rms(o) * silu(z), rms over the head with eps, instead of o.  q, k, v, z, out at 16-byte boundaries with
+ * strides multiples of 16 bytes.  out overlaps none of the inputs. */
+typedef struct chpe_delta_tokens {
+  int type;
+  const void *q, *k, *v, *z;
+  void *out;
+  uint64_t q_stride, k_stride, v_stride, z_stride, out_stride;
+  const float *a, *b;
+  uint64_t a_stride, b_stride;
+  const float *A_log, *dt_bias;                   /* [v_heads] */
+  const float *norm_w;                            /* [head_dim], at a 16-byte boundary */
+  float eps;
+} chpe_delta_tokens;
+
+/* One token per row (token r is row r's).  Returns 0, -1 bad arguments, -3 device error. */
+int chpe_delta_step(const chpe_delta_states *states, const chpe_delta_tokens *t, uint32_t rows, const int32_t *slot_in,
+                    const int32_t *slot_out, void *stream);
+/* Any number of tokens per row: prompts, drafts.  Sums and states are f32 as in chpe_delta_step.
+ * workspace: chpe_delta_prompt_workspace bytes for the same states, tokens, rows and norm (z given), at a 16-byte
+ * boundary, any content; calls that may overlap need one each.
+ * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
+int chpe_delta_prompt(const chpe_delta_states *states, const chpe_delta_tokens *t, uint32_t tokens, uint32_t rows,
+                      const int32_t *starts, const int32_t *slot_in, const int32_t *slot_out, void *workspace,
+                      size_t workspace_bytes, void *stream);
+/* bytes; 0 for arguments that the call refuses */
+size_t chpe_delta_prompt_workspace(const chpe_delta_states *states, uint32_t tokens, uint32_t rows, int norm);
+
+/* The causal depthwise convolution in front of the rule, with SiLU: y_t = silu(sum_j w[c][j] x_(t - taps + 1 + j)) for
+ * every channel c, what lies before a row's first token from its state.  conv_state: slot s at s * slot_stride floats,
+ * [channels][taps - 1], oldest first; w [channels][taps] f32; x, y [tokens][channels] of `type`, rows x_stride / y_stride
+ * elements apart, y not overlapping x.  taps 2 .. 8, channels a multiple of 8; all arrays of floats and rows at 16-byte
+ * boundaries.  starts null: token r is row r's.  Returns 0, -1 bad arguments, -3 device error. */
+int chpe_delta_conv(float *conv_state, uint64_t slot_stride, uint32_t n_slots, uint32_t channels, uint32_t taps,
+                    const float *w, int type, const void *x, uint64_t x_stride, void *y, uint64_t y_stride,
+                    uint32_t tokens, uint32_t rows, const int32_t *starts, const int32_t *slot_in,
+                    const int32_t *slot_out, void *stream);
+
 /* Gated-DeltaNet (Qwen3.5 linear-attention layers) decode-step kernels on caller data.  The
  * reference has no code for these layers (README claims only); the arithmetic is the gated
  * delta rule as defined by transformers 5.15.0 models/qwen3_5/modeling_qwen3_5.py.
