@@ -1,0 +1,745 @@
+// delta_prompt.hip -- chpe_delta_prompt: the gated delta rule over prompts, in chunks of 64 tokens.
+// Within a chunk, with g_i the sum of the tokens' log decays up to i, G its value at the chunk's end, S the state
+// before it, k and q normalised:
+//   A_ij = b_i (k_i . k_j) e^(g_i - g_j) for j < i,  T = (I + A)^-1,  u = T diag(b) (v - e^g (K S))
+//   o_i = e^g_i q_i S + sum_(j <= i) (q_i . k_j) e^(g_i - g_j) u_j,   S <- e^G S + sum_j e^(G - g_j) k_j u_j^T
+// which is the recurrence of chpe_delta_step unrolled: u_j are the updates b (v - S'^T k) of its tokens.
+// k_delta_prep forms T and the matrix of o for every chunk at once, k_delta_scan carries the state over a row's chunks
+// and writes the outputs, k_delta_gnorm applies the gated norm, which needs a head's whole row.
+#include "delta.hpp"
+
+namespace chpe {
+namespace {
+using namespace dev;
+
+constexpr int kChunkShift = 6, kChunk = 1 << kChunkShift;
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+// What a chunk of a value head leaves for the scan, in the order of its lanes: u's matrix T diag(b) and o's matrix,
+// rows of 16 tokens as products of 16 x 32 (mma below), then per token the factors of K S, Q S and k u^T, then e^G.
+constexpr int kFrag = 512;                              // floats of 16 x 32 values
+__device__ __host__ constexpr int frag_of(int w) { return w < 2 ? w : 2 * w - 2; }  // row w's first of w / 2 + 1
+constexpr int kOffO = 6 * kFrag, kOffScale = 12 * kFrag, kChunkFloats = kOffScale + 256;
+
+struct PromptArgs {
+  DeltaArgs d;
+  float *chunks, *o32;  // o32 [token][NV][D]: the outputs before the gated norm, null without it
+};
+
+// ---- products in 32 bits on the 16-bit matrix cores ---------------------------------------------------------
+// A value is taken apart into bf16 parts: three hold all 24 bits of an f32, two an fp16, one a bf16.  Of the products of
+// two values' parts those below 2^-25 of the whole are left out (three by three: six of nine remain), less than
+// the rounding of the f32 sums.
+template <class T>
+constexpr int kParts = 0;
+template <>
+constexpr int kParts<float> = 3;
+template <>
+constexpr int kParts<_Float16> = 2;
+template <>
+constexpr int kParts<Bf16> = 1;
+
+// the parts of two values, as words of two bf16
+template <int N>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&w)[N]) {
+#pragma unroll
+  for (int p = 0; p < N; ++p) {
+    w[p] = __builtin_bit_cast(uint32_t, b2_t{__bf16(x), __bf16(y)});
+    x -= __uint_as_float(w[p] << 16);
+    y -= __uint_as_float(w[p] & 0xffff0000u);
+  }
+}
+template <int NA, int NB>
+__device__ __forceinline__ f4_t mma(const u32x4_t (&a)[NA], const u32x4_t (&b)[NB], f4_t c) {
+#pragma unroll
+  for (int o = 2; o >= 0; --o)  // the small ones first
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (o - i >= 0 && o - i < NB)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a[i]), __builtin_bit_cast(b8_t, b[o - i]), c, 0, 0, 0);
+  return c;
+}
+template <int N>
+__device__ __forceinline__ void ld_parts(const u32x4_t (&src)[N][64], int lane, u32x4_t (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = src[i][lane];
+}
+// 16 x 16 by 16 x 16 in f32: a lane (G, n) holds row (or column) n, inner indexes 4 G + r
+__device__ __forceinline__ f4_t mma16(f4_t a, f4_t b, f4_t c) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+  return c;
+}
+
+// A token's key or query row in a wave that holds 16 tokens: lane (G, i) = (lane / 16, lane % 16) has dims G D / 4 ..
+// of token i, 4 groups of D / 16.  Product s of D / 32 takes dims 2 s, 2 s + 1 of every group of every lane: the inner
+// index of a product is free as long as both sides agree, and so 16-bit rows are operands as they come.
+template <int D, class T>
+struct Row16 {
+  static constexpr int W = D / 4 * int(sizeof(T)) / 16, KS = D / 32, GW = D / 32;  // GW: words of a group in 16 bits
+  u32x4_t w[W];
+  __device__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = gld(reinterpret_cast<const u32x4_t*>(p) + i);
+  }
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = u32x4_t{0, 0, 0, 0};
+  }
+  __device__ void pair(int e, float* x, float* y) const {  // elements e, e + 1 (e even)
+    if constexpr (sizeof(T) == 4) {
+      *x = __uint_as_float(w[e / 4][e % 4]);
+      *y = __uint_as_float(w[e / 4][e % 4 + 1]);
+    } else {
+      const uint32_t v = w[e / 8][e / 2 % 4];
+      if constexpr (__is_same(T, Bf16)) {
+        *x = __uint_as_float(v << 16);
+        *y = __uint_as_float(v & 0xffff0000u);
+      } else {
+        *x = half_lo(v);
+        *y = half_hi(v);
+      }
+    }
+  }
+  __device__ void operand(int s, u32x4_t (&out)[kParts<T>]) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if constexpr (__is_same(T, Bf16)) {
+        const int e = GW * r + s;
+        out[0][r] = w[e / 4][e % 4];
+      } else {
+        float x, y;
+        uint32_t p[kParts<T>];
+        pair(2 * (GW * r + s), &x, &y);
+        split2(x, y, p);
+#pragma unroll
+        for (int i = 0; i < kParts<T>; ++i) out[i][r] = p[i];
+      }
+    }
+  }
+  __device__ float sum2() const {  // of the token's squares, in all its lanes
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 4; e += 2) {
+      float x, y;
+      pair(e, &x, &y);
+      a = fmaf(x, x, a);
+      b = fmaf(y, y, b);
+    }
+    return pair_sum(pair_sum(a + b, 16), 32);
+  }
+};
+
+// Keys and queries whose squares leave this range, and gates that are NaN, make a chunk run token by token: the
+// products above take keys before their norm, and 0 times what is not finite would reach earlier tokens.
+__device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e30f; }
+
+// ---- T and o's matrix of a chunk --------------------------------------------------------------------------------
+// A workgroup per (chunk, value head); wave w forms o's row w (16 tokens) and A's row 3 - w, as many products for each.
+// Both are formed transposed (rows: j, columns: i), which is the order in which the scan takes them.
+// (I + A)^-1: the four 16 x 16 blocks on the diagonal by substitution, a column a lane; then row i from the right,
+// T_ij = -(sum_(j < k <= i) T_ik A_kj) T_jj, in a wave's registers.  |k| <= 1 and b < 1 keep T's elements within products
+// of contractions; a series in powers of A would not stay there.
+template <int D, class T>
+__global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
+  const DeltaArgs& a = pa.d;
+  constexpr int NP = kParts<T>, KS = D / 32, AS = 68;
+  constexpr int kBytesK = 4 * KS * NP * 1024, kBytesA = 64 * AS * 4;
+  __shared__ __align__(16) uint8_t s_mem[kBytesK > kBytesA ? kBytesK : kBytesA];
+  __shared__ __align__(16) float s_diag[4][16][20];
+  __shared__ double s_g[64];
+  __shared__ __align__(16) float s_beta[64], s_rk[64], s_rq[64];
+  auto s_k = reinterpret_cast<u32x4_t(*)[KS][NP][64]>(s_mem);
+  auto s_A = reinterpret_cast<float(*)[AS]>(s_mem);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+  const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
+  const int row = a.r.row_of(b, kChunkShift, lane);
+  uint32_t lo, hi;
+  if (row < 0 || !a.r.range(row, &lo, &hi)) return;
+  const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
+  if (t0 >= hi) return;
+  const uint32_t nt = min(hi - t0, uint32_t(kChunk)), mine = 16 * wave + n;
+  float* out = pa.chunks + size_t(blockIdx.x) * kChunkFloats;
+  Row16<D, T> kr, qr;
+  if (mine < nt) {
+    const size_t at = kh * D + G * (D / 4);
+    kr.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + at);
+    qr.load(static_cast<const T*>(a.q) + (t0 + mine) * a.q_stride + at);
+  } else {
+    kr.clear();
+    qr.clear();
+  }
+  float ld = 0.0f, beta = 0.0f;
+  bool fine = true;
+  if (wave == 0 && uint32_t(lane) < nt) {
+    ld = delta_log_decay(gld(a.A_log + h), gld(a.a + (t0 + lane) * a.a_stride + h) + gld(a.dt_bias + h));
+    beta = delta_beta(gld(a.b + (t0 + lane) * a.b_stride + h));
+    fine = ld == ld && beta == beta;
+    ld = ld < -200.0f ? -200.0f : ld;  // e^-200 is 0 in f32; differences of sums stay numbers
+  }
+  const float k2 = kr.sum2(), q2 = qr.sum2();
+  const float rk = 1.0f / sqrtf(k2 + 1e-6f), rq = 1.0f / sqrtf(q2 + 1e-6f) * (1.0f / sqrtf(float(D)));
+  if (G == 0) {
+    s_rk[mine] = in_range(k2) ? rk : -1.0f;  // (told below)
+    s_rq[mine] = in_range(q2) ? rq : -1.0f;
+  }
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    u32x4_t f[NP];
+    kr.operand(s, f);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) s_k[wave][s][p][lane] = f[p];
+  }
+  if (wave == 0) {
+    // sums in 64 bits: their differences are what counts, and in 32 bits 1e3 - 1e3 leaves 6e-5
+    double g = double(ld);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double p = __shfl_up(g, o);
+      g += lane >= o ? p : 0.0;
+    }
+    s_g[lane] = g;
+    s_beta[lane] = beta;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const double g = s_g[lane], end = s_g[63];
+    const float k = s_rk[lane], q = s_rq[lane];
+    fine = fine && k >= 0.0f && q >= 0.0f;
+    const bool all = __ballot(!fine) == 0;
+    float* sc = out + kOffScale;
+    sc[lane] = expf(float(g)) * k;
+    sc[64 + lane] = expf(float(g)) * q;
+    sc[128 + lane] = expf(float(end - g)) * k;
+    if (lane == 0) {
+      sc[192] = expf(float(end));
+      sc[193] = all ? 1.0f : 0.0f;
+    }
+  }
+  // tiles (j, i) transposed: lane (G, n) gets tokens j = 16 jt + 4 G + r of i = 16 it + n
+  f4_t At[4];
+  const int R = 3 - wave;
+  auto weight = [&](int it, int jt, f4_t v, bool below, float fi) {
+    const int i = 16 * it + n;
+    const double gi = s_g[i];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = 16 * jt + 4 * G + r;
+      v[r] = j < i || (j == i && !below) ? v[r] * (fi * s_rk[j]) * expf(float(gi - s_g[j])) : 0.0f;
+    }
+    return v;
+  };
+  {
+    u32x4_t qf[KS][NP];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qr.operand(s, qf[s]);
+    float* o = out + kOffO + frag_of(wave) * kFrag;
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+      if (jt > (wave | 1)) break;
+      f4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (jt <= wave) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          u32x4_t f[NP];
+          ld_parts(s_k[jt][s], lane, f);
+          v = mma(f, qf[s], v);
+        }
+        v = weight(wave, jt, v, false, s_rq[16 * wave + n]);
+      }
+      *reinterpret_cast<f4_t*>(o + (jt * 64 + lane) * 4) = v;
+    }
+  }
+  {
+    u32x4_t kf[KS][NP];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      ld_parts(s_k[R][s], lane, kf[s]);
+    const float fi = s_beta[16 * R + n] * s_rk[16 * R + n];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+      if (jt > R) break;
+      f4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4_t f[NP];
+        ld_parts(s_k[jt][s], lane, f);
+        v = mma(f, kf[s], v);
+      }
+      At[jt] = weight(R, jt, v, true, fi);
+    }
+  }
+  __syncthreads();  // (the keys have been read: A takes their place)
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt)
+    if (jt <= R) *reinterpret_cast<f4_t*>(&s_A[16 * R + n][16 * jt + 4 * G]) = At[jt];
+  __syncthreads();
+  {
+    float t[16];  // column n of T_ww
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x = i == n ? 1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) x = fmaf(-s_A[16 * wave + i][16 * wave + j], t[j], x);
+      t[i] = x;
+    }
+    if (G == 0) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(&s_diag[wave][n][i]) = make_float4(t[i], t[i + 1], t[i + 2], t[i + 3]);
+    }
+  }
+  __syncthreads();
+  f4_t Tt[4];  // T_wj transposed: lane (G, n) has row n, columns 4 G + r
+#pragma unroll
+  for (int j = 3; j >= 0; --j) {
+    if (j > wave) {
+      Tt[j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    } else if (j == wave) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) Tt[j][r] = s_diag[j][4 * G + r][n];
+    } else {
+      f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 3; k > j; --k) {
+        if (k > wave) continue;
+        f4_t x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = s_A[16 * k + 4 * G + r][16 * j + n];
+        acc = mma16(x, Tt[k], acc);
+      }
+      const f4_t d = -*reinterpret_cast<const f4_t*>(&s_diag[j][n][4 * G]);
+      Tt[j] = mma16(d, acc, f4_t{0.0f, 0.0f, 0.0f, 0.0f});
+    }
+  }
+  float* o = out + frag_of(wave) * kFrag;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > (wave | 1)) break;
+    const f4_t be = *reinterpret_cast<const f4_t*>(&s_beta[16 * j + 4 * G]);
+    *reinterpret_cast<f4_t*>(o + (j * 64 + lane) * 4) = Tt[j] * be;
+  }
+}
+
+// ---- the state over a row's chunks --------------------------------------------------------------------------------
+// A workgroup takes 16 NT columns of a value head's state over all chunks of a row; wave w holds D / 4 of its rows and
+// 16 tokens of a chunk.  A chunk is three steps with a barrier behind each, what one leaves to the others in LDS as
+// operands: v - e^g (K S) of the wave's tokens (Q S with it); u of its tokens; its rows of S (o with it).  The next
+// chunk's keys, queries, values and matrices are loaded meanwhile.
+// Keys as operands of k u^T have tokens inside: a product with a selection of unit vectors turns the wave's 16 tokens
+// of an operand of K S into that order, exactly.
+template <int D, class T, int NT>
+__global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
+  const DeltaArgs& a = pa.d;
+  constexpr int NP = kParts<T>, KS = D / 32, RT = D / 64, CB = D / (16 * NT), CH = D / 16;
+  __shared__ u32x4_t s_kt[D / 16][2][NP][64];
+  __shared__ u32x4_t s_s[KS][NT][3][64];
+  __shared__ u32x4_t s_x[NT][2][3][64], s_u[NT][2][3][64], s_us[NT][2][3][64];
+  __shared__ float s_red[2][4], s_col[2][4][16 * NT];
+  __shared__ int s_bad[2];
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+  // the column blocks of a head on one XCD (workgroup i runs on XCD i % 8), whose L2 they share
+  const uint32_t item = blockIdx.x / (8 * CB) * 8 + blockIdx.x % 8, c0 = blockIdx.x / 8 % CB * (16 * NT);
+  if (item >= a.r.rows * a.NV) return;
+  const uint32_t h = item % a.NV, row = item / a.NV, kh = h / (a.NV / a.NK);
+  uint32_t lo, hi;
+  float fill;
+  if (!a.r.range(row, &lo, &hi)) return;
+  const int slot = a.r.before(row, &fill), to = a.r.after(row);
+  // the wave's rows of the state: dim(u, r) = CH (4 G + r) + 2 wave + u (D = 64: + wave)
+  const int d0 = CH * 4 * G + RT * wave;
+  f4_t S[RT][NT];
+#pragma unroll
+  for (int u = 0; u < RT; ++u)
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        S[u][ct][r] = slot >= 0 ? gld(a.state + uint64_t(slot) * a.slot_stride + (size_t(h) * D + d0 + CH * r + u) * D + c0 + 16 * ct + n) : fill;
+  // leaves S as operands
+  auto leave_s = [&] {
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      if constexpr (RT == 2) {
+        u32x4_t f[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          uint32_t p[3];
+          split2(S[0][ct][r], S[1][ct][r], p);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) f[i][r] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) s_s[wave][ct][i][lane] = f[i];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          uint32_t p[3];
+          split2(S[0][ct][r], S[0][ct][r + 1], p);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            uint16_t* d = reinterpret_cast<uint16_t*>(&s_s[wave >> 1][ct][i][lane]) + (wave & 1);
+            d[2 * r] = uint16_t(p[i]);
+            d[2 * r + 2] = uint16_t(p[i] >> 16);
+          }
+        }
+      }
+    }
+  };
+  // leaves 16 tokens of one column tile as half of an operand with tokens inside
+  auto leave_u = [&](u32x4_t (&dst)[2][3][64], f4_t v) {
+    uint32_t p[2][3];
+    split2(v[0], v[1], p[0]);
+    split2(v[2], v[3], p[1]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      reinterpret_cast<u32x2_t*>(&dst[wave >> 1][i][lane])[wave & 1] = u32x2_t{p[0][i], p[1][i]};
+  };
+  // what a chunk reads
+  const int ns = (wave >> 1) + 1;  // products of 32 tokens in the wave's row of a matrix
+  struct Chunk {
+    Row16<D, T> k, q;
+    f4_t t[2][2], o[2][2], fx, fy, fz;
+    float v[NT][4], end, fine;
+  } cur;
+  const uint32_t first = a.r.first_block(row, lo, kChunkShift);
+  auto load = [&](uint32_t t0) {
+    const uint32_t last = hi - 1 - t0, at = kh * D + G * (D / 4);
+    const float* m = pa.chunks + (size_t(first + ((t0 - lo) >> kChunkShift)) * a.NV + h) * kChunkFloats;
+    const uint32_t mine = 16 * wave + n;
+    if (mine <= last) {
+      cur.k.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + at);
+      cur.q.load(static_cast<const T*>(a.q) + (t0 + mine) * a.q_stride + at);
+    } else {
+      cur.k.clear();
+      cur.q.clear();
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (s >= ns) break;
+        const float* f = m + (frag_of(wave) + s) * kFrag + (u * 64 + lane) * 4;
+        cur.t[s][u] = gld(reinterpret_cast<const f4_t*>(f));
+        cur.o[s][u] = gld(reinterpret_cast<const f4_t*>(f + kOffO));
+      }
+    const float* sc = m + kOffScale + 16 * wave + 4 * G;
+    cur.fx = gld(reinterpret_cast<const f4_t*>(sc));
+    cur.fy = gld(reinterpret_cast<const f4_t*>(sc + 64));
+    cur.fz = gld(reinterpret_cast<const f4_t*>(sc + 128));
+    cur.end = gld(m + kOffScale + 192);
+    cur.fine = gld(m + kOffScale + 193);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint32_t i = 16 * wave + 4 * G + r;
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
+        cur.v[ct][r] = i <= last ? Elem<T>::get(static_cast<const T*>(a.v) + (t0 + i) * a.v_stride + h * D + c0 + 16 * ct + n) : 0.0f;
+    }
+  };
+  auto put = [&](uint32_t t, int ct, float v) {
+    const size_t at = size_t(h) * D + c0 + 16 * ct + n;
+    if (pa.o32) pa.o32[size_t(t) * a.NV * D + at] = v;
+    else static_cast<T*>(a.out)[t * a.out_stride + at] = Elem<T>::put(v);
+  };
+  // the recurrence itself, token by token (inputs that are not finite: see in_range)
+  auto tokens = [&](uint32_t t0, uint32_t t1) {
+    const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
+    for (uint32_t t = t0; t < t1; ++t) {
+      float k[RT][4], q[RT][4], k2 = 0.0f, q2 = 0.0f;
+#pragma unroll
+      for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const size_t d = kh * D + d0 + CH * r + u;
+          k[u][r] = Elem<T>::get(static_cast<const T*>(a.k) + t * a.k_stride + d);
+          q[u][r] = Elem<T>::get(static_cast<const T*>(a.q) + t * a.q_stride + d);
+          k2 = fmaf(k[u][r], k[u][r], k2);
+          q2 = fmaf(q[u][r], q[u][r], q2);
+        }
+      k2 = pair_sum(pair_sum(k2, 16), 32);
+      q2 = pair_sum(pair_sum(q2, 16), 32);
+      if (lane == 0) {
+        s_red[0][wave] = k2;
+        s_red[1][wave] = q2;
+      }
+      __syncthreads();
+      k2 = (s_red[0][0] + s_red[0][1]) + (s_red[0][2] + s_red[0][3]);
+      q2 = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+      const float ki = 1.0f / sqrtf(k2 + 1e-6f), qi = 1.0f / sqrtf(q2 + 1e-6f) * (1.0f / sqrtf(float(D)));
+      const float decay = expf(delta_log_decay(A_log, gld(a.a + t * a.a_stride + h) + dt));
+      const float beta = delta_beta(gld(a.b + t * a.b_stride + h));
+      auto total = [&](float (&p)[NT], int buf) {
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+          p[ct] = pair_sum(pair_sum(p[ct], 16), 32);
+          if (G == 0) s_col[buf][wave][16 * ct + n] = p[ct];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) {
+          const int c = 16 * ct + n;
+          p[ct] = (s_col[buf][0][c] + s_col[buf][1][c]) + (s_col[buf][2][c] + s_col[buf][3][c]);
+        }
+      };
+      float p[NT], o[NT];
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        p[ct] = o[ct] = 0.0f;
+#pragma unroll
+        for (int u = 0; u < RT; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            S[u][ct][r] *= decay;
+            p[ct] = fmaf(S[u][ct][r], k[u][r] * ki, p[ct]);
+          }
+      }
+      total(p, 0);
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        const float v = Elem<T>::get(static_cast<const T*>(a.v) + t * a.v_stride + h * D + c0 + 16 * ct + n);
+        const float x = (v - p[ct]) * beta;
+#pragma unroll
+        for (int u = 0; u < RT; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            S[u][ct][r] = fmaf(k[u][r] * ki, x, S[u][ct][r]);
+            o[ct] = fmaf(S[u][ct][r], q[u][r] * qi, o[ct]);
+          }
+      }
+      total(o, 1);
+      if (wave == 0 && G == 0) {
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) put(t, ct, o[ct]);
+      }
+    }
+  };
+
+  u32x4_t unit[2];  // word r is (1, 0) or (0, 1) where 4 G + r is the lane's column
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    unit[0][r] = 4 * G + r == n ? 0x00003f80u : 0u;
+    unit[1][r] = unit[0][r] << 16;
+  }
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+  leave_s();
+  if (lo < hi) load(lo);
+  __syncthreads();
+  int turn = 0;
+  for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
+    // 1. v - e^g (K S) and Q S of the wave's tokens
+    u32x4_t kf[KS][NP], qf[KS][NP], tf[2][3], of[2][3];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      cur.k.operand(s, kf[s]);
+      cur.q.operand(s, qf[s]);
+    }
+    const f4_t fx = cur.fx, fy = cur.fy, fz = cur.fz;
+    const float end = cur.end;
+    float v[NT][4];
+    bool bad = cur.fine != 1.0f;
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[ct][r] = cur.v[ct][r];
+        bad |= !(fabsf(v[ct][r]) < 1e38f);
+      }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s >= ns) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t p[3];
+        split2(cur.t[s][e / 2][e % 2 * 2], cur.t[s][e / 2][e % 2 * 2 + 1], p);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) tf[s][i][e] = p[i];
+        split2(cur.o[s][e / 2][e % 2 * 2], cur.o[s][e / 2][e % 2 * 2 + 1], p);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) of[s][i][e] = p[i];
+      }
+    }
+    if (t0 + kChunk < hi) load(t0 + kChunk);
+    if (__ballot(bad) != 0 && lane == 0) s_bad[turn] = 1;
+    f4_t ks[NT], qs[NT];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      ks[ct] = qs[ct] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4_t f[3];
+        ld_parts(s_s[s][ct], lane, f);
+        ks[ct] = mma(kf[s], f, ks[ct]);
+        qs[ct] = mma(qf[s], f, qs[ct]);
+      }
+      leave_u(s_x[ct], f4_t{v[ct][0], v[ct][1], v[ct][2], v[ct][3]} - fx * ks[ct]);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const f4_t x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, kf[s][p]), __builtin_bit_cast(b8_t, unit[u]),
+                                                                f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+          reinterpret_cast<u32x2_t*>(&s_kt[2 * s + u][wave >> 1][p][lane])[wave & 1] =
+              u32x2_t{__builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u),
+                      __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302u)};
+        }
+    __syncthreads();
+    if (s_bad[turn] != 0) {  // (the same for all)
+      tokens(t0, min(hi, t0 + kChunk));
+      leave_s();
+      __syncthreads();
+      if (threadIdx.x == 0) s_bad[turn] = 0;  // (set again two chunks later)
+      continue;
+    }
+    // 2. u of the wave's tokens
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      f4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s >= ns) break;
+        u32x4_t f[3];
+        ld_parts(s_x[ct][s], lane, f);
+        u = mma(tf[s], f, u);
+      }
+      leave_u(s_u[ct], u);
+      leave_u(s_us[ct], u * fz);
+    }
+    __syncthreads();
+    // 3. the wave's rows of the state, the outputs of its tokens
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        f4_t x = S[u][ct] * end;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32x4_t f[3];
+        ld_parts(s_us[ct][s], lane, f);
+          u32x4_t kt[NP];
+          ld_parts(s_kt[RT * wave + u][s], lane, kt);
+          x = mma(kt, f, x);
+        }
+        S[u][ct] = x;
+      }
+    leave_s();
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
+      f4_t o = fy * qs[ct];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s >= ns) break;
+        u32x4_t f[3];
+        ld_parts(s_u[ct][s], lane, f);
+        o = mma(of[s], f, o);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t t = t0 + 16 * wave + 4 * G + r;
+        if (t < hi) put(t, ct, o[r]);
+      }
+    }
+    __syncthreads();
+  }
+  if (to < 0) return;
+#pragma unroll
+  for (int u = 0; u < RT; ++u)
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        st_once(a.state + uint64_t(to) * a.slot_stride + (size_t(h) * D + d0 + CH * r + u) * D + c0 + 16 * ct + n, S[u][ct][r]);
+}
+
+// ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per (chunk, value head), 4 dims a lane -------------------
+template <int D, class T>
+__global__ void __launch_bounds__(256) k_delta_gnorm(PromptArgs pa) {
+  const DeltaArgs& a = pa.d;
+  constexpr int LPR = D / 4, RG = 256 / LPR;
+  const int c = threadIdx.x % LPR * 4;
+  const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV;
+  const int row = a.r.row_of(b, kChunkShift, threadIdx.x & 63);
+  uint32_t lo, hi;
+  if (row < 0 || !a.r.range(row, &lo, &hi)) return;
+  const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
+  if (t0 >= hi) return;
+  const uint32_t end = min(hi, t0 + kChunk);
+  float w[4];
+  ld_row(a.norm_w + c, w);
+  for (uint32_t t = t0 + threadIdx.x / LPR; t - threadIdx.x / LPR < end; t += RG) {  // (all lanes: the sums below)
+    const uint32_t at = min(t, end - 1);
+    float o[4], z[4], s2 = 0.0f;
+    ld_row(pa.o32 + (size_t(at) * a.NV + h) * D + c, o);
+    ld_row(static_cast<const T*>(a.z) + at * a.z_stride + h * D + c, z);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s2 = fmaf(o[e], o[e], s2);
+#pragma unroll
+    for (int m = 1; m < LPR; m <<= 1) s2 = pair_sum(s2, m);
+    const float rr = 1.0f / sqrtf(s2 / float(D) + a.eps);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = w[e] * (o[e] * rr) * delta_silu(z[e]);
+    if (t < end) st_row(static_cast<T*>(a.out) + t * a.out_stride + h * D + c, o);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------
+struct PromptPlan {
+  bool ok = false;
+  uint64_t chunks = 0;  // (chunk, value head) pairs
+  size_t off_o = 0, bytes = 0;
+};
+PromptPlan prompt_plan(const chpe_delta_states* s, uint32_t tokens, uint32_t rows, bool norm) {
+  PromptPlan p;
+  const uint64_t blocks = (uint64_t(tokens) >> kChunkShift) + rows, vw = uint64_t(s->v_heads) * s->head_dim;
+  if (tokens > kMaxTokens || rows > kMaxTokens || blocks * s->v_heads > kMaxItems / 256) return p;
+  p.chunks = blocks * s->v_heads;
+  if ((uint64_t(rows) * s->v_heads + 7) / 8 * 8 * (s->head_dim / 16) > kMaxItems / 256) return p;
+  p.off_o = p.chunks * kChunkFloats * 4;
+  p.bytes = p.off_o + (norm ? tokens * vw * 4 : 0);
+  p.ok = true;
+  return p;
+}
+
+template <int D, class T>
+bool launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t st) {
+  const uint64_t items = (uint64_t(a.d.r.rows) * a.d.NV + 7) / 8 * 8;
+  if (a.d.r.tokens != 0 && !launch(&k_delta_prep<D, T>, p.chunks, 256, st, a)) return false;
+  if (!launch(&k_delta_scan<D, T, 1>, items * (D / 16), 256, st, a)) return false;
+  return !a.o32 || a.d.r.tokens == 0 || launch(&k_delta_gnorm<D, T>, p.chunks, 256, st, a);
+}
+template <int D>
+bool launch_prompt(const PromptArgs& a, const PromptPlan& p, int type, hipStream_t st) {
+  return type == 0   ? launch_prompt<D, float>(a, p, st)
+         : type == 1 ? launch_prompt<D, _Float16>(a, p, st)
+                     : launch_prompt<D, Bf16>(a, p, st);
+}
+
+}  // namespace
+}  // namespace chpe
+
+using namespace chpe;
+
+extern "C" size_t chpe_delta_prompt_workspace(const chpe_delta_states* states, uint32_t tokens, uint32_t rows, int norm) {
+  if (!delta_states_ok(states)) return 0;
+  const PromptPlan p = prompt_plan(states, tokens, rows, norm != 0);
+  return p.ok ? p.bytes : 0;
+}
+
+extern "C" int chpe_delta_prompt(const chpe_delta_states* states, const chpe_delta_tokens* t, uint32_t tokens,
+                                 uint32_t rows, const int32_t* starts, const int32_t* slot_in, const int32_t* slot_out,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  PromptArgs a{};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!delta_from(states, t, tokens, rows, starts, slot_in, slot_out, &a.d) || !stream_here(st)) return -1;
+  if (rows == 0) return 0;
+  const PromptPlan p = prompt_plan(states, tokens, rows, t->z != nullptr);
+  if (!p.ok || !starts || !workspace || !aligned16(workspace)) return -1;
+  if (workspace_bytes < p.bytes) return -2;
+  a.chunks = static_cast<float*>(workspace);
+  a.o32 = t->z ? a.chunks + p.off_o / 4 : nullptr;
+  return (states->head_dim == 128 ? launch_prompt<128>(a, p, t->type, st) : launch_prompt<64>(a, p, t->type, st)) ? 0 : -3;
+}

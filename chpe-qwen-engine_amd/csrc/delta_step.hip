@@ -147,20 +147,3 @@ extern "C" int chpe_delta_step(const chpe_delta_states* states, const chpe_delta
   if (rows == 0) return 0;
   return (states->head_dim == 128 ? launch_step<128>(a, t->type, st) : launch_step<64>(a, t->type, st)) ? 0 : -3;
 }
-
-extern "C" size_t chpe_delta_prompt_workspace(const chpe_delta_states* states, uint32_t tokens, uint32_t rows, int norm) {
-  if (!delta_states_ok(states) || tokens > kMaxTokens || uint64_t(rows) * states->v_heads > kMaxItems / 256) return 0;
-  return 256;
-}
-
-extern "C" int chpe_delta_prompt(const chpe_delta_states* states, const chpe_delta_tokens* t, uint32_t tokens,
-                                 uint32_t rows, const int32_t* starts, const int32_t* slot_in, const int32_t* slot_out,
-                                 void* workspace, size_t workspace_bytes, void* stream) {
-  DeltaArgs a{};
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!delta_from(states, t, tokens, rows, starts, slot_in, slot_out, &a) || !stream_here(st)) return -1;
-  if (rows == 0) return 0;
-  if (!starts || !workspace || !aligned16(workspace) || uint64_t(rows) * a.NV > kMaxItems / 256) return -1;
-  if (workspace_bytes < chpe_delta_prompt_workspace(states, tokens, rows, t->z != nullptr)) return -2;
-  return (states->head_dim == 128 ? launch_step<128>(a, t->type, st) : launch_step<64>(a, t->type, st)) ? 0 : -3;
-}
