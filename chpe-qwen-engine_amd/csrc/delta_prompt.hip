@@ -17,10 +17,11 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// What a chunk of a value head leaves for the scan, in the order of its lanes: u's matrix T diag(b) and o's matrix,
-// rows of 16 tokens as products of 16 x 32 (mma below), then per token the factors of K S, Q S and k u^T, then e^G.
-constexpr int kFrag = 512;                              // floats of 16 x 32 values
-__device__ __host__ constexpr int frag_of(int w) { return w < 2 ? w : 2 * w - 2; }  // row w's first of w / 2 + 1
+// What a chunk of a value head leaves for the scan, as operands (mma below): u's matrix T diag(b) and o's matrix in
+// fragments of 16 x 32, row w of 16 tokens in w / 2 + 1 of them; then per token the factors of K S, Q S and k u^T, e^G
+// and whether all is finite.
+constexpr int kFrag = 3 * 256;  // words
+__device__ __host__ constexpr int frag_of(int w) { return w < 2 ? w : 2 * w - 2; }  // row w's first
 constexpr int kOffO = 6 * kFrag, kOffScale = 12 * kFrag, kChunkFloats = kOffScale + 256;
 
 struct PromptArgs {
@@ -73,16 +74,21 @@ __device__ __forceinline__ f4_t mma16(f4_t a, f4_t b, f4_t c) {
   return c;
 }
 
-// A token's key or query row in a wave that holds 16 tokens: lane (G, i) = (lane / 16, lane % 16) has dims G D / 4 ..
-// of token i, 4 groups of D / 16.  Product s of D / 32 takes dims 2 s, 2 s + 1 of every group of every lane: the inner
-// index of a product is free as long as both sides agree, and so 16-bit rows are operands as they come.
+// A token's key or query row in a wave that holds 16 tokens: lane (G, i) = (lane / 16, lane % 16) has every fourth 16
+// bytes of token i, from the G-th on (the four lanes of a token load next to each other).  Product s of D / 32 takes
+// the next 8 of each lane's dims, in halves u: the inner index of a product is free as long as both sides agree, and
+// so 16-bit rows are operands as they come.
 template <int D, class T>
 struct Row16 {
-  static constexpr int W = D / 4 * int(sizeof(T)) / 16, KS = D / 32, GW = D / 32;  // GW: words of a group in 16 bits
+  static constexpr int W = D / 4 * int(sizeof(T)) / 16;
   u32x4_t w[W];
-  __device__ void load(const T* p) {
+  // the dim of product s, half u, element r < 4
+  static __device__ constexpr int dim(int G, int s, int u, int r) {
+    return sizeof(T) == 4 ? 32 * s + 16 * u + 4 * G + r : 32 * s + 8 * G + 4 * u + r;
+  }
+  __device__ void load(const T* row, int G) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = gld(reinterpret_cast<const u32x4_t*>(p) + i);
+    for (int i = 0; i < W; ++i) w[i] = gld(reinterpret_cast<const u32x4_t*>(row) + 4 * i + G);
   }
   __device__ void clear() {
 #pragma unroll
@@ -104,18 +110,17 @@ struct Row16 {
     }
   }
   __device__ void operand(int s, u32x4_t (&out)[kParts<T>]) const {
+    if constexpr (__is_same(T, Bf16)) {
+      out[0] = w[s];
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if constexpr (__is_same(T, Bf16)) {
-        const int e = GW * r + s;
-        out[0][r] = w[e / 4][e % 4];
-      } else {
+      for (int e = 0; e < 4; ++e) {
         float x, y;
         uint32_t p[kParts<T>];
-        pair(2 * (GW * r + s), &x, &y);
+        pair(8 * s + 2 * e, &x, &y);
         split2(x, y, p);
 #pragma unroll
-        for (int i = 0; i < kParts<T>; ++i) out[i][r] = p[i];
+        for (int i = 0; i < kParts<T>; ++i) out[i][e] = p[i];
       }
     }
   }
@@ -131,6 +136,34 @@ struct Row16 {
     return pair_sum(pair_sum(a + b, 16), 32);
   }
 };
+
+// one element as it lies in memory, and its value
+template <class T>
+struct Raw {
+  static __device__ uint16_t bits(const T* p) { return gld(reinterpret_cast<const uint16_t*>(p)); }
+  static __device__ float value(uint16_t b) {
+    if constexpr (__is_same(T, Bf16)) return bf2f(b);
+    else return h2f(b);
+  }
+};
+template <>
+struct Raw<float> {
+  static __device__ float bits(const float* p) { return gld(p); }
+  static __device__ float value(float b) { return b; }
+};
+
+// a read of LDS that transposes 4 x 16 values of 16 bits among 16 lanes
+__device__ __forceinline__ u32x2_t ld_transposed(const u32x2_t* p) {
+  typedef short s4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(p)));
+}
+
+// a barrier for what lies in LDS: loads from memory stay on their way (__syncthreads would wait for them)
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 // Keys and queries whose squares leave this range, and gates that are NaN, make a chunk run token by token: the
 // products above take keys before their norm, and 0 times what is not finite would reach earlier tokens.
@@ -164,9 +197,8 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
   float* out = pa.chunks + size_t(blockIdx.x) * kChunkFloats;
   Row16<D, T> kr, qr;
   if (mine < nt) {
-    const size_t at = kh * D + G * (D / 4);
-    kr.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + at);
-    qr.load(static_cast<const T*>(a.q) + (t0 + mine) * a.q_stride + at);
+    kr.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + kh * D, G);
+    qr.load(static_cast<const T*>(a.q) + (t0 + mine) * a.q_stride + kh * D, G);
   } else {
     kr.clear();
     qr.clear();
@@ -218,6 +250,24 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
       sc[193] = all ? 1.0f : 0.0f;
     }
   }
+  // row `wave` of a matrix, as the scan's operands
+  auto leave = [&](float* dst, const f4_t (&v)[4]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s > wave >> 1) break;
+      u32x4_t f[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t p[3];
+        split2(v[2 * s + e / 2][e % 2 * 2], v[2 * s + e / 2][e % 2 * 2 + 1], p);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) f[i][e] = p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        *reinterpret_cast<u32x4_t*>(dst + (frag_of(wave) + s) * kFrag + (i * 64 + lane) * 4) = f[i];
+    }
+  };
   // tiles (j, i) transposed: lane (G, n) gets tokens j = 16 jt + 4 G + r of i = 16 it + n
   f4_t At[4];
   const int R = 3 - wave;
@@ -235,10 +285,9 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
     u32x4_t qf[KS][NP];
 #pragma unroll
     for (int s = 0; s < KS; ++s) qr.operand(s, qf[s]);
-    float* o = out + kOffO + frag_of(wave) * kFrag;
+    f4_t o[4];
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) {
-      if (jt > (wave | 1)) break;
       f4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
       if (jt <= wave) {
 #pragma unroll
@@ -249,8 +298,9 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
         }
         v = weight(wave, jt, v, false, s_rq[16 * wave + n]);
       }
-      *reinterpret_cast<f4_t*>(o + (jt * 64 + lane) * 4) = v;
+      o[jt] = v;
     }
+    leave(out + kOffO, o);
   }
   {
     u32x4_t kf[KS][NP];
@@ -313,32 +363,31 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
       Tt[j] = mma16(d, acc, f4_t{0.0f, 0.0f, 0.0f, 0.0f});
     }
   }
-  float* o = out + frag_of(wave) * kFrag;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j > (wave | 1)) break;
-    const f4_t be = *reinterpret_cast<const f4_t*>(&s_beta[16 * j + 4 * G]);
-    *reinterpret_cast<f4_t*>(o + (j * 64 + lane) * 4) = Tt[j] * be;
-  }
+  for (int j = 0; j < 4; ++j) Tt[j] *= *reinterpret_cast<const f4_t*>(&s_beta[16 * j + 4 * G]);
+  leave(out, Tt);
 }
 
 // ---- the state over a row's chunks --------------------------------------------------------------------------------
-// A workgroup takes 16 NT columns of a value head's state over all chunks of a row; wave w holds D / 4 of its rows and
-// 16 tokens of a chunk.  A chunk is three steps with a barrier behind each, what one leaves to the others in LDS as
-// operands: v - e^g (K S) of the wave's tokens (Q S with it); u of its tokens; its rows of S (o with it).  The next
-// chunk's keys, queries, values and matrices are loaded meanwhile.
-// Keys as operands of k u^T have tokens inside: a product with a selection of unit vectors turns the wave's 16 tokens
-// of an operand of K S into that order, exactly.
+// A workgroup takes 16 NT columns of a value head's state over all chunks of a row.  A chunk is three steps with a
+// barrier behind each, what one leaves to the others in LDS as operands.  Four waves carry the state, each with 16 tokens
+// of a chunk and D / 4 rows of S: 1. v - e^g (K S) of their tokens, 2. u of their tokens, 3. their rows of S.  Four others
+// form the outputs of 16 tokens each: Q S in 1., o in 3.  Everybody loads its own operands of the next chunk where the
+// others leave it time.  (Rows behind the end are the last token again: b, and so u, is 0 there.)
+// Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
 template <int D, class T, int NT>
-__global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
+__global__ void __launch_bounds__(512, 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
-  constexpr int NP = kParts<T>, KS = D / 32, RT = D / 64, CB = D / (16 * NT), CH = D / 16;
-  __shared__ u32x4_t s_kt[D / 16][2][NP][64];
+  constexpr int NP = kParts<T>, KS = D / 32, RT = D / 64, CB = D / (16 * NT);
+  constexpr int KR = D / 8 + 2;  // a token's keys in LDS, with room so that neither side's accesses meet in a few banks
+  __shared__ u32x4_t s_k[NP][kChunk][KR];
   __shared__ u32x4_t s_s[KS][NT][3][64];
   __shared__ u32x4_t s_x[NT][2][3][64], s_u[NT][2][3][64], s_us[NT][2][3][64];
+  __shared__ __align__(16) float s_scale[2][256];
   __shared__ float s_red[2][4], s_col[2][4][16 * NT];
   __shared__ int s_bad[2];
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+  const int wave8 = uniform(threadIdx.x >> 6), wave = wave8 & 3, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
+  const bool carry = wave8 < 4;  // (uniform)
   // the column blocks of a head on one XCD (workgroup i runs on XCD i % 8), whose L2 they share
   const uint32_t item = blockIdx.x / (8 * CB) * 8 + blockIdx.x % 8, c0 = blockIdx.x / 8 % CB * (16 * NT);
   if (item >= a.r.rows * a.NV) return;
@@ -347,43 +396,29 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
   float fill;
   if (!a.r.range(row, &lo, &hi)) return;
   const int slot = a.r.before(row, &fill), to = a.r.after(row);
-  // the wave's rows of the state: dim(u, r) = CH (4 G + r) + 2 wave + u (D = 64: + wave)
-  const int d0 = CH * 4 * G + RT * wave;
+  // the wave's rows of the state: those of its two (D = 64: of its one) operands' elements
+  auto dim = [&](int r, int u) { return RT == 2 ? Row16<D, T>::dim(G, wave, u, r) : Row16<D, T>::dim(G, wave >> 1, wave & 1, r); };
   f4_t S[RT][NT];
+  if (carry) {
 #pragma unroll
-  for (int u = 0; u < RT; ++u)
+    for (int u = 0; u < RT; ++u)
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct)
+      for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S[u][ct][r] = slot >= 0 ? gld(a.state + uint64_t(slot) * a.slot_stride + (size_t(h) * D + d0 + CH * r + u) * D + c0 + 16 * ct + n) : fill;
+        for (int r = 0; r < 4; ++r)
+          S[u][ct][r] = slot >= 0 ? gld(a.state + uint64_t(slot) * a.slot_stride + (size_t(h) * D + dim(r, u)) * D + c0 + 16 * ct + n) : fill;
+  }
   // leaves S as operands
   auto leave_s = [&] {
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      if constexpr (RT == 2) {
-        u32x4_t f[3];
+      uint32_t p[2 * RT][3];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          uint32_t p[3];
-          split2(S[0][ct][r], S[1][ct][r], p);
+      for (int e = 0; e < 2 * RT; ++e) split2(S[e / 2][ct][e % 2 * 2], S[e / 2][ct][e % 2 * 2 + 1], p[e]);
 #pragma unroll
-          for (int i = 0; i < 3; ++i) f[i][r] = p[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 3; ++i) s_s[wave][ct][i][lane] = f[i];
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          uint32_t p[3];
-          split2(S[0][ct][r], S[0][ct][r + 1], p);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) {
-            uint16_t* d = reinterpret_cast<uint16_t*>(&s_s[wave >> 1][ct][i][lane]) + (wave & 1);
-            d[2 * r] = uint16_t(p[i]);
-            d[2 * r + 2] = uint16_t(p[i] >> 16);
-          }
-        }
+      for (int i = 0; i < 3; ++i) {
+        if constexpr (RT == 2) s_s[wave][ct][i][lane] = u32x4_t{p[0][i], p[1][i], p[2][i], p[3][i]};
+        else reinterpret_cast<u32x2_t*>(&s_s[wave >> 1][ct][i][lane])[wave & 1] = u32x2_t{p[0][i], p[1][i]};
       }
     }
   };
@@ -396,46 +431,32 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
     for (int i = 0; i < 3; ++i)
       reinterpret_cast<u32x2_t*>(&dst[wave >> 1][i][lane])[wave & 1] = u32x2_t{p[0][i], p[1][i]};
   };
-  // what a chunk reads
+  using Bits = __typeof__(Raw<T>::bits(nullptr));
   const int ns = (wave >> 1) + 1;  // products of 32 tokens in the wave's row of a matrix
-  struct Chunk {
-    Row16<D, T> k, q;
-    f4_t t[2][2], o[2][2], fx, fy, fz;
-    float v[NT][4], end, fine;
-  } cur;
   const uint32_t first = a.r.first_block(row, lo, kChunkShift);
-  auto load = [&](uint32_t t0) {
-    const uint32_t last = hi - 1 - t0, at = kh * D + G * (D / 4);
-    const float* m = pa.chunks + (size_t(first + ((t0 - lo) >> kChunkShift)) * a.NV + h) * kChunkFloats;
-    const uint32_t mine = 16 * wave + n;
-    if (mine <= last) {
-      cur.k.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + at);
-      cur.q.load(static_cast<const T*>(a.q) + (t0 + mine) * a.q_stride + at);
-    } else {
-      cur.k.clear();
-      cur.q.clear();
-    }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (s >= ns) break;
-        const float* f = m + (frag_of(wave) + s) * kFrag + (u * 64 + lane) * 4;
-        cur.t[s][u] = gld(reinterpret_cast<const f4_t*>(f));
-        cur.o[s][u] = gld(reinterpret_cast<const f4_t*>(f + kOffO));
-      }
-    const float* sc = m + kOffScale + 16 * wave + 4 * G;
-    cur.fx = gld(reinterpret_cast<const f4_t*>(sc));
-    cur.fy = gld(reinterpret_cast<const f4_t*>(sc + 64));
-    cur.fz = gld(reinterpret_cast<const f4_t*>(sc + 128));
-    cur.end = gld(m + kOffScale + 192);
-    cur.fine = gld(m + kOffScale + 193);
+  const T* v_at = static_cast<const T*>(a.v) + h * D + c0 + n;
+  auto chunk_at = [&](uint32_t t0) { return pa.chunks + (size_t(first + ((t0 - lo) >> kChunkShift)) * a.NV + h) * kChunkFloats; };
+  // the values of the tokens of a wave that carries S
+  Bits v16[NT][4];  // (as they lie there: widened here, they would be waited for at once)
+  auto load_v = [&](uint32_t t0) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint32_t i = 16 * wave + 4 * G + r;
+      const T* p = v_at + min(t0 + 16 * wave + 4 * G + r, hi - 1) * a.v_stride;
 #pragma unroll
-      for (int ct = 0; ct < NT; ++ct)
-        cur.v[ct][r] = i <= last ? Elem<T>::get(static_cast<const T*>(a.v) + (t0 + i) * a.v_stride + h * D + c0 + 16 * ct + n) : 0.0f;
+      for (int ct = 0; ct < NT; ++ct) v16[ct][r] = Raw<T>::bits(p + 16 * ct);
+    }
+  };
+  // 16 tokens' keys or queries, the wave's row of a chunk's matrix
+  auto load_x = [&](Row16<D, T>& x, const void* p, uint64_t stride, uint32_t t0) {
+    x.load(static_cast<const T*>(p) + min(t0 + 16 * wave + n, hi - 1) * stride + kh * D, G);
+  };
+  auto load_m = [&](u32x4_t (&m)[2][3], uint32_t t0, int at) {
+    const float* p = chunk_at(t0) + at + frag_of(wave) * kFrag + lane * 4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s >= ns) break;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) m[s][i] = gld(reinterpret_cast<const u32x4_t*>(p + s * kFrag + i * 256));
     }
   };
   auto put = [&](uint32_t t, int ct, float v) {
@@ -443,16 +464,16 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
     if (pa.o32) pa.o32[size_t(t) * a.NV * D + at] = v;
     else static_cast<T*>(a.out)[t * a.out_stride + at] = Elem<T>::put(v);
   };
-  // the recurrence itself, token by token (inputs that are not finite: see in_range)
+  // the recurrence itself, token by token (inputs that are not finite: see in_range), by the waves that carry S: three barriers a token
   auto tokens = [&](uint32_t t0, uint32_t t1) {
     const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
     for (uint32_t t = t0; t < t1; ++t) {
-      float k[RT][4], q[RT][4], k2 = 0.0f, q2 = 0.0f;
+      float k[RT][4], q[RT][4], k2 = 0.0f, q2 = 0.0f, p[NT], o[NT];
 #pragma unroll
       for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const size_t d = kh * D + d0 + CH * r + u;
+          const size_t d = kh * D + dim(r, u);
           k[u][r] = Elem<T>::get(static_cast<const T*>(a.k) + t * a.k_stride + d);
           q[u][r] = Elem<T>::get(static_cast<const T*>(a.q) + t * a.q_stride + d);
           k2 = fmaf(k[u][r], k[u][r], k2);
@@ -464,7 +485,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
         s_red[0][wave] = k2;
         s_red[1][wave] = q2;
       }
-      __syncthreads();
+      lds_barrier();
       k2 = (s_red[0][0] + s_red[0][1]) + (s_red[0][2] + s_red[0][3]);
       q2 = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
       const float ki = 1.0f / sqrtf(k2 + 1e-6f), qi = 1.0f / sqrtf(q2 + 1e-6f) * (1.0f / sqrtf(float(D)));
@@ -476,14 +497,13 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
           p[ct] = pair_sum(pair_sum(p[ct], 16), 32);
           if (G == 0) s_col[buf][wave][16 * ct + n] = p[ct];
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int ct = 0; ct < NT; ++ct) {
           const int c = 16 * ct + n;
           p[ct] = (s_col[buf][0][c] + s_col[buf][1][c]) + (s_col[buf][2][c] + s_col[buf][3][c]);
         }
       };
-      float p[NT], o[NT];
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
         p[ct] = o[ct] = 0.0f;
@@ -498,8 +518,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
       total(p, 0);
 #pragma unroll
       for (int ct = 0; ct < NT; ++ct) {
-        const float v = Elem<T>::get(static_cast<const T*>(a.v) + t * a.v_stride + h * D + c0 + 16 * ct + n);
-        const float x = (v - p[ct]) * beta;
+        const float x = (Elem<T>::get(v_at + t * a.v_stride + 16 * ct) - p[ct]) * beta;
 #pragma unroll
         for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -516,134 +535,175 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
     }
   };
 
-  u32x4_t unit[2];  // word r is (1, 0) or (0, 1) where 4 G + r is the lane's column
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    unit[0][r] = 4 * G + r == n ? 0x00003f80u : 0u;
-    unit[1][r] = unit[0][r] << 16;
-  }
-  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-  leave_s();
-  if (lo < hi) load(lo);
-  __syncthreads();
-  int turn = 0;
-  for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
-    // 1. v - e^g (K S) and Q S of the wave's tokens
-    u32x4_t kf[KS][NP], qf[KS][NP], tf[2][3], of[2][3];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      cur.k.operand(s, kf[s]);
-      cur.q.operand(s, qf[s]);
-    }
-    const f4_t fx = cur.fx, fy = cur.fy, fz = cur.fz;
-    const float end = cur.end;
-    float v[NT][4];
-    bool bad = cur.fine != 1.0f;
-#pragma unroll
-    for (int ct = 0; ct < NT; ++ct)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        v[ct][r] = cur.v[ct][r];
-        bad |= !(fabsf(v[ct][r]) < 1e38f);
-      }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      if (s >= ns) break;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t p[3];
-        split2(cur.t[s][e / 2][e % 2 * 2], cur.t[s][e / 2][e % 2 * 2 + 1], p);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) tf[s][i][e] = p[i];
-        split2(cur.o[s][e / 2][e % 2 * 2], cur.o[s][e / 2][e % 2 * 2 + 1], p);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) of[s][i][e] = p[i];
-      }
-    }
-    if (t0 + kChunk < hi) load(t0 + kChunk);
-    if (__ballot(bad) != 0 && lane == 0) s_bad[turn] = 1;
-    f4_t ks[NT], qs[NT];
+  // X S of the wave's tokens
+  auto times_s = [&](const u32x4_t (&x)[KS][NP], f4_t (&y)[NT]) {
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      ks[ct] = qs[ct] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      f4_t sum[2] = {f4_t{0.0f, 0.0f, 0.0f, 0.0f}, f4_t{0.0f, 0.0f, 0.0f, 0.0f}};  // (two chains of products)
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         u32x4_t f[3];
         ld_parts(s_s[s][ct], lane, f);
-        ks[ct] = mma(kf[s], f, ks[ct]);
-        qs[ct] = mma(qf[s], f, qs[ct]);
+        sum[s & 1] = mma(x[s], f, sum[s & 1]);
       }
-      leave_u(s_x[ct], f4_t{v[ct][0], v[ct][1], v[ct][2], v[ct][3]} - fx * ks[ct]);
+      y[ct] = sum[0] + sum[1];
+    }
+  };
+  // M x of the wave's row of a matrix
+  auto times_x = [&](const u32x4_t (&m)[2][3], const u32x4_t (&x)[2][3][64], f4_t y) {
+    f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4_t f[3];
+    ld_parts(x[0], lane, f);
+    y = mma(m[0], f, y);
+    if (ns > 1) {
+      ld_parts(x[1], lane, f);
+      sum = mma(m[1], f, sum);
+    }
+    return y + sum;
+  };
+  Row16<D, T> x16;
+  u32x4_t m16[2][3];
+  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+  int turn = 0;
+  if (!carry) {
+    f4_t f16;
+    auto load_scale = [&](uint32_t t0) {
+      if (wave == 0) f16 = gld(reinterpret_cast<const f4_t*>(chunk_at(t0) + kOffScale + lane * 4));
+    };
+    auto leave_scale = [&](int turn) {
+      if (wave == 0) *reinterpret_cast<f4_t*>(&s_scale[turn][lane * 4]) = f16;
+    };
+    u32x4_t xf[KS][NP];
+    auto take_x = [&] {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) x16.operand(s, xf[s]);
+    };
+    f4_t y[NT], done[NT];
+    uint32_t from = hi;  // tokens of `done`
+    auto store = [&] {
+      const uint32_t t = from + 16 * wave + 4 * G;
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t + r < hi) put(t + r, ct, done[ct][r]);
+    };
+    if (lo < hi) {
+      load_scale(lo);
+      load_x(x16, a.q, a.q_stride, lo);
+      load_m(m16, lo, kOffO);
+      leave_scale(0);
+      take_x();
+    }
+    lds_barrier();
+    for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
+      const uint32_t next = t0 + kChunk < hi ? t0 + kChunk : t0;  // (behind the last chunk: that one again, not used)
+      times_s(xf, y);
+      load_x(x16, a.q, a.q_stride, next);
+      load_scale(next);
+      const f4_t g = *reinterpret_cast<const f4_t*>(&s_scale[turn][64 + 16 * wave + 4 * G]);
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) y[ct] *= g;
+      lds_barrier();
+      store();
+      take_x();
+      if (s_bad[turn] != 0) {  // (the same for all)
+        for (uint32_t i = 3 * min(hi - t0, uint32_t(kChunk)); i != 0; --i) lds_barrier();
+        from = hi;
+      } else {
+        lds_barrier();
+#pragma unroll
+        for (int ct = 0; ct < NT; ++ct) done[ct] = times_x(m16, s_u[ct], y[ct]);
+        from = t0;
+      }
+      load_m(m16, next, kOffO);
+      leave_scale(turn ^ 1);
+      lds_barrier();
+    }
+    store();
+    return;
+  }
+
+  if (lo < hi) {
+    load_x(x16, a.k, a.k_stride, lo);
+    load_v(lo);
+    load_m(m16, lo, 0);
+  }
+  leave_s();
+  lds_barrier();
+  for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
+    const uint32_t next = t0 + kChunk < hi ? t0 + kChunk : t0;
+    // 1.
+    f4_t v[NT], y[NT];
+    u32x4_t xf[KS][NP];
+    bool bad = s_scale[turn][193] != 1.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      x16.operand(s, xf[s]);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) s_k[p][16 * wave + n][4 * s + G] = xf[s][p];
     }
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int r = 0; r < 4; ++r) {
+        v[ct][r] = Raw<T>::value(v16[ct][r]);
+        bad |= !(fabsf(v[ct][r]) < 1e38f);
+      }
+    if (__ballot(bad) != 0 && lane == 0) s_bad[turn] = 1;
+    times_s(xf, y);
+    const float* scale = s_scale[turn] + 16 * wave + 4 * G;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          const f4_t x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, kf[s][p]), __builtin_bit_cast(b8_t, unit[u]),
-                                                                f4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-          reinterpret_cast<u32x2_t*>(&s_kt[2 * s + u][wave >> 1][p][lane])[wave & 1] =
-              u32x2_t{__builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u),
-                      __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302u)};
-        }
-    __syncthreads();
+    for (int ct = 0; ct < NT; ++ct) leave_u(s_x[ct], v[ct] - *reinterpret_cast<const f4_t*>(scale) * y[ct]);
+    lds_barrier();
     if (s_bad[turn] != 0) {  // (the same for all)
       tokens(t0, min(hi, t0 + kChunk));
       leave_s();
-      __syncthreads();
-      if (threadIdx.x == 0) s_bad[turn] = 0;  // (set again two chunks later)
+      load_x(x16, a.k, a.k_stride, next);
+      load_v(next);
+      load_m(m16, next, 0);
+      lds_barrier();
+      if (wave == 0 && lane == 0) s_bad[turn] = 0;  // (set again two chunks later)
       continue;
     }
-    // 2. u of the wave's tokens
+    // 2.
+    f4_t u[NT];
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) u[ct] = times_x(m16, s_x[ct], f4_t{0.0f, 0.0f, 0.0f, 0.0f});
+    load_x(x16, a.k, a.k_stride, next);
+    load_v(next);
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      f4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
+      leave_u(s_u[ct], u[ct]);
+      leave_u(s_us[ct], u[ct] * *reinterpret_cast<const f4_t*>(scale + 128));
+    }
+    const float end = s_scale[turn][192];
+    lds_barrier();
+    // 3.
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const int at = 4 * (RT == 2 ? wave : wave >> 1), half = RT == 2 ? u : wave & 1;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (s >= ns) break;
-        u32x4_t f[3];
-        ld_parts(s_x[ct][s], lane, f);
-        u = mma(tf[s], f, u);
-      }
-      leave_u(s_u[ct], u);
-      leave_u(s_us[ct], u * fz);
-    }
-    __syncthreads();
-    // 3. the wave's rows of the state, the outputs of its tokens
+        u32x4_t kt[NP];
 #pragma unroll
-    for (int u = 0; u < RT; ++u)
-#pragma unroll
-      for (int ct = 0; ct < NT; ++ct) {
-        f4_t x = S[u][ct] * end;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4_t f[3];
-        ld_parts(s_us[ct][s], lane, f);
-          u32x4_t kt[NP];
-          ld_parts(s_kt[RT * wave + u][s], lane, kt);
-          x = mma(kt, f, x);
+        for (int p = 0; p < NP; ++p) {
+          // lane n of a group of 16 names 4 keys of token n / 4 and gets key n of the four tokens
+          const u32x2_t lo4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 4 * G + n / 4][at + n % 4]) + half);
+          const u32x2_t hi4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 16 + 4 * G + n / 4][at + n % 4]) + half);
+          kt[p] = u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y};
         }
-        S[u][ct] = x;
-      }
-    leave_s();
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      f4_t o = fy * qs[ct];
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s >= ns) break;
-        u32x4_t f[3];
-        ld_parts(s_u[ct][s], lane, f);
-        o = mma(of[s], f, o);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t t = t0 + 16 * wave + 4 * G + r;
-        if (t < hi) put(t, ct, o[r]);
+        for (int ct = 0; ct < NT; ++ct) {
+          u32x4_t f[3];
+          ld_parts(s_us[ct][s], lane, f);
+          S[u][ct] = mma(kt, f, s == 0 ? S[u][ct] * end : S[u][ct]);
+        }
       }
     }
-    __syncthreads();
+    load_m(m16, next, 0);
+    leave_s();
+    lds_barrier();
   }
   if (to < 0) return;
 #pragma unroll
@@ -652,7 +712,7 @@ __global__ void __launch_bounds__(256) k_delta_scan(PromptArgs pa) {
     for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        st_once(a.state + uint64_t(to) * a.slot_stride + (size_t(h) * D + d0 + CH * r + u) * D + c0 + 16 * ct + n, S[u][ct][r]);
+        st_once(a.state + uint64_t(to) * a.slot_stride + (size_t(h) * D + dim(r, u)) * D + c0 + 16 * ct + n, S[u][ct][r]);
 }
 
 // ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per (chunk, value head), 4 dims a lane -------------------
@@ -697,7 +757,7 @@ PromptPlan prompt_plan(const chpe_delta_states* s, uint32_t tokens, uint32_t row
   const uint64_t blocks = (uint64_t(tokens) >> kChunkShift) + rows, vw = uint64_t(s->v_heads) * s->head_dim;
   if (tokens > kMaxTokens || rows > kMaxTokens || blocks * s->v_heads > kMaxItems / 256) return p;
   p.chunks = blocks * s->v_heads;
-  if ((uint64_t(rows) * s->v_heads + 7) / 8 * 8 * (s->head_dim / 16) > kMaxItems / 256) return p;
+  if ((uint64_t(rows) * s->v_heads + 7) / 8 * 8 * (s->head_dim / 16) > kMaxItems / 512) return p;
   p.off_o = p.chunks * kChunkFloats * 4;
   p.bytes = p.off_o + (norm ? tokens * vw * 4 : 0);
   p.ok = true;
@@ -708,7 +768,12 @@ template <int D, class T>
 bool launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t st) {
   const uint64_t items = (uint64_t(a.d.r.rows) * a.d.NV + 7) / 8 * 8;
   if (a.d.r.tokens != 0 && !launch(&k_delta_prep<D, T>, p.chunks, 256, st, a)) return false;
-  if (!launch(&k_delta_scan<D, T, 1>, items * (D / 16), 256, st, a)) return false;
+  static const int nt = getenv("NT") ? atoi(getenv("NT")) : 1;
+  bool ok = false;
+  if (nt == 1) ok = launch(&k_delta_scan<D, T, 1>, items * (D / 16), 512, st, a);
+  if (nt == 2) ok = launch(&k_delta_scan<D, T, 2>, items * (D / 32), 512, st, a);
+  if constexpr (sizeof(T) == 2) if constexpr (__is_same(T, Bf16)) if (nt == 4) ok = launch(&k_delta_scan<D, T, 4>, items * (D / 64), 512, st, a);
+  if (!ok) return false;
   return !a.o32 || a.d.r.tokens == 0 || launch(&k_delta_gnorm<D, T>, p.chunks, 256, st, a);
 }
 template <int D>
