@@ -4,7 +4,6 @@
 #include "paged.hpp"
 
 namespace chpe {
-namespace {
 
 // The rows of a call: row r is tokens starts[r] .. starts[r + 1] - 1 (starts null: token r alone); its state is
 // read from slot_in[r] and left in slot_out[r].
@@ -66,6 +65,10 @@ struct DeltaArgs {
   uint32_t NV, NK;
   float eps;
 };
+
+// The rows of up to `longest` tokens, token by token (delta_step.hip).
+bool launch_delta_tokens(const DeltaArgs& a, uint32_t head_dim, int type, uint32_t longest, hipStream_t st);
+namespace {
 
 // N consecutive elements (16 bytes, or all N where they are fewer) widened to f32, and rounded from it
 template <int N>

@@ -27,6 +27,12 @@ constexpr int kOffO = 6 * kFrag, kOffScale = 12 * kFrag, kChunkFloats = kOffScal
 struct PromptArgs {
   DeltaArgs d;
   float *chunks, *o32;  // o32 [token][NV][D]: the outputs before the gated norm, null without it
+  uint32_t shortest;    // tokens of the shortest row that is theirs: the others run token by token (delta_step.hip)
+
+  // the row's range; false for a row that is left out or not theirs
+  __device__ bool range(uint32_t row, uint32_t* lo, uint32_t* hi) const {
+    return d.r.range(row, lo, hi) && *hi - *lo >= shortest;
+  }
 };
 
 // ---- products in 32 bits on the 16-bit matrix cores ---------------------------------------------------------
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
   const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
   const int row = a.r.row_of(b, kChunkShift, lane);
   uint32_t lo, hi;
-  if (row < 0 || !a.r.range(row, &lo, &hi)) return;
+  if (row < 0 || !pa.range(row, &lo, &hi)) return;
   const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
   if (t0 >= hi) return;
   const uint32_t nt = min(hi - t0, uint32_t(kChunk)), mine = 16 * wave + n;
@@ -375,8 +381,10 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
 // form the outputs of 16 tokens each: Q S in 1., o in 3.  Everybody loads its own operands of the next chunk where the
 // others leave it time.  (Rows behind the end are the last token again: b, and so u, is 0 there.)
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
+// (Two workgroups on a CU where their LDS allows it: 24 prompts of up to 4097 bf16 tokens of the 9B layout 1.45 ms, with
+// one 1.88.)
 template <int D, class T, int NT>
-__global__ void __launch_bounds__(512, 2) k_delta_scan(PromptArgs pa) {
+__global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 4 : 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
   constexpr int NP = kParts<T>, KS = D / 32, RT = D / 64, CB = D / (16 * NT);
   constexpr int KR = D / 8 + 2;  // a token's keys in LDS, with room so that neither side's accesses meet in a few banks
@@ -394,7 +402,7 @@ __global__ void __launch_bounds__(512, 2) k_delta_scan(PromptArgs pa) {
   const uint32_t h = item % a.NV, row = item / a.NV, kh = h / (a.NV / a.NK);
   uint32_t lo, hi;
   float fill;
-  if (!a.r.range(row, &lo, &hi)) return;
+  if (!pa.range(row, &lo, &hi)) return;
   const int slot = a.r.before(row, &fill), to = a.r.after(row);
   // the wave's rows of the state: those of its two (D = 64: of its one) operands' elements
   auto dim = [&](int r, int u) { return RT == 2 ? Row16<D, T>::dim(G, wave, u, r) : Row16<D, T>::dim(G, wave >> 1, wave & 1, r); };
@@ -724,7 +732,7 @@ __global__ void __launch_bounds__(256) k_delta_gnorm(PromptArgs pa) {
   const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV;
   const int row = a.r.row_of(b, kChunkShift, threadIdx.x & 63);
   uint32_t lo, hi;
-  if (row < 0 || !a.r.range(row, &lo, &hi)) return;
+  if (row < 0 || !pa.range(row, &lo, &hi)) return;
   const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
   if (t0 >= hi) return;
   const uint32_t end = min(hi, t0 + kChunk);
@@ -764,15 +772,30 @@ PromptPlan prompt_plan(const chpe_delta_states* s, uint32_t tokens, uint32_t row
   return p;
 }
 
+// Rows of up to this many tokens run token by token, each state read and written once for all of them, and no launch
+// knows the rows' lengths: where there are several rows both kinds are launched and leave the other's rows alone.
+constexpr uint32_t kShort = 8;
+
 template <int D, class T>
 bool launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t st) {
   const uint64_t items = (uint64_t(a.d.r.rows) * a.d.NV + 7) / 8 * 8;
   if (a.d.r.tokens != 0 && !launch(&k_delta_prep<D, T>, p.chunks, 256, st, a)) return false;
-  static const int nt = getenv("NT") ? atoi(getenv("NT")) : 1;
-  bool ok = false;
-  if (nt == 1) ok = launch(&k_delta_scan<D, T, 1>, items * (D / 16), 512, st, a);
-  if (nt == 2) ok = launch(&k_delta_scan<D, T, 2>, items * (D / 32), 512, st, a);
-  if constexpr (sizeof(T) == 2) if constexpr (__is_same(T, Bf16)) if (nt == 4) ok = launch(&k_delta_scan<D, T, 4>, items * (D / 64), 512, st, a);
+  // Columns of a workgroup: 16, so that few rows reach all CUs; where head dim 128 gives more workgroups than those, 32 (one
+  // row of 1000 tokens of the 9B layout in f32 84 us with 16, 100 with 32; four rows 305 and 234; bf16 53 / 66 and
+  // 141 / 137; at head dim 64 16 is ahead or within 7 % throughout), and 64 for many bf16 rows, where LDS holds
+  // that (8 rows 270 us with 32, 247 with 64; 6 rows 199 and 230).
+  const uint64_t many = uint64_t(a.d.r.rows) * a.d.NV;
+  bool ok;
+  if constexpr (D == 128 && __is_same(T, Bf16)) {
+    ok = many * 2 >= 512  ? launch(&k_delta_scan<D, T, 4>, items * 2, 512, st, a)
+         : many * 8 > 256 ? launch(&k_delta_scan<D, T, 2>, items * 4, 512, st, a)
+                          : launch(&k_delta_scan<D, T, 1>, items * 8, 512, st, a);
+  } else if constexpr (D == 128) {
+    ok = many * 8 > 256 ? launch(&k_delta_scan<D, T, 2>, items * 4, 512, st, a)
+                        : launch(&k_delta_scan<D, T, 1>, items * 8, 512, st, a);
+  } else {
+    ok = launch(&k_delta_scan<D, T, 1>, items * 4, 512, st, a);
+  }
   if (!ok) return false;
   return !a.o32 || a.d.r.tokens == 0 || launch(&k_delta_gnorm<D, T>, p.chunks, 256, st, a);
 }
@@ -806,5 +829,9 @@ extern "C" int chpe_delta_prompt(const chpe_delta_states* states, const chpe_del
   if (workspace_bytes < p.bytes) return -2;
   a.chunks = static_cast<float*>(workspace);
   a.o32 = t->z ? a.chunks + p.off_o / 4 : nullptr;
+  const bool some_short = rows > 1 || tokens <= kShort, some_long = tokens > kShort;
+  a.shortest = some_short ? kShort + 1 : 0;
+  if (some_short && !launch_delta_tokens(a.d, states->head_dim, t->type, kShort, st)) return -3;
+  if (!some_long) return 0;
   return (states->head_dim == 128 ? launch_prompt<128>(a, p, t->type, st) : launch_prompt<64>(a, p, t->type, st)) ? 0 : -3;
 }

@@ -7,29 +7,53 @@ namespace chpe {
 namespace {
 using namespace dev;
 
-// A workgroup takes one value head of one row: 256 threads hold its state, 4 columns of D / RG rows each (RG groups of
-// rows), 16 bytes a lane, read once and written once.  The column sums (S^T k before the update, S^T q after it) meet
+// A workgroup takes one value head of one row: its threads hold the state, 4 columns of D / 16 or D / 8 rows each (16 or 8
+// groups of rows), 16 bytes a lane, read once and written once.  The column sums (S^T k before the update, S^T q after it) meet
 // over the groups of a wave, then over the waves in LDS, in a fixed order.
-// Bound by memory: 2 x 64 KB a head of 128.
-template <int D, class T>
-__global__ void __launch_bounds__(256) k_delta_step(DeltaArgs a) {
-  constexpr int LPR = D / 4, RG = 256 / LPR, RPT = D / RG, PL = D / 64;
+// Bound by memory: 2 x 64 KB a head of 128 (256 rows of the 9B layout, 1.08 GB: 195 us, 5.5 TB/s; one row, 4 MB: 5 us, two
+// memory latencies and the sums).  ONE: a token per row, with nothing to load ahead; else rows of up to `longest`, the
+// next token's inputs on the way meanwhile.  (16 groups for one token at D = 128: 256 rows take 207 us with 8; 8 for
+// more: 32 rows of 5 tokens take 54 us with 16, 46 with 8.)
+template <int D, bool ONE>
+constexpr int kGroups = D == 64 || ONE ? 16 : 8;
+template <int D, class T, bool ONE>
+__global__ void __launch_bounds__(kGroups<D, ONE> * D / 4) k_delta_step(DeltaArgs a, uint32_t longest) {
+  constexpr int LPR = D / 4, RG = kGroups<D, ONE>, RPT = D / RG, PL = D / 64, NW = RG * LPR / 64;
   const uint32_t h = blockIdx.x % a.NV, row = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR * 4, rg = tid / LPR;
   __shared__ float s_q[D], s_k[D];
-  __shared__ __align__(16) float s_sum[2][4][D];
+  __shared__ __align__(16) float s_sum[2][NW][D];
   uint32_t lo, hi;
   float fill;
   const bool there = a.r.range(row, &lo, &hi);
   const int slot = a.r.before(row, &fill), to = a.r.after(row);
-  if (!there) return;
+  if (!there || hi - lo > longest) return;
+  const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
+  float w[4];
+  if (a.z) ld_row(a.norm_w + c, w);
+  struct Token {
+    float v[4], x[PL], y[PL], z[4], a, b;
+  };
+  auto load = [&](uint32_t t) {
+    Token k;
+    ld_row(static_cast<const T*>(a.q) + t * a.q_stride + kh * D + lane * PL, k.x);
+    ld_row(static_cast<const T*>(a.k) + t * a.k_stride + kh * D + lane * PL, k.y);
+    ld_row(static_cast<const T*>(a.v) + t * a.v_stride + h * D + c, k.v);
+    if (a.z) ld_row(static_cast<const T*>(a.z) + t * a.z_stride + h * D + c, k.z);
+    k.a = gld(a.a + t * a.a_stride + h);
+    k.b = gld(a.b + t * a.b_stride + h);
+    return k;
+  };
+  Token next;  // (requested before the state, whose slot is on its way)
+  if (ONE || lo < hi) next = load(lo);
   float s[RPT][4];
-  const size_t at = size_t(h) * D * D + size_t(rg) * D + c;
+  // (the head's place is the same for all lanes: scalar registers hold the rows' addresses)
+  const uint32_t at = rg * D + c;
   if (slot >= 0) {
-    const float* S = a.state + uint64_t(slot) * a.slot_stride + at;
+    const float* S = a.state + uniform(slot) * a.slot_stride + size_t(h) * D * D;
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
-      const f32x4_t v = ld_once(reinterpret_cast<const f32x4_t*>(S + size_t(r) * RG * D));
+      const f32x4_t v = ld_once(reinterpret_cast<const f32x4_t*>(S + r * RG * D + at));
       s[r][0] = v.x, s[r][1] = v.y, s[r][2] = v.z, s[r][3] = v.w;
     }
   } else {
@@ -49,24 +73,17 @@ __global__ void __launch_bounds__(256) k_delta_step(DeltaArgs a) {
     __syncthreads();
     float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(&s_sum[buf][w][c]);
       t.x += x.x, t.y += x.y, t.z += x.z, t.w += x.w;
     }
     p[0] = t.x, p[1] = t.y, p[2] = t.z, p[3] = t.w;
   };
-  const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
   for (uint32_t t = lo; t < hi; ++t) {
-    float v[4], x[PL], y[PL], z[4], w[4];
-    ld_row(static_cast<const T*>(a.q) + t * a.q_stride + kh * D + lane * PL, x);
-    ld_row(static_cast<const T*>(a.k) + t * a.k_stride + kh * D + lane * PL, y);
-    ld_row(static_cast<const T*>(a.v) + t * a.v_stride + h * D + c, v);
-    if (a.z) {
-      ld_row(static_cast<const T*>(a.z) + t * a.z_stride + h * D + c, z);
-      ld_row(a.norm_w + c, w);
-    }
-    const float decay = expf(delta_log_decay(A_log, gld(a.a + t * a.a_stride + h) + dt));
-    const float beta = delta_beta(gld(a.b + t * a.b_stride + h));
+    const Token now = next;
+    const float(&v)[4] = now.v, (&x)[PL] = now.x, (&y)[PL] = now.y, (&z)[4] = now.z;
+    if (!ONE && t + 1 < hi) next = load(t + 1);
+    const float decay = expf(delta_log_decay(A_log, now.a + dt)), beta = delta_beta(now.b);
     float q2 = 0.0f, k2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
@@ -74,7 +91,7 @@ __global__ void __launch_bounds__(256) k_delta_step(DeltaArgs a) {
       k2 = fmaf(y[i], y[i], k2);
     }
     const float qi = 1.0f / sqrtf(wave_sum(q2) + 1e-6f) * (1.0f / sqrtf(float(D))), ki = 1.0f / sqrtf(wave_sum(k2) + 1e-6f);
-    if (t != lo) __syncthreads();  // (s_q, s_k)
+    if (!ONE && t != lo) __syncthreads();  // (s_q, s_k)
     if (wave == 0) {
 #pragma unroll
       for (int i = 0; i < PL; ++i) {
@@ -119,21 +136,28 @@ __global__ void __launch_bounds__(256) k_delta_step(DeltaArgs a) {
     if (rg == 0) st_row(static_cast<T*>(a.out) + t * a.out_stride + h * D + c, o);
   }
   if (to >= 0) {
-    float* S = a.state + uint64_t(to) * a.slot_stride + at;
+    float* S = a.state + uniform(to) * a.slot_stride + size_t(h) * D * D;
 #pragma unroll
-    for (int r = 0; r < RPT; ++r) st_row(S + size_t(r) * RG * D, s[r]);
+    for (int r = 0; r < RPT; ++r) st_row(S + r * RG * D + at, s[r]);
   }
 }
 
 template <int D>
-bool launch_step(const DeltaArgs& a, int type, hipStream_t st) {
+bool launch_step(const DeltaArgs& a, int type, uint32_t longest, hipStream_t st) {
   const uint64_t blocks = uint64_t(a.r.rows) * a.NV;
-  return type == 0   ? launch(&k_delta_step<D, float>, blocks, 256, st, a)
-         : type == 1 ? launch(&k_delta_step<D, _Float16>, blocks, 256, st, a)
-                     : launch(&k_delta_step<D, Bf16>, blocks, 256, st, a);
+  auto run = [&](auto one, auto many) { return a.r.starts ? launch(many, blocks, kGroups<D, false> * D / 4, st, a, longest)
+                                                                        : launch(one, blocks, kGroups<D, true> * D / 4, st, a, longest); };
+  return type == 0   ? run(&k_delta_step<D, float, true>, &k_delta_step<D, float, false>)
+         : type == 1 ? run(&k_delta_step<D, _Float16, true>, &k_delta_step<D, _Float16, false>)
+                     : run(&k_delta_step<D, Bf16, true>, &k_delta_step<D, Bf16, false>);
 }
 
 }  // namespace
+
+bool launch_delta_tokens(const DeltaArgs& a, uint32_t head_dim, int type, uint32_t longest, hipStream_t st) {
+  return head_dim == 128 ? launch_step<128>(a, type, longest, st) : launch_step<64>(a, type, longest, st);
+}
+
 }  // namespace chpe
 
 using namespace chpe;
@@ -143,7 +167,7 @@ extern "C" int chpe_delta_step(const chpe_delta_states* states, const chpe_delta
   DeltaArgs a{};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (!delta_from(states, t, rows, rows, nullptr, slot_in, slot_out, &a) || !stream_here(st)) return -1;
-  if (uint64_t(rows) * a.NV > kMaxItems / 256) return -1;
+  if (uint64_t(rows) * a.NV > kMaxItems / 512) return -1;
   if (rows == 0) return 0;
-  return (states->head_dim == 128 ? launch_step<128>(a, t->type, st) : launch_step<64>(a, t->type, st)) ? 0 : -3;
+  return launch_delta_tokens(a, states->head_dim, t->type, 1, st) ? 0 : -3;
 }
