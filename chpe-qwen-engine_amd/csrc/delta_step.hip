@@ -17,7 +17,7 @@ using namespace dev;
 template <int D, bool ONE>
 constexpr int kGroups = D == 64 || ONE ? 16 : 8;
 template <int D, class T, bool ONE>
-__global__ void __launch_bounds__(kGroups<D, ONE> * D / 4) k_delta_step(DeltaArgs a, uint32_t longest) {
+__global__ void __launch_bounds__((kGroups<D, ONE> * D / 4)) k_delta_step(DeltaArgs a, uint32_t longest) {
   constexpr int LPR = D / 4, RG = kGroups<D, ONE>, RPT = D / RG, PL = D / 64, NW = RG * LPR / 64;
   const uint32_t h = blockIdx.x % a.NV, row = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = tid % LPR * 4, rg = tid / LPR;
@@ -145,8 +145,10 @@ __global__ void __launch_bounds__(kGroups<D, ONE> * D / 4) k_delta_step(DeltaArg
 template <int D>
 bool launch_step(const DeltaArgs& a, int type, uint32_t longest, hipStream_t st) {
   const uint64_t blocks = uint64_t(a.r.rows) * a.NV;
-  auto run = [&](auto one, auto many) { return a.r.starts ? launch(many, blocks, kGroups<D, false> * D / 4, st, a, longest)
-                                                                        : launch(one, blocks, kGroups<D, true> * D / 4, st, a, longest); };
+  auto run = [&](auto one, auto many) {
+    return a.r.starts ? launch(many, blocks, kGroups<D, false> * D / 4, st, a, longest)
+                      : launch(one, blocks, kGroups<D, true> * D / 4, st, a, longest);
+  };
   return type == 0   ? run(&k_delta_step<D, float, true>, &k_delta_step<D, float, false>)
          : type == 1 ? run(&k_delta_step<D, _Float16, true>, &k_delta_step<D, _Float16, false>)
                      : run(&k_delta_step<D, Bf16, true>, &k_delta_step<D, Bf16, false>);
