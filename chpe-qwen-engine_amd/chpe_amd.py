@@ -31,7 +31,7 @@ ENGINE_SYMBOLS = [
     "chpe_time_steps", "chpe_time_stage", "chpe_time_stage_live", "chpe_stage_bytes", "chpe_step_bytes", "chpe_stage_kernel",
     "chpe_debug_gemv", "chpe_debug_flat_tile_weights", "chpe_debug_gemv_flat", "chpe_debug_gemv_cells", "chpe_debug_gemv_poly", "chpe_debug_gemv_raw", "chpe_debug_embed_row_cell",
     "chpe_debug_attention", "chpe_debug_attention_block", "chpe_attention_noalloc", "chpe_paged_append",
-    "chpe_paged_attention", "chpe_paged_attention_workspace", "chpe_paged_evict", "chpe_paged_evict_workspace",
+    "chpe_paged_attention", "chpe_paged_attention_workspace", "chpe_paged_prefix_attention", "chpe_paged_prefix_workspace", "chpe_paged_evict", "chpe_paged_evict_workspace",
     "chpe_delta_step", "chpe_delta_prompt", "chpe_delta_prompt_workspace", "chpe_delta_conv",
     "chpe_debug_deltanet_conv", "chpe_debug_deltanet_step",
 ]
@@ -149,6 +149,8 @@ def load_engine_lib():
                                       V, U64, V]),
             "chpe_paged_attention": (I, [P, U32, V, U32, V, U64, F, U32, V, U64, V, V, U64, V, S, V]),
             "chpe_paged_attention_workspace": (S, [P, U32, U32, I]),
+            "chpe_paged_prefix_attention": (I, [P, U32, V, U32, V, V, U32, U32, V, U64, F, V, U64, V, S, V]),
+            "chpe_paged_prefix_workspace": (S, [P, U32, U32, U32, U32]),
             "chpe_paged_evict": (I, [P, V, U32, U32, U32, U32, V, V, U64, V, V, V, V, V, S, V]),
             "chpe_paged_evict_workspace": (S, [P, U32]),
             "chpe_delta_step": (I, [DS, DT, U32, V, V, V]),
@@ -537,6 +539,39 @@ class KvPages:
         self._call("chpe_paged_attention", heads, lp, max_len, qp, width,
                    1.0 / self.head_dim ** 0.5 if scale is None else scale, window, op, width, wi, wo, stride, ws,
                    workspace.numel())
+        return out
+
+    def prefix_workspace(self, heads, groups, max_prefix, max_rest):
+        """Bytes that prefix_attention() needs for these sizes."""
+        if min(heads, groups, max_prefix, max_rest) < 0 or max(heads, groups, max_prefix, max_rest) > _U32_MAX:
+            raise ValueError("heads, groups, max_prefix and max_rest: from 0 to 2^32 - 1")
+        n = self.lib.chpe_paged_prefix_workspace(self._c, heads, groups, max_prefix, max_rest)
+        if n == 0 and self.rows:
+            raise ValueError("chpe_paged_prefix_workspace rejected the arguments")
+        return n
+
+    def prefix_attention(self, q, lens, group_rows, prefix_lens, max_prefix, max_rest, scale=None, out=None,
+                         workspace=None):
+        """chpe_paged_prefix_attention: q [rows, heads, head_dim] f32; rows group_rows[g] .. group_rows[g + 1] - 1 share
+        the first prefix_lens[g] <= max_prefix slots, which lie in the pages of the first of them, and have up to max_rest
+        slots of their own behind; lens [rows], group_rows [groups + 1], prefix_lens [groups] int32."""
+        f32, i32 = self._f32, self._i32
+        if q.dim() != 3:
+            raise ValueError("q: [rows, heads, head_dim]")
+        heads, width, groups = q.shape[1], q.shape[1] * self.head_dim, prefix_lens.numel()
+        if min(max_prefix, max_rest) < 0 or max(max_prefix, max_rest, groups) > _U32_MAX:
+            raise ValueError("max_prefix and max_rest: from 0 to 2^32 - 1")
+        qp = self._take(q, "q", f32, (self.rows, heads, self.head_dim))
+        if out is None:
+            out = self._torch.empty(q.shape, dtype=f32, device=self.device)
+        if workspace is None:
+            workspace = self._torch.empty(self.prefix_workspace(heads, groups, max_prefix, max_rest),
+                                          dtype=self._torch.uint8, device=self.device)
+        self._call("chpe_paged_prefix_attention", heads, self._take(lens, "lens", i32, (self.rows,)), groups,
+                   self._take(group_rows, "group_rows", i32, (groups + 1,)),
+                   self._take(prefix_lens, "prefix_lens", i32, (groups,)), max_prefix, max_rest, qp, width,
+                   1.0 / self.head_dim ** 0.5 if scale is None else scale, self._take(out, "out", f32, q.shape), width,
+                   self._take(workspace, "workspace", self._torch.uint8, (workspace.numel(),)), workspace.numel())
         return out
 
     def evict_workspace(self, max_len):

@@ -1,0 +1,322 @@
+// paged_prefix.hip -- chpe_paged_prefix_attention: the attention of one new token per row where groups of rows share
+// the first slots of their cache.  The softmax over a row's slots is joined from parts, so a group's prefix is read
+// once for the queries of all its rows (as if they were query heads of one row), the rest of a row for its own, and a
+// last launch joins them: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts s of a row.
+#include "paged_attention_kernels.hpp"
+
+namespace chpe {
+namespace {
+using namespace dev;
+
+struct PrefixArgs {
+  Pages c;
+  const float* q;
+  const int32_t *lens, *group_rows, *prefix_lens;
+  float *out, *part_ml, *part_acc;  // parts: [row][head][prefix splits, rest splits]
+  uint64_t q_stride, out_stride;
+  uint32_t rows, H, groups, max_prefix, max_rest;
+  uint32_t prefix_splits, prefix_chunk, rest_splits, rest_chunk, hz;
+  float scale;
+
+  static constexpr bool kScores = false;
+  __device__ bool eager() const { return false; }
+  __device__ uint32_t eager_slot(const Place&) const { return 0; }
+  __device__ bool whole() const { return false; }
+  template <int HD>
+  __device__ void leave_none(const Place&) const {}  // (the join goes by the lengths)
+
+  // group g's rows r0 .. r1 - 1 and prefix; false where they do not lie in the rows, or in max_prefix
+  __device__ bool group(uint32_t g, uint32_t* r0, uint32_t* r1, uint32_t* prefix) const {
+    *r0 = uint32_t(gld(group_rows + g));
+    *r1 = uint32_t(gld(group_rows + g + 1));
+    *prefix = uint32_t(gld(prefix_lens + g));
+    return *r0 <= *r1 && *r1 <= rows && *prefix <= max_prefix;
+  }
+  // the last group of which `first`(its first row, its number) <= x, 64 candidates a step; -1: none
+  template <class F>
+  __device__ int last_group(uint32_t x, F first) const {
+    if (groups == 0) return -1;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t at = 0, n = groups;
+    do {
+      const uint32_t step = (n + 63) / 64, g = at + min(lane * step, n - 1);
+      const uint64_t in = __ballot(lane * step < n && first(uint32_t(max(gld(group_rows + g), 0)), g) <= x);
+      if (in == 0) return -1;
+      const uint32_t last = 63u - uint32_t(__builtin_clzll(in));
+      at += last * step;
+      n = min(step, n - last * step);
+    } while (n > 1);
+    return int(at);
+  }
+  // where the row's own slots begin (0 in no group) and end; false for a length or a group that is not valid
+  __device__ bool row_range(uint32_t row, uint32_t* prefix, uint32_t* len) const {
+    const int g = last_group(row, [](uint32_t r, uint32_t) { return r; });
+    uint32_t r0, r1;
+    bool ok = true;
+    *prefix = 0;
+    if (g >= 0) {
+      ok = group(g, &r0, &r1, prefix);
+      if (ok && row >= r1) *prefix = 0;
+    }
+    *len = uint32_t(gld(lens + row));
+    return ok && *len <= 0x7fffffffu && (*len <= *prefix || *len - *prefix <= max_rest);
+  }
+};
+
+// a row's own slots: a workgroup's queries are query heads of one kv head
+struct RestArgs : PrefixArgs {
+  template <int HD>
+  __device__ const float* query(const Place& p, uint32_t i) const {
+    return q + p.row * q_stride + size_t(p.h0 + i) * HD;
+  }
+  __device__ uint32_t end_of(const Place& p, uint32_t) const { return p.end; }
+  __device__ size_t part_of(const Place& p, uint32_t i) const {
+    return (size_t(p.row) * H + p.h0 + i) * (prefix_splits + rest_splits) + prefix_splits + p.split;
+  }
+  template <int HT>
+  __device__ Place place_of() const {
+    Place p;
+    const uint32_t gq = H / c.KV;
+    uint32_t b = blockIdx.x;
+    p.split = (b + b / rest_splits) % rest_splits;  // (the last ones not all on one XCD)
+    b /= rest_splits;
+    const uint32_t z = b % hz;
+    b /= hz;
+    p.kvh = b % c.KV;
+    p.row = b / c.KV;
+    p.h0 = p.kvh * gq + z * HT;
+    p.nh = min(uint32_t(HT), gq - z * HT);
+    return p;
+  }
+  __device__ void place_slots(Place* p) const {
+    uint32_t len;
+    p->ok = row_range(p->row, &p->lo, &len);
+    p->begin = p->lo + p->split * rest_chunk;
+    p->end = p->ok ? min(len, p->begin + rest_chunk) : 0u;
+  }
+};
+
+// a group's prefix: a workgroup's queries are HT of all its rows' query heads of one kv head, row by row.  A launch does
+// not know the groups' sizes: group g's tiles have the numbers from (its first row) * gq / HT + g on.
+struct SharedArgs : PrefixArgs {
+  __device__ void at(const Place& p, uint32_t i, uint32_t* row, uint32_t* head) const {
+    const uint32_t gq = H / c.KV, x = p.h0 + min(i, p.nh - 1);
+    *row = p.row + x / gq;
+    *head = p.kvh * gq + x % gq;
+  }
+  template <int HD>
+  __device__ const float* query(const Place& p, uint32_t i) const {
+    uint32_t row, head;
+    at(p, i, &row, &head);
+    return q + row * q_stride + size_t(head) * HD;
+  }
+  __device__ uint32_t end_of(const Place& p, uint32_t i) const {
+    uint32_t row, head;
+    at(p, i, &row, &head);
+    return min(p.end, uint32_t(gld(lens + row)));
+  }
+  __device__ size_t part_of(const Place& p, uint32_t i) const {
+    uint32_t row, head;
+    at(p, i, &row, &head);
+    return (size_t(row) * H + head) * (prefix_splits + rest_splits) + p.split;
+  }
+  template <int HT>
+  __device__ Place place_of() const {
+    Place p;
+    const uint32_t gq = H / c.KV;
+    uint32_t b = blockIdx.x;
+    p.split = b % prefix_splits;
+    b /= prefix_splits;
+    p.kvh = b % c.KV;
+    b /= c.KV;
+    auto first = [&](uint32_t r, uint32_t g) { return uint32_t(uint64_t(r) * gq / HT) + g; };
+    const int g = last_group(b, first);
+    uint32_t r0 = 0, r1 = 0, prefix = 0;
+    p.ok = g >= 0 && group(g, &r0, &r1, &prefix);
+    const uint32_t n = (r1 - r0) * gq;
+    p.row = p.ok ? r0 : 0u;
+    p.h0 = p.ok ? (b - first(r0, g)) * HT : 0u;
+    p.ok = p.ok && p.h0 < n;
+    p.nh = p.ok ? min(uint32_t(HT), n - p.h0) : 1u;
+    p.len = p.ok ? prefix : 0u;
+    return p;
+  }
+  __device__ void place_slots(Place* p) const {
+    p->lo = 0;
+    p->begin = p->split * prefix_chunk;
+    p->end = min(p->len, p->begin + prefix_chunk);
+  }
+};
+
+// ---- the join: a workgroup per (row, query head), 256 / (HD / 4) parts at a time ----------------------------------
+template <int HD>
+__global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
+  constexpr int D4 = HD / 4, GR = 256 / D4;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint32_t h = blockIdx.x % a.H, row = blockIdx.x / a.H;
+  __shared__ __align__(16) float s_o[GR][HD];
+  __shared__ float s_f[2 * kMaxSplits];
+  uint32_t prefix, len;
+  const bool ok = a.row_range(row, &prefix, &len);
+  const uint32_t np = ok ? (prefix + a.prefix_chunk - 1) / a.prefix_chunk : 0u;
+  const uint32_t nr = ok && len > prefix ? (len - prefix + a.rest_chunk - 1) / a.rest_chunk : 0u, ns = np + nr;
+  const size_t base = size_t(blockIdx.x) * (a.prefix_splits + a.rest_splits);
+  auto place = [&](uint32_t s) { return base + (s < np ? s : a.prefix_splits + (s - np)); };
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  float M = -INFINITY, L = 0.0f;  // (every wave for itself)
+  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[place(s)].x);
+  M = wave_max(M);
+  if (M == -INFINITY) M = 0.0f;  // (no score above -inf)
+  for (uint32_t s = lane; s < ns; s += 64) {
+    const float2 x = ml[place(s)];
+    const float f = __builtin_amdgcn_exp2f(x.x - M);
+    L += x.y * f;
+    if (tid < 64) s_f[s] = f;
+  }
+  L = wave_sum(L);
+  __syncthreads();
+  f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t s = tid / D4; s < ns; s += GR) {
+    const float4 v = ld_f4(a.part_acc + place(s) * HD + tid % D4 * 4);
+    o += f4_t{v.x, v.y, v.z, v.w} * s_f[s];
+  }
+  *reinterpret_cast<f4_t*>(&s_o[tid / D4][tid % D4 * 4]) = o;
+  __syncthreads();
+  if (tid >= HD) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int g = 0; g < GR; ++g) v += s_o[g][tid];
+  v = !ok ? __builtin_nanf("") : (L == 0.0f ? 0.0f : v / L);
+  if (!(fabsf(v) < INFINITY) && ok && L == L) {
+    // an infinite sum counts whatever its part's factor, which may be 0
+    float inf = 0.0f;
+    for (uint32_t s = 0; s < ns; ++s) {
+      const float x = gld(a.part_acc + place(s) * HD + tid);
+      inf += fabsf(x) < INFINITY ? 0.0f : x;
+    }
+    if (inf != 0.0f) v = inf;
+  }
+  a.out[row * a.out_stride + size_t(h) * HD + tid] = v;
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------
+struct PrefixPlan {
+  bool ok = false;
+  uint32_t prefix_splits = 1, prefix_chunk = 1, rest_splits = 1, rest_chunk = 1, ht = 0, hz = 0, pt = 0;
+  uint64_t prefix_blocks = 0, rest_blocks = 0, joins = 0;
+  size_t off_acc = 0, bytes = 0;
+};
+
+PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, uint32_t max_prefix, uint32_t max_rest) {
+  PrefixPlan p;
+  const uint32_t gq = heads / c->kv_heads, step = (c->type == 0 ? 16 : 32) * tiles_at_once(c->head_dim);
+  const uint64_t large = (512 << 10) / (2 * c->head_dim * (c->type == 0 ? 4 : 2));  // slots
+  auto split = [&](uint64_t items, uint64_t want, uint32_t range, uint32_t* splits, uint32_t* chunk) {
+    const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step), some = std::max<uint64_t>(1, items);
+    uint64_t n = std::min<uint64_t>({std::max<uint64_t>((1024 + some - 1) / some, want), steps, kMaxSplits});
+    n = std::max<uint64_t>(1, std::min<uint64_t>(n, kMaxBlocks / some));
+    const uint64_t per = (steps + n - 1) / n;
+    *chunk = uint32_t(per * step);
+    *splits = uint32_t((steps + per - 1) / per);
+  };
+  const uint64_t in_all = uint64_t(c->rows) * heads;
+  if (in_all > kMaxBlocks) return p;
+  p.ht = c->type == 0 || (gq > 8 && c->head_dim <= kWaveDims) ? 16 : 8;
+  p.hz = (gq + p.ht - 1) / p.ht;
+  p.pt = c->type == 0 || c->head_dim <= kWaveDims ? 16 : 8;
+  const uint64_t rest = uint64_t(c->rows) * c->kv_heads * p.hz;
+  const uint64_t shared = (uint64_t(c->rows) * gq / p.pt + groups) * c->kv_heads;
+  if (shared > kMaxBlocks) return p;
+  split(rest, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
+  split(shared, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
+  p.rest_blocks = rest * p.rest_splits;
+  p.prefix_blocks = max_prefix == 0 || groups == 0 ? 0 : shared * p.prefix_splits;
+  p.joins = in_all;
+  const uint64_t places = in_all * (p.prefix_splits + p.rest_splits);
+  p.off_acc = (places * 8 + 255) / 256 * 256;
+  p.bytes = p.off_acc + places * c->head_dim * 4;
+  p.ok = true;
+  return p;
+}
+
+template <int HD, class Args>
+bool launch_part(const Args& a, int type, uint32_t ht, uint64_t blocks, hipStream_t st) {
+  const uint32_t thr = kWaves * 64;
+  if (type == 0) return launch(&k_paged_32<HD, Args>, blocks, thr, st, a);
+  if constexpr (HD <= 128) {
+    if (ht == 16)
+      return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2, Args>, blocks, thr, st, a)
+                       : launch(&k_paged_16<HD, Bf16, 8, 2, Args>, blocks, thr, st, a);
+  }
+  return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, Args>, blocks, thr, st, a)
+                   : launch(&k_paged_16<HD, Bf16, 8, 1, Args>, blocks, thr, st, a);
+}
+template <int HD>
+bool launch_prefix(const PrefixArgs& a, const PrefixPlan& p, int type, hipStream_t st) {
+  if (p.prefix_blocks != 0 && !launch_part<HD>(SharedArgs{a}, type, p.pt, p.prefix_blocks, st)) return false;
+  if (a.max_rest != 0 && !launch_part<HD>(RestArgs{a}, type, p.ht, p.rest_blocks, st)) return false;
+  return launch(&k_prefix_join<HD>, p.joins, 256, st, a);
+}
+
+bool prefix_shape_ok(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, uint32_t max_prefix, uint32_t max_rest) {
+  return heads != 0 && heads % c->kv_heads == 0 && heads <= 65536 && groups <= 0x7ffffffeu &&
+         uint64_t(max_prefix) + max_rest <= uint64_t(c->pages_per_row) * c->page_size;
+}
+
+}  // namespace
+}  // namespace chpe
+
+using namespace chpe;
+
+extern "C" size_t chpe_paged_prefix_workspace(const chpe_kv_pages* cache, uint32_t heads, uint32_t groups,
+                                              uint32_t max_prefix, uint32_t max_rest) {
+  Pages c;
+  if (!pages_from(cache, &c) || !prefix_shape_ok(cache, heads, groups, max_prefix, max_rest)) return 0;
+  const PrefixPlan p = prefix_plan(cache, heads, groups, max_prefix, max_rest);
+  return p.ok ? p.bytes : 0;
+}
+
+extern "C" int chpe_paged_prefix_attention(const chpe_kv_pages* cache, uint32_t heads, const int32_t* lens,
+                                           uint32_t groups, const int32_t* group_rows, const int32_t* prefix_lens,
+                                           uint32_t max_prefix, uint32_t max_rest, const float* q, uint64_t q_stride,
+                                           float scale, float* out, uint64_t out_stride, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  PrefixArgs a{};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!pages_from(cache, &a.c) || !stream_here(st) || !prefix_shape_ok(cache, heads, groups, max_prefix, max_rest)) return -1;
+  if (cache->rows == 0) return 0;
+  const uint64_t width = uint64_t(heads) * cache->head_dim;
+  if (!lens || !q || !out || !workspace || !aligned16(q) || !aligned16(out) || !aligned16(workspace)) return -1;
+  if (groups != 0 && (!group_rows || !prefix_lens)) return -1;
+  if (q_stride % 4 || out_stride % 4 || (cache->rows > 1 && (q_stride < width || out_stride < width))) return -1;
+  if (cache->rows > 1 && (q_stride > (uint64_t(1) << 60) / cache->rows || out_stride > (uint64_t(1) << 60) / cache->rows)) return -1;
+  const PrefixPlan p = prefix_plan(cache, heads, groups, max_prefix, max_rest);
+  if (!p.ok) return -1;
+  if (workspace_bytes < p.bytes) return -2;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.q = q;
+  a.lens = lens;
+  a.group_rows = group_rows;
+  a.prefix_lens = prefix_lens;
+  a.out = out;
+  a.part_ml = reinterpret_cast<float*>(ws);
+  a.part_acc = reinterpret_cast<float*>(ws + p.off_acc);
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.rows = cache->rows;
+  a.H = heads;
+  a.groups = groups;
+  a.max_prefix = max_prefix;
+  a.max_rest = max_rest;
+  a.prefix_splits = p.prefix_splits;
+  a.prefix_chunk = p.prefix_chunk;
+  a.rest_splits = p.rest_splits;
+  a.rest_chunk = p.rest_chunk;
+  a.hz = p.hz;
+  a.scale = scale;
+  const bool ok = cache->head_dim == 64    ? launch_prefix<64>(a, p, cache->type, st)
+                  : cache->head_dim == 128 ? launch_prefix<128>(a, p, cache->type, st)
+                                           : launch_prefix<256>(a, p, cache->type, st);
+  return ok ? 0 : -3;
+}

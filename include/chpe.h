@@ -278,6 +278,25 @@ int chpe_paged_attention(const chpe_kv_pages *cache, uint32_t heads, const int32
 /* bytes; 0 for arguments that the call refuses */
 size_t chpe_paged_attention_workspace(const chpe_kv_pages *cache, uint32_t heads, uint32_t max_len, int weights);
 
+/* chpe_paged_attention for rows that share a prefix (a system prompt, the samples of one prompt), which is read once
+ * for all of them: row r of group g (rows group_rows[g] .. group_rows[g + 1] - 1; group_rows [groups + 1], ascending, and
+ * prefix_lens [groups] on the device) has slots 0 .. prefix_lens[g] - 1 in the pages of the group's first row, whatever
+ * its own table holds there, and the slots behind them, up to lens[r] - 1, in its own pages.  A row in no group has no
+ * prefix.  max_prefix and max_rest bound the prefixes and what rows have behind them (and size the launches).  A row of
+ * length 0 gives zeros, one shorter than its prefix sees lens[r] slots of it; a row of a negative length or with more
+ * than max_rest slots of its own gives NaN, and so do the rows of a group whose rows or prefix are out of bounds or whose
+ * prefix has a page id outside the pool.  Everything else as chpe_paged_attention.
+ * workspace: chpe_paged_prefix_workspace bytes for the same cache, heads, groups and bounds, at a 16-byte boundary, any
+ * content; calls that may overlap need one each.
+ * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
+int chpe_paged_prefix_attention(const chpe_kv_pages *cache, uint32_t heads, const int32_t *lens, uint32_t groups,
+                                const int32_t *group_rows, const int32_t *prefix_lens, uint32_t max_prefix,
+                                uint32_t max_rest, const float *q, uint64_t q_stride, float scale, float *out,
+                                uint64_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
+/* bytes; 0 for arguments that the call refuses */
+size_t chpe_paged_prefix_workspace(const chpe_kv_pages *cache, uint32_t heads, uint32_t groups, uint32_t max_prefix,
+                                   uint32_t max_rest);
+
 /* Cuts every row to at most `budget` slots per kv head, each head its own: the slots whose position is
  * among the newest `recent` ones (above the head's newest minus recent) or below `sinks` stay, then those of the
  * largest weight (equal: the lower slot; NaN last); recent + sinks <= budget.  Of the kept slots those at
