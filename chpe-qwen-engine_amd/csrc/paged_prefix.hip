@@ -1,7 +1,7 @@
 // paged_prefix.hip -- chpe_paged_prefix_attention: the attention of one new token per row where groups of rows share
 // the first slots of their cache.  The softmax over a row's slots is joined from parts, so a group's prefix is read
-// once for the queries of all its rows (as if they were query heads of one row), the rest of a row for its own, and a
-// last launch joins them: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts s of a row.
+// once for the queries of all its rows (as if they were query heads of one row), the rest of a row for its own, both in one
+// launch, and a second one joins them: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the parts s of a row.
 #include "paged_attention_kernels.hpp"
 
 namespace chpe {
@@ -15,7 +15,7 @@ struct PrefixArgs {
   float *out, *part_ml, *part_acc;  // parts: [row][head][prefix splits, rest splits]
   uint64_t q_stride, out_stride;
   uint32_t rows, H, groups, max_prefix, max_rest;
-  uint32_t prefix_splits, prefix_chunk, rest_splits, rest_chunk, hz;
+  uint32_t prefix_splits, prefix_chunk, prefix_blocks, rest_splits, rest_chunk, hz;
   float scale;
 
   static constexpr bool kScores = false;
@@ -63,42 +63,10 @@ struct PrefixArgs {
   }
 };
 
-// a row's own slots: a workgroup's queries are query heads of one kv head
-struct RestArgs : PrefixArgs {
-  template <int HD>
-  __device__ const float* query(const Place& p, uint32_t i) const {
-    return q + p.row * q_stride + size_t(p.h0 + i) * HD;
-  }
-  __device__ uint32_t end_of(const Place& p, uint32_t) const { return p.end; }
-  __device__ size_t part_of(const Place& p, uint32_t i) const {
-    return (size_t(p.row) * H + p.h0 + i) * (prefix_splits + rest_splits) + prefix_splits + p.split;
-  }
-  template <int HT>
-  __device__ Place place_of() const {
-    Place p;
-    const uint32_t gq = H / c.KV;
-    uint32_t b = blockIdx.x;
-    p.split = (b + b / rest_splits) % rest_splits;  // (the last ones not all on one XCD)
-    b /= rest_splits;
-    const uint32_t z = b % hz;
-    b /= hz;
-    p.kvh = b % c.KV;
-    p.row = b / c.KV;
-    p.h0 = p.kvh * gq + z * HT;
-    p.nh = min(uint32_t(HT), gq - z * HT);
-    return p;
-  }
-  __device__ void place_slots(Place* p) const {
-    uint32_t len;
-    p->ok = row_range(p->row, &p->lo, &len);
-    p->begin = p->lo + p->split * rest_chunk;
-    p->end = p->ok ? min(len, p->begin + rest_chunk) : 0u;
-  }
-};
-
-// a group's prefix: a workgroup's queries are HT of all its rows' query heads of one kv head, row by row.  A launch does
-// not know the groups' sizes: group g's tiles have the numbers from (its first row) * gq / HT + g on.
-struct SharedArgs : PrefixArgs {
+// The parts.  A workgroup's queries are HT of the query heads of one kv head, row by row: of all rows of a group for a split
+// of its prefix (blocks up to prefix_blocks), of one row for a split of its own slots.  A launch does not know the
+// groups' sizes: group g's tiles of queries have the numbers from (its first row) * gq / HT + g on.
+struct PartArgs : PrefixArgs {
   __device__ void at(const Place& p, uint32_t i, uint32_t* row, uint32_t* head) const {
     const uint32_t gq = H / c.KV, x = p.h0 + min(i, p.nh - 1);
     *row = p.row + x / gq;
@@ -125,26 +93,46 @@ struct SharedArgs : PrefixArgs {
     Place p;
     const uint32_t gq = H / c.KV;
     uint32_t b = blockIdx.x;
-    p.split = b % prefix_splits;
-    b /= prefix_splits;
+    p.lo = 0;
+    p.ok = b < prefix_blocks;
+    if (p.ok) {
+      p.split = b % prefix_splits;
+      b /= prefix_splits;
+      p.kvh = b % c.KV;
+      b /= c.KV;
+      auto first = [&](uint32_t r, uint32_t g) { return uint32_t(uint64_t(r) * gq / HT) + g; };
+      const int g = last_group(b, first);
+      uint32_t r0 = 0, r1 = 0, prefix = 0;
+      const bool there = g >= 0 && group(g, &r0, &r1, &prefix);
+      const uint32_t n = there ? (r1 - r0) * gq : 0u, h0 = there ? (b - first(r0, g)) * HT : 0u;
+      p.row = h0 < n ? r0 : 0u;
+      p.h0 = h0 < n ? h0 : 0u;
+      p.nh = h0 < n ? min(uint32_t(HT), n - h0) : 1u;
+      p.len = h0 < n ? prefix : 0u;
+      return p;
+    }
+    b -= prefix_blocks;
+    p.split = (b + b / rest_splits) % rest_splits;  // (the last ones not all on one XCD)
+    b /= rest_splits;
+    const uint32_t z = b % hz;
+    b /= hz;
     p.kvh = b % c.KV;
-    b /= c.KV;
-    auto first = [&](uint32_t r, uint32_t g) { return uint32_t(uint64_t(r) * gq / HT) + g; };
-    const int g = last_group(b, first);
-    uint32_t r0 = 0, r1 = 0, prefix = 0;
-    p.ok = g >= 0 && group(g, &r0, &r1, &prefix);
-    const uint32_t n = (r1 - r0) * gq;
-    p.row = p.ok ? r0 : 0u;
-    p.h0 = p.ok ? (b - first(r0, g)) * HT : 0u;
-    p.ok = p.ok && p.h0 < n;
-    p.nh = p.ok ? min(uint32_t(HT), n - p.h0) : 1u;
-    p.len = p.ok ? prefix : 0u;
+    p.row = b / c.KV;
+    p.h0 = z * HT;
+    p.nh = min(uint32_t(HT), gq - z * HT);
     return p;
   }
   __device__ void place_slots(Place* p) const {
-    p->lo = 0;
-    p->begin = p->split * prefix_chunk;
-    p->end = min(p->len, p->begin + prefix_chunk);
+    if (p->ok) {
+      p->begin = p->split * prefix_chunk;
+      p->end = min(p->len, p->begin + prefix_chunk);
+      return;
+    }
+    uint32_t len;
+    const bool ok = row_range(p->row, &p->lo, &len);
+    p->begin = p->lo + p->split * rest_chunk;
+    p->end = ok ? min(len, p->begin + rest_chunk) : 0u;
+    p->split += prefix_splits;
   }
 };
 
@@ -203,7 +191,7 @@ __global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
 // ---- host -----------------------------------------------------------------------------------------------------
 struct PrefixPlan {
   bool ok = false;
-  uint32_t prefix_splits = 1, prefix_chunk = 1, rest_splits = 1, rest_chunk = 1, ht = 0, hz = 0, pt = 0;
+  uint32_t prefix_splits = 1, prefix_chunk = 1, rest_splits = 1, rest_chunk = 1, ht = 0, hz = 0;
   uint64_t prefix_blocks = 0, rest_blocks = 0, joins = 0;
   size_t off_acc = 0, bytes = 0;
 };
@@ -222,11 +210,12 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   };
   const uint64_t in_all = uint64_t(c->rows) * heads;
   if (in_all > kMaxBlocks) return p;
-  p.ht = c->type == 0 || (gq > 8 && c->head_dim <= kWaveDims) ? 16 : 8;
+  // queries of a workgroup: 16 where the registers allow them and the groups have as many
+  const bool many = gq > 8 || (max_prefix != 0 && groups != 0 && uint64_t(c->rows) * gq > 8 * uint64_t(groups));
+  p.ht = c->type == 0 || (many && c->head_dim <= kWaveDims) ? 16 : 8;
   p.hz = (gq + p.ht - 1) / p.ht;
-  p.pt = c->type == 0 || c->head_dim <= kWaveDims ? 16 : 8;
   const uint64_t rest = uint64_t(c->rows) * c->kv_heads * p.hz;
-  const uint64_t shared = (uint64_t(c->rows) * gq / p.pt + groups) * c->kv_heads;
+  const uint64_t shared = (uint64_t(c->rows) * gq / p.ht + groups) * c->kv_heads;
   if (shared > kMaxBlocks) return p;
   split(rest, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
   split(shared, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
@@ -240,23 +229,24 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   return p;
 }
 
-template <int HD, class Args>
-bool launch_part(const Args& a, int type, uint32_t ht, uint64_t blocks, hipStream_t st) {
-  const uint32_t thr = kWaves * 64;
-  if (type == 0) return launch(&k_paged_32<HD, Args>, blocks, thr, st, a);
-  if constexpr (HD <= 128) {
-    if (ht == 16)
-      return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2, Args>, blocks, thr, st, a)
-                       : launch(&k_paged_16<HD, Bf16, 8, 2, Args>, blocks, thr, st, a);
-  }
-  return type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, Args>, blocks, thr, st, a)
-                   : launch(&k_paged_16<HD, Bf16, 8, 1, Args>, blocks, thr, st, a);
-}
 template <int HD>
-bool launch_prefix(const PrefixArgs& a, const PrefixPlan& p, int type, hipStream_t st) {
-  if (p.prefix_blocks != 0 && !launch_part<HD>(SharedArgs{a}, type, p.pt, p.prefix_blocks, st)) return false;
-  if (a.max_rest != 0 && !launch_part<HD>(RestArgs{a}, type, p.ht, p.rest_blocks, st)) return false;
-  return launch(&k_prefix_join<HD>, p.joins, 256, st, a);
+bool launch_prefix(const PrefixArgs& x, const PrefixPlan& p, int type, hipStream_t st) {
+  const uint32_t thr = kWaves * 64;
+  const uint64_t blocks = p.prefix_blocks + (x.max_rest != 0 ? p.rest_blocks : 0);
+  const PartArgs a{x};
+  bool ok = true;
+  if (blocks != 0) {
+    if (type == 0) {
+      ok = launch(&k_paged_32<HD, PartArgs>, blocks, thr, st, a);
+    } else if (p.ht == 8) {
+      ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, PartArgs>, blocks, thr, st, a)
+                     : launch(&k_paged_16<HD, Bf16, 8, 1, PartArgs>, blocks, thr, st, a);
+    } else if constexpr (HD <= kWaveDims) {
+      ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2, PartArgs>, blocks, thr, st, a)
+                     : launch(&k_paged_16<HD, Bf16, 8, 2, PartArgs>, blocks, thr, st, a);
+    }
+  }
+  return ok && launch(&k_prefix_join<HD>, p.joins, 256, st, x);
 }
 
 bool prefix_shape_ok(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, uint32_t max_prefix, uint32_t max_rest) {
@@ -311,6 +301,7 @@ extern "C" int chpe_paged_prefix_attention(const chpe_kv_pages* cache, uint32_t 
   a.max_rest = max_rest;
   a.prefix_splits = p.prefix_splits;
   a.prefix_chunk = p.prefix_chunk;
+  a.prefix_blocks = uint32_t(p.prefix_blocks);
   a.rest_splits = p.rest_splits;
   a.rest_chunk = p.rest_chunk;
   a.hz = p.hz;
