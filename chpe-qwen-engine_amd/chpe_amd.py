@@ -635,12 +635,12 @@ class _OnDevice:
         """Address and token stride of a [tokens, ..] tensor that is contiguous within a token."""
         if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index:
             raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} on {self.device}")
-        width = 1
-        for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if n != 1 and st != width and t.numel():
+        st, width = t.stride(), 1
+        for i in range(len(st) - 1, 0, -1):
+            if st[i] != width and shape[i] != 1 and t.numel():
                 raise ValueError(f"{name}: contiguous within a token")
-            width *= n
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+            width *= shape[i]
+        return t.data_ptr(), st[0] if shape[0] > 1 else width
 
     def _rows(self, starts, slot_in, slot_out, rows):
         """The addresses of a call's rows: starts [rows + 1] (or None), slot_in and slot_out [rows], int32."""

@@ -182,7 +182,7 @@ inline bool delta_from(const chpe_delta_states* s, const chpe_delta_tokens* t, u
         !rows_ok(t->v, t->v_stride, vw, tokens, t->type) || !rows_ok(t->out, t->out_stride, vw, tokens, t->type))
       return false;
     if (t->z && !rows_ok(t->z, t->z_stride, vw, tokens, t->type)) return false;
-    if (!t->a || !t->b || !t->A_log || !t->dt_bias || (t->z == nullptr) != (t->norm_w == nullptr)) return false;
+    if (!t->a || !t->b || !t->A_log || !t->dt_bias || (t->z == nullptr) != (t->norm_w == nullptr) || !aligned16(t->norm_w)) return false;
     if (tokens > 1 && (t->a_stride < s->v_heads || t->b_stride < s->v_heads || t->a_stride > kMaxExtent / tokens ||
                        t->b_stride > kMaxExtent / tokens))
       return false;

@@ -333,14 +333,18 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
     if (jt <= R) *reinterpret_cast<f4_t*>(&s_A[16 * R + n][16 * jt + 4 * G]) = At[jt];
   __syncthreads();
   {
-    float t[16];  // column n of T_ww
+    float t[16];  // column n of T_ww; what a row has taken off the others first, so that few sums wait for each other
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float x = i == n ? 1.0f : 0.0f;
+    for (int i = 0; i < 16; ++i) t[i] = i == n ? 1.0f : 0.0f;
 #pragma unroll
-      for (int j = 0; j < i; ++j) x = fmaf(-s_A[16 * wave + i][16 * wave + j], t[j], x);
-      t[i] = x;
-    }
+    for (int j = 0; j < 16; j += 4)
+#pragma unroll
+      for (int i = j + 1; i < 16; ++i) {
+        const f4_t x = *reinterpret_cast<const f4_t*>(&s_A[16 * wave + i][16 * wave + j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < i) t[i] = fmaf(-x[e], t[j + e], t[i]);
+      }
     if (G == 0) {
 #pragma unroll
       for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(&s_diag[wave][n][i]) = make_float4(t[i], t[i + 1], t[i + 2], t[i + 3]);
@@ -723,34 +727,39 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
         st_once(a.state + uint64_t(to) * a.slot_stride + (size_t(h) * D + dim(r, u)) * D + c0 + 16 * ct + n, S[u][ct][r]);
 }
 
-// ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per (chunk, value head), 4 dims a lane -------------------
+// ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per 16 tokens of a (chunk, value head), 4 dims a lane ------
+constexpr int kNormTokens = 16;
 template <int D, class T>
 __global__ void __launch_bounds__(256) k_delta_gnorm(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
-  constexpr int LPR = D / 4, RG = 256 / LPR;
+  constexpr int LPR = D / 4, RG = 256 / LPR, PARTS = kChunk / kNormTokens;
   const int c = threadIdx.x % LPR * 4;
-  const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV;
+  const uint32_t part = blockIdx.x % PARTS, h = blockIdx.x / PARTS % a.NV, b = blockIdx.x / (PARTS * a.NV);
   const int row = a.r.row_of(b, kChunkShift, threadIdx.x & 63);
   uint32_t lo, hi;
   if (row < 0 || !pa.range(row, &lo, &hi)) return;
-  const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
+  const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk + part * kNormTokens;
   if (t0 >= hi) return;
-  const uint32_t end = min(hi, t0 + kChunk);
-  float w[4];
+  float w[4], o[kNormTokens / RG][4], z[kNormTokens / RG][4];
   ld_row(a.norm_w + c, w);
-  for (uint32_t t = t0 + threadIdx.x / LPR; t - threadIdx.x / LPR < end; t += RG) {  // (all lanes: the sums below)
-    const uint32_t at = min(t, end - 1);
-    float o[4], z[4], s2 = 0.0f;
-    ld_row(pa.o32 + (size_t(at) * a.NV + h) * D + c, o);
-    ld_row(static_cast<const T*>(a.z) + at * a.z_stride + h * D + c, z);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s2 = fmaf(o[e], o[e], s2);
+  for (int i = 0; i < kNormTokens / RG; ++i) {  // (behind the row's end: its last token again)
+    const size_t t = min(t0 + i * RG + threadIdx.x / LPR, hi - 1);
+    ld_row(pa.o32 + (t * a.NV + h) * D + c, o[i]);
+    ld_row(static_cast<const T*>(a.z) + t * a.z_stride + h * D + c, z[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kNormTokens / RG; ++i) {
+    const uint32_t t = t0 + i * RG + threadIdx.x / LPR;
+    float s2 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s2 = fmaf(o[i][e], o[i][e], s2);
 #pragma unroll
     for (int m = 1; m < LPR; m <<= 1) s2 = pair_sum(s2, m);
     const float rr = 1.0f / sqrtf(s2 / float(D) + a.eps);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = w[e] * (o[e] * rr) * delta_silu(z[e]);
-    if (t < end) st_row(static_cast<T*>(a.out) + t * a.out_stride + h * D + c, o);
+    for (int e = 0; e < 4; ++e) o[i][e] = w[e] * (o[i][e] * rr) * delta_silu(z[i][e]);
+    if (t < hi) st_row(static_cast<T*>(a.out) + t * a.out_stride + h * D + c, o[i]);
   }
 }
 
@@ -763,7 +772,7 @@ struct PromptPlan {
 PromptPlan prompt_plan(const chpe_delta_states* s, uint32_t tokens, uint32_t rows, bool norm) {
   PromptPlan p;
   const uint64_t blocks = (uint64_t(tokens) >> kChunkShift) + rows, vw = uint64_t(s->v_heads) * s->head_dim;
-  if (tokens > kMaxTokens || rows > kMaxTokens || blocks * s->v_heads > kMaxItems / 256) return p;
+  if (tokens > kMaxTokens || rows > kMaxTokens || blocks * s->v_heads > kMaxItems / 1024) return p;  // (the norm's launch)
   p.chunks = blocks * s->v_heads;
   if ((uint64_t(rows) * s->v_heads + 7) / 8 * 8 * (s->head_dim / 16) > kMaxItems / 512) return p;
   p.off_o = p.chunks * kChunkFloats * 4;
@@ -797,7 +806,7 @@ bool launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t st) {
     ok = launch(&k_delta_scan<D, T, 1>, items * 4, 512, st, a);
   }
   if (!ok) return false;
-  return !a.o32 || a.d.r.tokens == 0 || launch(&k_delta_gnorm<D, T>, p.chunks, 256, st, a);
+  return !a.o32 || a.d.r.tokens == 0 || launch(&k_delta_gnorm<D, T>, p.chunks * (kChunk / kNormTokens), 256, st, a);
 }
 template <int D>
 bool launch_prompt(const PromptArgs& a, const PromptPlan& p, int type, hipStream_t st) {

@@ -31,7 +31,6 @@ struct PagedAttnArgs {
   __device__ const float* query(const Place& p, uint32_t i) const {
     return q + p.row * q_stride + size_t(p.h0 + i) * HD;
   }
-  __device__ uint32_t end_of(const Place& p, uint32_t) const { return p.end; }
   __device__ size_t part_of(const Place& p, uint32_t i) const { return (size_t(p.row) * H + p.h0 + i) * splits + p.split; }
   template <int HT>
   __device__ Place place_of() const;
@@ -63,7 +62,7 @@ __device__ __forceinline__ Place PagedAttnArgs::place_of() const {
   const uint32_t z = b % a.hz;
   b /= a.hz;
   p.kvh = b % a.c.KV;
-  p.row = b / a.c.KV;
+  p.row = p.table = b / a.c.KV;
   p.h0 = p.kvh * gq + z * HT;
   p.nh = min(uint32_t(HT), gq - z * HT);
   return p;

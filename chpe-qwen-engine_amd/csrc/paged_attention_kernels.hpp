@@ -3,7 +3,7 @@
 // Args (a kernel's argument) says where a workgroup's queries, slots and results lie:
 //   place_of<HT>(), place_slots(&p)  its place and the slots of it
 //   eager(), eager_slot(p)           whether the first slot is known before the rows' lengths, and that slot
-//   query<HD>(p, i), end_of(p, i)    query i of the workgroup, and the end of the slots that it sees
+//   query<HD>(p, i)                  query i of the workgroup
 //   part_of(p, i), whole()           where its sums go; whether they are the output
 //   leave_none<HD>(p)                what a place without slots leaves
 //   kScores, scores, score_stride    whether the scores are left too, and where
@@ -19,10 +19,10 @@ using namespace dev;
 
 constexpr int kWaves = 4;  // of a workgroup
 
-// a workgroup's place: slots begin .. end - 1 of row `row`, whose range is lo .. len - 1, for query heads
-// h0 .. h0 + nh - 1
+// a workgroup's place: slots begin .. end - 1 in the pages of row `table`, of row `row`'s range lo .. len - 1, for query
+// heads h0 .. h0 + nh - 1
 struct Place {
-  uint32_t row, kvh, h0, nh, split, begin, end, lo, len;
+  uint32_t row, table, kvh, h0, nh, split, begin, end, lo, len;
   bool ok;
 };
 // ---- the sums of a split ------------------------------------------------------------------------------------
@@ -132,12 +132,12 @@ __device__ __forceinline__ bool all_finite(f4_t v) {
   return fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY && fabsf(v.w) < INFINITY;
 }
 template <class T, class Args>
-__device__ __forceinline__ f4_t non_finite_sum(const Args& a, const Place& p, uint32_t end, uint32_t dim, f4_t v) {
+__device__ __forceinline__ f4_t non_finite_sum(const Args& a, const Place& p, uint32_t dim, f4_t v) {
   f4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (uint32_t j = p.begin; j < end; ++j) {
+  for (uint32_t j = p.begin; j < p.end; ++j) {
     uint32_t page;
-    a.c.page_of(p.row, j, &page);  // (a bad one: the head's sum of weights is NaN and nothing comes here)
+    a.c.page_of(p.table, j, &page);  // (a bad one: the head's sum of weights is NaN and nothing comes here)
     const T* src = reinterpret_cast<const T*>(a.c.v) + a.c.at(page, p.kvh, j) + dim;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -214,7 +214,7 @@ __device__ __forceinline__ void leave(const Args& a, const Place& p, WaveSums<LA
     if (none(k)) break;
     f4_t* d = reinterpret_cast<f4_t*>(dst + dim_of(k));
     const f4_t v = *d;
-    if (!all_finite(v)) *d = non_finite_sum<T>(a, p, a.end_of(p, head), dim_of(k), v);
+    if (!all_finite(v)) *d = non_finite_sum<T>(a, p, dim_of(k), v);
   }
 }
 
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
   const int part = n / W, col = n % W;  // the column's part and head
   Place p = a.template place_of<HT>();
   TileRows<32, 2> rows{s_off[wave], 0, 0, false};
-  if (a.eager()) rows.next(a, p.row, a.eager_slot(p) + 32 * (wave / DS), a.c.capacity - 1, lane);
+  if (a.eager()) rows.next(a, p.table, a.eager_slot(p) + 32 * (wave / DS), a.c.capacity - 1, lane);
   a.place_slots(&p);
   if (p.begin >= p.end) return a.template leave_none<HD>(p);  // (the whole workgroup)
   uint32_t t = p.begin + 32 * (wave / DS);
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
       }
     }
   };
-  if (!a.eager()) rows.next(a, p.row, t, p.end - 1, lane);
+  if (!a.eager()) rows.next(a, p.table, t, p.end - 1, lane);
   // the queries: HD / 8 threads a head take 8 dims each (dims (G + 4 s) * 8 .. + 7 are what lanes of group G
   // need in step s); they are taken apart while the first tile's rows are on their way
   constexpr int TH = HD / 8;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
     rows.put(a, p, 0, lane);
     load_k(0);
     load_v(0);
-    rows.next(a, p.row, t + UNIT, p.end - 1, lane);
+    rows.next(a, p.table, t + UNIT, p.end - 1, lane);
   }
   if (qh < HT) {  // (whole groups of TH lanes)
     float top = 0.0f;
@@ -308,12 +308,10 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
   }
   __syncthreads();  // (the query operands)
   float mult[NT], m[NT], l[NT];
-  uint32_t end[NT];  // of the column's slots
   f4_t o[NT][VD];
 #pragma unroll
   for (int ht = 0; ht < NT; ++ht) {
     mult[ht] = s_mult[ht * W + col];
-    end[ht] = a.end_of(p, ht * W + col);
     m[ht] = -INFINITY;
     l[ht] = 0.0f;
 #pragma unroll
@@ -345,7 +343,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p.row, t + 2 * UNIT, p.end - 1, lane);
+      rows.next(a, p.table, t + 2 * UNIT, p.end - 1, lane);
     }
     if constexpr (DS > 1) {
       // (written anew two steps later, past the next step's barrier)
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
       for (int e = 0; e < 8; ++e) {
         const uint32_t j = t + (e >> 2) * 16 + 4 * G + (e & 3);
         s8[e] = sum_parts<W>(sc[ht][e >> 2][e & 3]);
-        top[e] = j < end[ht] ? s8[e] * mult[ht] : -INFINITY;
+        top[e] = j < p.end ? s8[e] * mult[ht] : -INFINITY;
         mx = fmaxf(mx, top[e]);
       }
       if constexpr (Args::kScores) {
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
   const int tid = threadIdx.x, lane = tid & 63, G = lane >> 4, n = lane & 15;
   Place p = a.template place_of<16>();
   TileRows<16, 4> rows{s_off[wave], 0, 0, false};
-  if (a.eager()) rows.next(a, p.row, a.eager_slot(p) + 16 * (wave / DS), a.c.capacity - 1, lane);
+  if (a.eager()) rows.next(a, p.table, a.eager_slot(p) + 16 * (wave / DS), a.c.capacity - 1, lane);
   a.place_slots(&p);
   if (p.begin >= p.end) return a.template leave_none<HD>(p);  // (the whole workgroup)
   uint32_t t = p.begin + 16 * (wave / DS);
@@ -462,7 +460,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
       for (int c = 0; c < VP; ++c) vf[r][c] = ld_once(reinterpret_cast<const f4_t*>(src + 256 * c));
     }
   };
-  if (!a.eager()) rows.next(a, p.row, t, p.end - 1, lane);
+  if (!a.eager()) rows.next(a, p.table, t, p.end - 1, lane);
   const bool head = uint32_t(n) < p.nh;
   constexpr int QW = HD / 16 / kWaves;
   f4_t x[QW];  // the wave's share of the queries
@@ -476,13 +474,12 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
     rows.put(a, p, 0, lane);
     load_k(0);
     load_v(0);
-    rows.next(a, p.row, t + UNIT, p.end - 1, lane);
+    rows.next(a, p.table, t + UNIT, p.end - 1, lane);
   }
 #pragma unroll
   for (int i = 0; i < QW; ++i) s_q[i * kWaves + wave][lane] = head ? x[i] : f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   __syncthreads();  // (the queries)
   const float mult = a.scale * kLog2e;
-  const uint32_t end = a.end_of(p, n);
   float m = -INFINITY, l = 0.0f;
   f4_t o[VD];
 #pragma unroll
@@ -509,7 +506,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
     if (more) {
       rows.put(a, p, buf, lane);
       load_k(buf);
-      rows.next(a, p.row, t + 2 * UNIT, p.end - 1, lane);
+      rows.next(a, p.table, t + 2 * UNIT, p.end - 1, lane);
     }
     if constexpr (DS > 1) {
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -521,7 +518,7 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
     float s4[4], top[4], mx = m;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      top[i] = t + 4 * G + i < end ? sc[i] * mult : -INFINITY;
+      top[i] = t + 4 * G + i < p.end ? sc[i] * mult : -INFINITY;
       mx = fmaxf(mx, top[i]);
     }
     if constexpr (Args::kScores) {

@@ -15,7 +15,7 @@ struct PrefixArgs {
   float *out, *part_ml, *part_acc;  // parts: [row][head][prefix splits, rest splits]
   uint64_t q_stride, out_stride;
   uint32_t rows, H, groups, max_prefix, max_rest;
-  uint32_t prefix_splits, prefix_chunk, prefix_blocks, rest_splits, rest_chunk, hz;
+  uint32_t prefix_splits, prefix_chunk, prefix_blocks, rest_splits, rest_chunk, step, hz;
   float scale;
 
   static constexpr bool kScores = false;
@@ -48,18 +48,28 @@ struct PrefixArgs {
     } while (n > 1);
     return int(at);
   }
-  // where the row's own slots begin (0 in no group) and end; false for a length or a group that is not valid
-  __device__ bool row_range(uint32_t row, uint32_t* prefix, uint32_t* len) const {
+  // What is joined of a row: `shared` splits of its group's prefix, then slots lo .. len - 1 in splits of `chunk`, in the
+  // pages of row `table`: its own slots in its own, or, for a row shorter than its prefix, what it sees of that (the
+  // prefix's sums hold slots that are not the row's, and an infinity there could not be taken out again).  false for a
+  // length or a group that is not valid.
+  struct Row {
+    uint32_t shared, lo, len, chunk, table;
+  };
+  __device__ bool row_parts(uint32_t row, Row* r) const {
     const int g = last_group(row, [](uint32_t r, uint32_t) { return r; });
-    uint32_t r0, r1;
+    uint32_t r0 = row, r1 = 0, prefix = 0;
     bool ok = true;
-    *prefix = 0;
     if (g >= 0) {
-      ok = group(g, &r0, &r1, prefix);
-      if (ok && row >= r1) *prefix = 0;
+      ok = group(g, &r0, &r1, &prefix);
+      if (ok && row >= r1) prefix = 0;
     }
-    *len = uint32_t(gld(lens + row));
-    return ok && *len <= 0x7fffffffu && (*len <= *prefix || *len - *prefix <= max_rest);
+    const uint32_t len = uint32_t(gld(lens + row));
+    *r = Row{(prefix + prefix_chunk - 1) / prefix_chunk, prefix, len, rest_chunk, row};
+    if (len < prefix) {
+      const uint32_t steps = (len + step - 1) / step;
+      *r = Row{0, 0, len, max(1u, (steps + rest_splits - 1) / rest_splits) * step, r0};
+    }
+    return ok && len <= 0x7fffffffu && (len <= prefix || len - prefix <= max_rest);
   }
 };
 
@@ -77,11 +87,6 @@ struct PartArgs : PrefixArgs {
     uint32_t row, head;
     at(p, i, &row, &head);
     return q + row * q_stride + size_t(head) * HD;
-  }
-  __device__ uint32_t end_of(const Place& p, uint32_t i) const {
-    uint32_t row, head;
-    at(p, i, &row, &head);
-    return min(p.end, uint32_t(gld(lens + row)));
   }
   __device__ size_t part_of(const Place& p, uint32_t i) const {
     uint32_t row, head;
@@ -105,7 +110,7 @@ struct PartArgs : PrefixArgs {
       uint32_t r0 = 0, r1 = 0, prefix = 0;
       const bool there = g >= 0 && group(g, &r0, &r1, &prefix);
       const uint32_t n = there ? (r1 - r0) * gq : 0u, h0 = there ? (b - first(r0, g)) * HT : 0u;
-      p.row = h0 < n ? r0 : 0u;
+      p.row = p.table = h0 < n ? r0 : 0u;
       p.h0 = h0 < n ? h0 : 0u;
       p.nh = h0 < n ? min(uint32_t(HT), n - h0) : 1u;
       p.len = h0 < n ? prefix : 0u;
@@ -128,10 +133,12 @@ struct PartArgs : PrefixArgs {
       p->end = min(p->len, p->begin + prefix_chunk);
       return;
     }
-    uint32_t len;
-    const bool ok = row_range(p->row, &p->lo, &len);
-    p->begin = p->lo + p->split * rest_chunk;
-    p->end = ok ? min(len, p->begin + rest_chunk) : 0u;
+    Row r;
+    const bool ok = row_parts(p->row, &r);
+    p->table = r.table;
+    p->lo = r.lo;
+    p->begin = r.lo + p->split * r.chunk;
+    p->end = ok ? min(r.len, p->begin + r.chunk) : 0u;
     p->split += prefix_splits;
   }
 };
@@ -144,10 +151,9 @@ __global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
   const uint32_t h = blockIdx.x % a.H, row = blockIdx.x / a.H;
   __shared__ __align__(16) float s_o[GR][HD];
   __shared__ float s_f[2 * kMaxSplits];
-  uint32_t prefix, len;
-  const bool ok = a.row_range(row, &prefix, &len);
-  const uint32_t np = ok ? (prefix + a.prefix_chunk - 1) / a.prefix_chunk : 0u;
-  const uint32_t nr = ok && len > prefix ? (len - prefix + a.rest_chunk - 1) / a.rest_chunk : 0u, ns = np + nr;
+  PrefixArgs::Row r;
+  const bool ok = a.row_parts(row, &r);
+  const uint32_t np = ok ? r.shared : 0u, ns = np + (ok && r.len > r.lo ? (r.len - r.lo + r.chunk - 1) / r.chunk : 0u);
   const size_t base = size_t(blockIdx.x) * (a.prefix_splits + a.rest_splits);
   auto place = [&](uint32_t s) { return base + (s < np ? s : a.prefix_splits + (s - np)); };
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
 // ---- host -----------------------------------------------------------------------------------------------------
 struct PrefixPlan {
   bool ok = false;
-  uint32_t prefix_splits = 1, prefix_chunk = 1, rest_splits = 1, rest_chunk = 1, ht = 0, hz = 0;
+  uint32_t prefix_splits = 1, prefix_chunk = 1, rest_splits = 1, rest_chunk = 1, ht = 0, hz = 0, step = 0;
   uint64_t prefix_blocks = 0, rest_blocks = 0, joins = 0;
   size_t off_acc = 0, bytes = 0;
 };
@@ -208,6 +214,7 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
     *chunk = uint32_t(per * step);
     *splits = uint32_t((steps + per - 1) / per);
   };
+  p.step = step;
   const uint64_t in_all = uint64_t(c->rows) * heads;
   if (in_all > kMaxBlocks) return p;
   // queries of a workgroup: 16 where the registers allow them and the groups have as many
@@ -216,7 +223,7 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   p.hz = (gq + p.ht - 1) / p.ht;
   const uint64_t rest = uint64_t(c->rows) * c->kv_heads * p.hz;
   const uint64_t shared = (uint64_t(c->rows) * gq / p.ht + groups) * c->kv_heads;
-  if (shared > kMaxBlocks) return p;
+  if (shared > kMaxBlocks || rest > kMaxBlocks) return p;
   split(rest, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
   split(shared, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
   p.rest_blocks = rest * p.rest_splits;
@@ -232,19 +239,17 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
 template <int HD>
 bool launch_prefix(const PrefixArgs& x, const PrefixPlan& p, int type, hipStream_t st) {
   const uint32_t thr = kWaves * 64;
-  const uint64_t blocks = p.prefix_blocks + (x.max_rest != 0 ? p.rest_blocks : 0);
+  const uint64_t blocks = p.prefix_blocks + p.rest_blocks;
   const PartArgs a{x};
-  bool ok = true;
-  if (blocks != 0) {
-    if (type == 0) {
-      ok = launch(&k_paged_32<HD, PartArgs>, blocks, thr, st, a);
-    } else if (p.ht == 8) {
-      ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, PartArgs>, blocks, thr, st, a)
-                     : launch(&k_paged_16<HD, Bf16, 8, 1, PartArgs>, blocks, thr, st, a);
-    } else if constexpr (HD <= kWaveDims) {
-      ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2, PartArgs>, blocks, thr, st, a)
-                     : launch(&k_paged_16<HD, Bf16, 8, 2, PartArgs>, blocks, thr, st, a);
-    }
+  bool ok = false;
+  if (type == 0) {
+    ok = launch(&k_paged_32<HD, PartArgs>, blocks, thr, st, a);
+  } else if (p.ht == 8) {
+    ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, PartArgs>, blocks, thr, st, a)
+                   : launch(&k_paged_16<HD, Bf16, 8, 1, PartArgs>, blocks, thr, st, a);
+  } else if constexpr (HD <= kWaveDims) {
+    ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 2, PartArgs>, blocks, thr, st, a)
+                   : launch(&k_paged_16<HD, Bf16, 8, 2, PartArgs>, blocks, thr, st, a);
   }
   return ok && launch(&k_prefix_join<HD>, p.joins, 256, st, x);
 }
@@ -304,6 +309,7 @@ extern "C" int chpe_paged_prefix_attention(const chpe_kv_pages* cache, uint32_t 
   a.prefix_blocks = uint32_t(p.prefix_blocks);
   a.rest_splits = p.rest_splits;
   a.rest_chunk = p.rest_chunk;
+  a.step = p.step;
   a.hz = p.hz;
   a.scale = scale;
   const bool ok = cache->head_dim == 64    ? launch_prefix<64>(a, p, cache->type, st)

@@ -283,9 +283,9 @@ size_t chpe_paged_attention_workspace(const chpe_kv_pages *cache, uint32_t heads
  * prefix_lens [groups] on the device) has slots 0 .. prefix_lens[g] - 1 in the pages of the group's first row, whatever
  * its own table holds there, and the slots behind them, up to lens[r] - 1, in its own pages.  A row in no group has no
  * prefix.  max_prefix and max_rest bound the prefixes and what rows have behind them (and size the launches).  A row of
- * length 0 gives zeros, one shorter than its prefix sees lens[r] slots of it; a row of a negative length or with more
- * than max_rest slots of its own gives NaN, and so do the rows of a group whose rows or prefix are out of bounds or whose
- * prefix has a page id outside the pool.  Everything else as chpe_paged_attention.
+ * length 0 gives zeros, one shorter than its prefix sees lens[r] slots of it (and is read on its own); a row of a negative
+ * length or with more than max_rest slots of its own gives NaN, and so do the rows of a group whose rows or prefix are
+ * out of bounds.  Everything else as chpe_paged_attention.
  * workspace: chpe_paged_prefix_workspace bytes for the same cache, heads, groups and bounds, at a 16-byte boundary, any
  * content; calls that may overlap need one each.
  * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
