@@ -6,6 +6,8 @@
 // which is the recurrence of chpe_delta_step unrolled: u_j are the updates b (v - S'^T k) of its tokens.
 // k_delta_prep forms T and the matrix of o for every chunk at once, k_delta_scan carries the state over a row's chunks
 // and writes the outputs, k_delta_gnorm applies the gated norm, which needs a head's whole row.
+#include <type_traits>
+
 #include "delta.hpp"
 
 namespace chpe {
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
 // A workgroup takes 16 NT columns of a value head's state over all chunks of a row.  A chunk is three steps with a
 // barrier behind each, what one leaves to the others in LDS as operands.  Four waves carry the state, each with 16 tokens
 // of a chunk and D / 4 rows of S: 1. v - e^g (K S) of their tokens, 2. u of their tokens, 3. their rows of S.  Four others
-// form the outputs of 16 tokens each: Q S in 1., o in 3.  Everybody loads its own operands of the next chunk where the
+// form the outputs of 16 tokens each: Q S in 2., o in 3.  Everybody loads its own operands of the next chunk where the
 // others leave it time.  (Rows behind the end are the last token again: b, and so u, is 0 there.)
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
 // (Two workgroups on a CU where their LDS allows it: 24 prompts of up to 4097 bf16 tokens of the 9B layout 1.45 ms, with
@@ -476,6 +478,12 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
     if (pa.o32) pa.o32[size_t(t) * a.NV * D + at] = v;
     else static_cast<T*>(a.out)[t * a.out_stride + at] = Elem<T>::put(v);
   };
+  auto put4 = [&](uint32_t t, int ct, f4_t v) {  // columns 4 G ..
+    const size_t at = size_t(h) * D + c0 + 16 * ct + 4 * G;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    if (pa.o32) *reinterpret_cast<f4_t*>(pa.o32 + size_t(t) * a.NV * D + at) = v;
+    else st_row(static_cast<T*>(a.out) + t * a.out_stride + at, x);
+  };
   // the recurrence itself, token by token (inputs that are not finite: see in_range), by the waves that carry S: three barriers a token
   auto tokens = [&](uint32_t t0, uint32_t t1) {
     const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
@@ -547,29 +555,34 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
     }
   };
 
-  // X S of the wave's tokens
-  auto times_s = [&](const u32x4_t (&x)[KS][NP], f4_t (&y)[NT]) {
+  // X S of the wave's tokens: lane (G, n) gets tokens 4 G + r of column n, or (the operands the other way round) columns
+  // 4 G + r of token n, so that outputs are stored 4 at a time
+  auto times_s = [&](const u32x4_t (&x)[KS][NP], f4_t (&y)[NT], auto turned) {
+    constexpr int N = KS * NT, AHEAD = 2;  // (operands are read two products ahead: LDS answers in some 100 cycles)
+    u32x4_t f[AHEAD + 1][3];
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) {
-      f4_t sum[2] = {f4_t{0.0f, 0.0f, 0.0f, 0.0f}, f4_t{0.0f, 0.0f, 0.0f, 0.0f}};  // (two chains of products)
+    for (int i = 0; i < AHEAD; ++i) ld_parts(s_s[i % KS][i / KS], lane, f[i]);
+    f4_t sum[2];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        u32x4_t f[3];
-        ld_parts(s_s[s][ct], lane, f);
-        sum[s & 1] = mma(x[s], f, sum[s & 1]);
-      }
-      y[ct] = sum[0] + sum[1];
+    for (int i = 0; i < N; ++i) {
+      if (i + AHEAD < N) ld_parts(s_s[(i + AHEAD) % KS][(i + AHEAD) / KS], lane, f[(i + AHEAD) % (AHEAD + 1)]);
+      __builtin_amdgcn_sched_barrier(0);
+      const int s = i % KS;
+      if (s == 0) sum[0] = sum[1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};  // (two chains of products)
+      const auto& g = f[i % (AHEAD + 1)];
+      sum[s & 1] = turned ? mma(g, x[s], sum[s & 1]) : mma(x[s], g, sum[s & 1]);
+      if (s == KS - 1) y[i / KS] = sum[0] + sum[1];
     }
   };
-  // M x of the wave's row of a matrix
-  auto times_x = [&](const u32x4_t (&m)[2][3], const u32x4_t (&x)[2][3][64], f4_t y) {
+  // M x of the wave's row of a matrix, the same ways
+  auto times_x = [&](const u32x4_t (&m)[2][3], const u32x4_t (&x)[2][3][64], f4_t y, auto turned) {
     f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
     u32x4_t f[3];
     ld_parts(x[0], lane, f);
-    y = mma(m[0], f, y);
+    y = turned ? mma(f, m[0], y) : mma(m[0], f, y);
     if (ns > 1) {
       ld_parts(x[1], lane, f);
-      sum = mma(m[1], f, sum);
+      sum = turned ? mma(f, m[1], sum) : mma(m[1], f, sum);
     }
     return y + sum;
   };
@@ -593,39 +606,34 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
     f4_t y[NT], done[NT];
     uint32_t from = hi;  // tokens of `done`
     auto store = [&] {
-      const uint32_t t = from + 16 * wave + 4 * G;
+      const uint32_t t = from + 16 * wave + n;
+      if (t >= hi) return;
 #pragma unroll
-      for (int ct = 0; ct < NT; ++ct)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (t + r < hi) put(t + r, ct, done[ct][r]);
+      for (int ct = 0; ct < NT; ++ct) put4(t, ct, done[ct]);
     };
     if (lo < hi) {
       load_scale(lo);
       load_x(x16, a.q, a.q_stride, lo);
       load_m(m16, lo, kOffO);
       leave_scale(0);
-      take_x();
     }
     lds_barrier();
     for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
       const uint32_t next = t0 + kChunk < hi ? t0 + kChunk : t0;  // (behind the last chunk: that one again, not used)
-      times_s(xf, y);
+      take_x();
       load_x(x16, a.q, a.q_stride, next);
       load_scale(next);
-      const f4_t g = *reinterpret_cast<const f4_t*>(&s_scale[turn][64 + 16 * wave + 4 * G]);
-#pragma unroll
-      for (int ct = 0; ct < NT; ++ct) y[ct] *= g;
-      lds_barrier();
       store();
-      take_x();
+      lds_barrier();
+      const float g = s_scale[turn][64 + 16 * wave + n];
       if (s_bad[turn] != 0) {  // (the same for all)
         for (uint32_t i = 3 * min(hi - t0, uint32_t(kChunk)); i != 0; --i) lds_barrier();
         from = hi;
       } else {
+        times_s(xf, y, std::true_type{});
         lds_barrier();
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) done[ct] = times_x(m16, s_u[ct], y[ct]);
+        for (int ct = 0; ct < NT; ++ct) done[ct] = times_x(m16, s_u[ct], y[ct] * g, std::true_type{});
         from = t0;
       }
       load_m(m16, next, kOffO);
@@ -663,7 +671,7 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
         bad |= !(fabsf(v[ct][r]) < 1e38f);
       }
     if (__ballot(bad) != 0 && lane == 0) s_bad[turn] = 1;
-    times_s(xf, y);
+    times_s(xf, y, std::false_type{});
     const float* scale = s_scale[turn] + 16 * wave + 4 * G;
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) leave_u(s_x[ct], v[ct] - *reinterpret_cast<const f4_t*>(scale) * y[ct]);
@@ -681,7 +689,7 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
     // 2.
     f4_t u[NT];
 #pragma unroll
-    for (int ct = 0; ct < NT; ++ct) u[ct] = times_x(m16, s_x[ct], f4_t{0.0f, 0.0f, 0.0f, 0.0f});
+    for (int ct = 0; ct < NT; ++ct) u[ct] = times_x(m16, s_x[ct], f4_t{0.0f, 0.0f, 0.0f, 0.0f}, std::false_type{});
     load_x(x16, a.k, a.k_stride, next);
     load_v(next);
 #pragma unroll
@@ -693,24 +701,24 @@ __global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 
     lds_barrier();
     // 3.
 #pragma unroll
-    for (int u = 0; u < RT; ++u) {
-      const int at = 4 * (RT == 2 ? wave : wave >> 1), half = RT == 2 ? u : wave & 1;
+    for (int s = 0; s < 2; ++s) {
+      u32x4_t kt[RT][NP];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4_t kt[NP];
+      for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           // lane n of a group of 16 names 4 keys of token n / 4 and gets key n of the four tokens
-          const u32x2_t lo4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 4 * G + n / 4][at + n % 4]) + half);
-          const u32x2_t hi4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 16 + 4 * G + n / 4][at + n % 4]) + half);
-          kt[p] = u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y};
+          const int at = 4 * (RT == 2 ? wave : wave >> 1) + n % 4, half = RT == 2 ? u : wave & 1;
+          const u32x2_t lo4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 4 * G + n / 4][at]) + half);
+          const u32x2_t hi4 = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_k[p][32 * s + 16 + 4 * G + n / 4][at]) + half);
+          kt[u][p] = u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y};
         }
 #pragma unroll
-        for (int ct = 0; ct < NT; ++ct) {
-          u32x4_t f[3];
-          ld_parts(s_us[ct][s], lane, f);
-          S[u][ct] = mma(kt, f, s == 0 ? S[u][ct] * end : S[u][ct]);
-        }
+      for (int ct = 0; ct < NT; ++ct) {
+        u32x4_t f[3];
+        ld_parts(s_us[ct][s], lane, f);
+#pragma unroll
+        for (int u = 0; u < RT; ++u) S[u][ct] = mma(kt[u], f, s == 0 ? S[u][ct] * end : S[u][ct]);
       }
     }
     load_m(m16, next, 0);
