@@ -184,16 +184,17 @@ __device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e30f; }
 // T_ij = -(sum_(j < k <= i) T_ik A_kj) T_jj, in a wave's registers.  |k| <= 1 and b < 1 keep T's elements within products
 // of contractions; a series in powers of A would not stay there.
 template <int D, class T>
-__global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
+__global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
   constexpr int NP = kParts<T>, KS = D / 32, AS = 68;
-  constexpr int kBytesK = 4 * KS * NP * 1024, kBytesA = 64 * AS * 4;
-  __shared__ __align__(16) uint8_t s_mem[kBytesK > kBytesA ? kBytesK : kBytesA];
-  __shared__ __align__(16) float s_diag[4][16][20];
+  constexpr int kBytesK = 4 * KS * NP * 1024, kBytesA = 64 * AS * 4, kBytesD = 4 * 16 * 20 * 4;
+  // (49 KB for f32 keys of 128: three workgroups on a CU)
+  __shared__ __align__(16) uint8_t s_mem[kBytesK > kBytesA + kBytesD ? kBytesK : kBytesA + kBytesD];
   __shared__ double s_g[64];
   __shared__ __align__(16) float s_beta[64], s_rk[64], s_rq[64];
   auto s_k = reinterpret_cast<u32x4_t(*)[KS][NP][64]>(s_mem);
   auto s_A = reinterpret_cast<float(*)[AS]>(s_mem);
+  auto s_diag = reinterpret_cast<float(*)[16][20]>(s_mem + kBytesA);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
   const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
   const int row = a.r.row_of(b, kChunkShift, lane);
@@ -387,10 +388,8 @@ __global__ void __launch_bounds__(256) k_delta_prep(PromptArgs pa) {
 // form the outputs of 16 tokens each: Q S in 2., o in 3.  Everybody loads its own operands of the next chunk where the
 // others leave it time.  (Rows behind the end are the last token again: b, and so u, is 0 there.)
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
-// (Two workgroups on a CU where their LDS allows it: 24 prompts of up to 4097 bf16 tokens of the 9B layout 1.45 ms, with
-// one 1.88.)
 template <int D, class T, int NT>
-__global__ void __launch_bounds__(512, (sizeof(T) == 2 || D == 64) && NT == 1 ? 4 : 2) k_delta_scan(PromptArgs pa) {
+__global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
   constexpr int NP = kParts<T>, KS = D / 32, RT = D / 64, CB = D / (16 * NT);
   constexpr int KR = D / 8 + 2;  // a token's keys in LDS, with room so that neither side's accesses meet in a few banks
