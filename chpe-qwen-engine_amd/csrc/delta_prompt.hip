@@ -160,19 +160,6 @@ struct Raw<float> {
   static __device__ float value(float b) { return b; }
 };
 
-// a read of LDS that transposes 4 x 16 values of 16 bits among 16 lanes
-__device__ __forceinline__ u32x2_t ld_transposed(const u32x2_t* p) {
-  typedef short s4_t __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(p)));
-}
-
-// a barrier for what lies in LDS: loads from memory stay on their way (__syncthreads would wait for them)
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // Keys and queries whose squares leave this range, and gates that are NaN, make a chunk run token by token: the
 // products above take keys before their norm, and 0 times what is not finite would reach earlier tokens.
 __device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e30f; }

@@ -110,6 +110,19 @@ template <class T>
 __device__ __forceinline__ void st_once(T* p, T v) {
   __builtin_nontemporal_store(v, (__attribute__((address_space(1))) T*)p);
 }
+// a read of LDS that transposes 4 x 16 values of 16 bits among 16 lanes
+__device__ __forceinline__ dev::u32x2_t ld_transposed(const dev::u32x2_t* p) {
+  typedef short s4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(dev::u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4_t*)(p)));
+}
+
+// a barrier for what lies in LDS: loads from memory stay on their way (__syncthreads would wait for them)
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // a value that is the same in all lanes, as a scalar
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) { return uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)); }

@@ -143,6 +143,241 @@ struct PartArgs : PrefixArgs {
   }
 };
 
+// ---- many queries ---------------------------------------------------------------------------------------------------
+// Where a group has more queries than a few: a wave keeps 16 QT of them as columns (QT = 2, at head dim 256 1), with
+// their parts as operands in registers, and the four waves of a workgroup share every 32 slots' K and V in LDS, the next
+// 32 on the way.  S^T = K . Q^T and O^T = V^T . P^T as in k_paged_16: a lane's column is a query in both, the scores' layout is
+// the weights'; V's rows become operands with slots inside by the transposing reads of LDS.
+// k_paged_16 reads each K and V row once per 16 queries, and every lane pair forms a score's weight twice: 64 rows of 8
+// query heads behind 8192 fp16 slots took 116 us there (1.1 GB through the CUs' caches at 27 bytes a cycle each, 65 us, and
+// 50 us of vector instructions).
+// Bound by the vector instructions of the softmax.
+template <class T>
+struct ManyParts;
+template <>
+struct ManyParts<_Float16> {
+  static constexpr int N = 2, kScaleExp = 15;  // (22 bits, x brought near 2^14: Parts<_Float16, 8>)
+  static __device__ void split(const float (&x)[8], u32x4_t (&out)[N]) {
+    h8_t hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      hi[e] = _Float16(x[e]);
+      lo[e] = _Float16(x[e] - float(hi[e]));
+    }
+    out[0] = __builtin_bit_cast(u32x4_t, hi);
+    out[1] = __builtin_bit_cast(u32x4_t, lo);
+  }
+  static __device__ f4_t mfma(u32x4_t a, u32x4_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct ManyParts<Bf16> {
+  static constexpr int N = 3, kScaleExp = 0;  // (all 24 bits)
+  static __device__ void split(const float (&x)[8], u32x4_t (&out)[N]) {
+    b8_t a, b, c;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a[e] = __bf16(x[e]);
+      const float r = x[e] - float(a[e]);
+      b[e] = __bf16(r);
+      c[e] = __bf16(r - float(b[e]));
+    }
+    out[0] = __builtin_bit_cast(u32x4_t, a);
+    out[1] = __builtin_bit_cast(u32x4_t, b);
+    out[2] = __builtin_bit_cast(u32x4_t, c);
+  }
+  static __device__ f4_t mfma(u32x4_t a, u32x4_t b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  }
+};
+constexpr int many_tiles(int hd) { return hd == 256 ? 1 : 2; }
+constexpr int many_queries(int hd) { return 64 * many_tiles(hd); }
+
+template <int HD, class T>
+__global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
+  using P = ManyParts<T>;
+  constexpr int NP = P::N, QT = many_tiles(HD), KS = HD / 32, VD = HD / 16;
+  constexpr int CPR = HD / 8, RPP = 256 / CPR, PASS = 32 / RPP;  // 16-byte pieces of a row; rows a pass of the workgroup loads
+  constexpr int KROW = CPR + 1, VROW = CPR + 2;                  // (room so that neither side's reads meet in a few banks)
+  __shared__ u32x4_t s_k[2][32][KROW], s_v[2][32][VROW];
+  __shared__ int s_bad;
+  const int wave = uniform(threadIdx.x >> 6), tid = threadIdx.x, lane = tid & 63, G = lane >> 4, n = lane & 15;
+  Place p = a.template place_of<many_queries(HD)>();
+  a.place_slots(&p);
+  if (p.begin >= p.end) return;  // (the whole workgroup)
+  if (tid == 0) s_bad = 0;
+  // the thread's pieces of a tile's rows
+  const int piece = tid % CPR, row0 = tid / CPR;
+  uint32_t id[PASS];
+  bool bad = false;
+  u32x4_t kr[PASS], vr[PASS];
+  auto ids = [&](uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const uint32_t slot = min(t + uint32_t(row0 + RPP * i), p.end - 1);
+      id[i] = uint32_t(gld(a.c.table + size_t(p.table) * a.c.table_stride + (slot >> a.c.shift)));
+    }
+  };
+  auto load = [&](uint32_t t) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const uint32_t slot = min(t + uint32_t(row0 + RPP * i), p.end - 1);
+      const bool in = id[i] < a.c.n_pages;
+      bad |= !in;
+      const size_t at = a.c.at(in ? id[i] : 0u, p.kvh, slot) * 2 + piece * 16;
+      kr[i] = gld(reinterpret_cast<const u32x4_t*>(a.c.k + at));
+      vr[i] = gld(reinterpret_cast<const u32x4_t*>(a.c.v + at));
+    }
+  };
+  auto leave = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      s_k[buf][row0 + RPP * i][piece] = kr[i];
+      s_v[buf][row0 + RPP * i][piece] = vr[i];
+    }
+  };
+  uint32_t t = p.begin;
+  ids(t);
+  load(t);
+  if (t + 32 < p.end) ids(t + 32);
+  // the queries: lane (G, n) has dims 32 s + 8 G .. of query n
+  const uint32_t q0 = wave * 16 * QT;
+  const bool idle = q0 >= p.nh;  // (a wave without queries loads and waits with the others)
+  u32x4_t qf[QT][KS][NP];
+  float mult[QT], m[QT], l[QT];
+  f4_t o[QT][VD];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const uint32_t i = q0 + 16 * qt + n;
+    const float* src = a.template query<HD>(p, i) + 8 * G;  // (behind the last query: that one again, not used)
+    float x[KS][8], top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const float4 u = ld_f4(src + 32 * s), v = ld_f4(src + 32 * s + 4);
+      const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[s][e] = w[e];
+        top = fmaxf(top, fabsf(w[e]));
+      }
+    }
+    int ex = 0;
+    if constexpr (P::kScaleExp != 0) {
+      top = pair_max(pair_max(top, 16), 32);
+      if (top > 0.0f && top < INFINITY) ex = 14 - __builtin_amdgcn_frexp_expf(top);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(x[s][e], ex);
+      P::split(x[s], qf[qt][s]);
+    }
+    mult[qt] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -ex);
+    m[qt] = -INFINITY;
+    l[qt] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VD; ++j) o[qt][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  leave(0);
+  if (t + 32 < p.end) {
+    load(t + 32);
+    if (t + 64 < p.end) ids(t + 64);
+  }
+  lds_barrier();
+  for (int buf = 0; t < p.end; t += 32, buf ^= 1) {
+    if (t + 32 < p.end) {
+      leave(buf ^ 1);
+      if (t + 64 < p.end) {
+        load(t + 64);
+        if (t + 96 < p.end) ids(t + 96);
+      }
+    }
+    if (!idle) {
+      f4_t sc[QT][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4_t kf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[s] = s_k[buf][16 * u + n][4 * s + G];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) sc[qt][u] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) sc[qt][u] = P::mfma(kf[s], qf[qt][s][i], sc[qt][u]);
+      }
+      u32x4_t pf[QT][NP];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float x[8], top[8], mx = m[qt];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = sc[qt][e >> 2][e & 3];
+          top[e] = t + (e >> 2) * 16 + 4 * G + (e & 3) < p.end ? x[e] * mult[qt] : -INFINITY;
+          mx = fmaxf(mx, top[e]);
+        }
+        mx = pair_max(pair_max(mx, 16), 32);
+        const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m[qt] - base);
+        if (__ballot(f != 1.0f) != 0) {
+          l[qt] *= f;
+#pragma unroll
+          for (int j = 0; j < VD; ++j) o[qt][j] *= f;
+        }
+        m[qt] = mx;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // (the product again inside the fma: rounded once, as small as the difference is)
+          x[e] = __builtin_amdgcn_exp2f(top[e] > -INFINITY ? fmaf(x[e], mult[qt], -base) : top[e]);
+          l[qt] += x[e];
+          x[e] *= float(1 << P::kScaleExp);
+        }
+        P::split(x, pf[qt]);
+      }
+#pragma unroll
+      for (int j = 0; j < VD; ++j) {
+        // lane n of a group of 16 names 4 dims of slot n / 4 and gets dim n of the four slots
+        const u32x2_t lo = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_v[buf][4 * G + n / 4][2 * j]) + n % 4);
+        const u32x2_t hi = ld_transposed(reinterpret_cast<const u32x2_t*>(&s_v[buf][16 + 4 * G + n / 4][2 * j]) + n % 4);
+        const u32x4_t vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) o[qt][j] = P::mfma(vf, pf[qt][i], o[qt][j]);
+      }
+    }
+    lds_barrier();
+  }
+  if (__ballot(bad) != 0 && lane == 0) s_bad = 1;
+  lds_barrier();
+  if (idle) return;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const uint32_t i = q0 + 16 * qt + n;
+    float L = pair_sum(pair_sum(l[qt], 16), 32);
+    if (s_bad != 0) L = __builtin_nanf("");
+    if (i >= p.nh) continue;
+    const size_t pt = a.part_of(p, i);
+    if (G == 0) reinterpret_cast<float2*>(a.part_ml)[pt] = make_float2(m[qt], L);
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < VD; ++j) {
+      const f4_t v = o[qt][j] * (1.0f / float(1 << P::kScaleExp));
+      finite &= all_finite(v);
+      *reinterpret_cast<f4_t*>(a.part_acc + pt * HD + 16 * j + 4 * G) = v;
+    }
+    if (finite || L != L) continue;
+#pragma unroll 1
+    for (int j = 0; j < VD; ++j) {
+      f4_t* d = reinterpret_cast<f4_t*>(a.part_acc + pt * HD + 16 * j + 4 * G);
+      const f4_t v = *d;
+      if (!all_finite(v)) *d = non_finite_sum<T>(a, p, 16 * j + 4 * G, v);
+    }
+  }
+}
+
 // ---- the join: a workgroup per (row, query head), 256 / (HD / 4) parts at a time ----------------------------------
 template <int HD>
 __global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
@@ -206,9 +441,9 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   PrefixPlan p;
   const uint32_t gq = heads / c->kv_heads, step = (c->type == 0 ? 16 : 32) * tiles_at_once(c->head_dim);
   const uint64_t large = (512 << 10) / (2 * c->head_dim * (c->type == 0 ? 4 : 2));  // slots
-  auto split = [&](uint64_t items, uint64_t want, uint32_t range, uint32_t* splits, uint32_t* chunk) {
+  auto split = [&](uint64_t items, uint64_t blocks, uint64_t want, uint32_t range, uint32_t* splits, uint32_t* chunk) {
     const uint64_t steps = std::max<uint64_t>(1, (uint64_t(range) + step - 1) / step), some = std::max<uint64_t>(1, items);
-    uint64_t n = std::min<uint64_t>({std::max<uint64_t>((1024 + some - 1) / some, want), steps, kMaxSplits});
+    uint64_t n = std::min<uint64_t>({std::max<uint64_t>((blocks + some - 1) / some, want), steps, kMaxSplits});
     n = std::max<uint64_t>(1, std::min<uint64_t>(n, kMaxBlocks / some));
     const uint64_t per = (steps + n - 1) / n;
     *chunk = uint32_t(per * step);
@@ -220,12 +455,19 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   // queries of a workgroup: 16 where the registers allow them and the groups have as many
   const bool many = gq > 8 || (max_prefix != 0 && groups != 0 && uint64_t(c->rows) * gq > 8 * uint64_t(groups));
   p.ht = c->type == 0 || (many && c->head_dim <= kWaveDims) ? 16 : 8;
+  // ... and k_prefix_many where they have more than a few, the calls are not all latency, and the rows' own slots, for which it
+  // has most of its columns idle, do not count: behind 4096 slots with 64 of their own 64 rows of the 72B layout take 53 us
+  // there and 74 in k_paged_16, 4 rows 17 and 20; 8 rows of the 9B layout (32 queries) 20 and 18; 64 rows behind 1000 slots
+  // with up to 1000 of their own 82 and 69; 8 groups of 6 rows of 6 queries 31 and 21.
+  if (c->type != 0 && groups != 0 && uint64_t(c->rows) * gq >= 24 * uint64_t(groups) &&
+      uint64_t(c->rows) * heads >= 256 && max_prefix / 2 >= max_rest)
+    p.ht = many_queries(c->head_dim);
   p.hz = (gq + p.ht - 1) / p.ht;
   const uint64_t rest = uint64_t(c->rows) * c->kv_heads * p.hz;
   const uint64_t shared = (uint64_t(c->rows) * gq / p.ht + groups) * c->kv_heads;
   if (shared > kMaxBlocks || rest > kMaxBlocks) return p;
-  split(rest, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
-  split(shared, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
+  split(rest, 1024, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
+  split(shared, p.ht > 16 ? 512 : 1024, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
   p.rest_blocks = rest * p.rest_splits;
   p.prefix_blocks = max_prefix == 0 || groups == 0 ? 0 : shared * p.prefix_splits;
   p.joins = in_all;
@@ -244,6 +486,8 @@ bool launch_prefix(const PrefixArgs& x, const PrefixPlan& p, int type, hipStream
   bool ok = false;
   if (type == 0) {
     ok = launch(&k_paged_32<HD, PartArgs>, blocks, thr, st, a);
+  } else if (p.ht > 16) {
+    ok = type == 1 ? launch(&k_prefix_many<HD, _Float16>, blocks, thr, st, a) : launch(&k_prefix_many<HD, Bf16>, blocks, thr, st, a);
   } else if (p.ht == 8) {
     ok = type == 1 ? launch(&k_paged_16<HD, _Float16, 8, 1, PartArgs>, blocks, thr, st, a)
                    : launch(&k_paged_16<HD, Bf16, 8, 1, PartArgs>, blocks, thr, st, a);
