@@ -270,10 +270,11 @@ __global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(x[s][e], ex);
+      for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(a.scale < 0.0f ? -x[s][e] : x[s][e], ex);
       P::split(x[s], qf[qt][s]);
     }
-    mult[qt] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -ex);
+    mult[qt] = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, -ex);
+    if (mult[qt] == 0.0f) mult[qt] = 1e-38f;  // (what scores come to stays 0; -inf behind the end stays -inf)
     m[qt] = -INFINITY;
     l[qt] = 0.0f;
 #pragma unroll
@@ -312,27 +313,30 @@ __global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
       u32x4_t pf[QT][NP];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        float x[8], top[8], mx = m[qt];
+        // weights are 2^(x mult - m + kScaleExp), m the largest x mult so far rounded up: a whole number, so that what older sums
+        // are multiplied by is exact, and 1 most of the time
+        float x[8], mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = sc[qt][e >> 2][e & 3];
-          top[e] = t + (e >> 2) * 16 + 4 * G + (e & 3) < p.end ? x[e] * mult[qt] : -INFINITY;
-          mx = fmaxf(mx, top[e]);
+        for (int e = 0; e < 8; ++e) x[e] = sc[qt][e >> 2][e & 3];
+        if (t + 32 > p.end) {  // (uniform: the last tile)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = t + (e >> 2) * 16 + 4 * G + (e & 3) < p.end ? x[e] : -INFINITY;
         }
-        mx = pair_max(pair_max(mx, 16), 32);
-        const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m[qt] - base);
-        if (__ballot(f != 1.0f) != 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, x[e]);
+        mx = fmaxf(m[qt], ceilf(pair_max(pair_max(mx, 16), 32) * mult[qt]));
+        if (__ballot(mx != m[qt]) != 0) {
+          const float f = m[qt] > -INFINITY ? __builtin_amdgcn_exp2f(m[qt] - mx) : 0.0f;
           l[qt] *= f;
 #pragma unroll
           for (int j = 0; j < VD; ++j) o[qt][j] *= f;
         }
         m[qt] = mx;
+        const float less = mx == -INFINITY ? 0.0f : float(P::kScaleExp) - mx;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          // (the product again inside the fma: rounded once, as small as the difference is)
-          x[e] = __builtin_amdgcn_exp2f(top[e] > -INFINITY ? fmaf(x[e], mult[qt], -base) : top[e]);
+          x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], mult[qt], less));
           l[qt] += x[e];
-          x[e] *= float(1 << P::kScaleExp);
         }
         P::split(x, pf[qt]);
       }
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const uint32_t i = q0 + 16 * qt + n;
-    float L = pair_sum(pair_sum(l[qt], 16), 32);
+    float L = pair_sum(pair_sum(l[qt], 16), 32) * (1.0f / float(1 << P::kScaleExp));
     if (s_bad != 0) L = __builtin_nanf("");
     if (i >= p.nh) continue;
     const size_t pt = a.part_of(p, i);
