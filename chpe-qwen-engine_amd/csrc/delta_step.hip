@@ -28,9 +28,13 @@ __global__ void __launch_bounds__((kGroups<D, ONE> * D / 4)) k_delta_step(DeltaA
   const bool there = a.r.range(row, &lo, &hi);
   const int slot = a.r.before(row, &fill), to = a.r.after(row);
   if (!there || hi - lo > longest) return;
-  const float A_log = gld(a.A_log + h), dt = gld(a.dt_bias + h);
-  float w[4];
-  if (a.z) ld_row(a.norm_w + c, w);
+  const bool any = ONE || lo < hi;
+  float A_log = 0.0f, dt = 0.0f, w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (any) {  // (a call without tokens has none of these)
+    A_log = gld(a.A_log + h);
+    dt = gld(a.dt_bias + h);
+    if (a.z) ld_row(a.norm_w + c, w);
+  }
   struct Token {
     float v[4], x[PL], y[PL], z[4], a, b;
   };
@@ -45,7 +49,7 @@ __global__ void __launch_bounds__((kGroups<D, ONE> * D / 4)) k_delta_step(DeltaA
     return k;
   };
   Token next;  // (requested before the state, whose slot is on its way)
-  if (ONE || lo < hi) next = load(lo);
+  if (any) next = load(lo);
   float s[RPT][4];
   // (the head's place is the same for all lanes: scalar registers hold the rows' addresses)
   const uint32_t at = rg * D + c;

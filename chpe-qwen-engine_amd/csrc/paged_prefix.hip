@@ -474,6 +474,7 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   split(shared, p.ht > 16 ? 512 : 1024, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
   p.rest_blocks = rest * p.rest_splits;
   p.prefix_blocks = max_prefix == 0 || groups == 0 ? 0 : shared * p.prefix_splits;
+  if (p.rest_blocks + p.prefix_blocks > kMaxItems / 256) return p;
   p.joins = in_all;
   const uint64_t places = in_all * (p.prefix_splits + p.rest_splits);
   p.off_acc = (places * 8 + 255) / 256 * 256;

@@ -118,3 +118,6 @@ def test_prefix_workspace():
     assert need > 0 and prefix(pages(), size=need - 1) == -2 and prefix(None) == -1
     assert prefix(pages(rows=0), size=0) == 0
     assert lib.chpe_paged_prefix_workspace(pages(), 64, 2, 49, 32) == 0 and lib.chpe_paged_prefix_workspace(None, 64, 2, 1, 1) == 0
+    # the two kinds of workgroups in one launch: together within what a launch can have
+    many, groups = pages(rows=1 << 20), (1 << 20) - (1 << 17)
+    assert lib.chpe_paged_prefix_workspace(many, 8, groups - 1, 16, 16) > 0 and lib.chpe_paged_prefix_workspace(many, 8, groups, 16, 16) == 0

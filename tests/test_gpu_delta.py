@@ -452,6 +452,18 @@ def test_nothing_to_do():
     assert h.prompt(*L.args(), dev([0]), dev([]), dev([])).shape == (0, NV, hd)
 
 
+def test_rows_without_tokens_need_no_inputs():
+    _, state = pool(3, 4, 64, 1)
+    old = state.clone()
+    s = ca._DeltaStates(state.data_ptr(), state.stride(0), 3, 4, 2, 64)
+    t = ca._DeltaTokens(*(0 if n in ("type", "eps") or n.endswith("_stride") else None for n, _ in ca._DeltaTokens._fields_))
+    starts, slots, to = dev([0, 0, 0, 0]), dev([0, -1, 2]), dev([1, 2, -1])
+    work = torch.empty(ca.load_engine_lib().chpe_delta_prompt_workspace(s, 0, 2, 0), dtype=torch.uint8, device="cuda")
+    assert ca.load_engine_lib().chpe_delta_prompt(s, t, 0, 2, starts.data_ptr(), slots.data_ptr(), to.data_ptr(), work.data_ptr(),
+                                                  work.numel(), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(state[0], old[0]) and torch.equal(state[1], old[0]) and (state[2] == 0).all()
+
+
 def test_what_python_refuses():
     NK, NV, hd, n = 2, 4, 64, 3
     L = Layer(n, NK, NV, hd, "f32", False, seed=1)

@@ -196,6 +196,94 @@ def test_values_that_are_not_finite(hd, dtype):
     g.check(q, out, rows=[1])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_queries_bad_pages_and_infinities(hd, dtype):
+    """As the two tests above, with as many queries a group as share their K and V in LDS."""
+    lens = [201, 200, 90, 240, 300, 0, 217, 299]
+    g = Groups([(200, lens), (70, [71, 80])], 1, hd, 16, dtype, seed=hd, own_tables=True)
+    put = lambda t, r, slot, x: t.select(0, int(g.table[r, slot // 16])).select(1, slot % 16).copy_(x)  # noqa: E731
+    for r, n in enumerate(g.lens):  # what no row sees
+        for slot in range(max(n, 200 if r == 0 else 70 if r == 8 else 0), g.table.shape[1] * 16):
+            put(g.k, r, slot, torch.full((1, hd), float("nan")))
+            put(g.v, r, slot, torch.full((1, hd), float("inf")))
+    q = queries(10, 40, hd)
+    out = g.run(q)
+    g.check(q, out)
+    # a page of the prefix: every row but those that end before it; a row's own
+    table = g.table.clone()
+    table[0, 9], table[8, 4] = -1, 1 << 30
+    table[4, 15] = 10 ** 6
+    g.p = ca.KvPages(g.k, g.v, table.cuda())
+    nan = torch.isnan(g.run(q)).flatten(1).all(1).tolist()
+    assert nan == [n > 144 for n in lens] + [True, True]
+    table[0, 9], table[8, 4] = g.table[0, 9], g.table[8, 4]
+    g.p = ca.KvPages(g.k, g.v, table.cuda())
+    again = g.run(q)
+    assert torch.isnan(again).flatten(1).all(1).tolist() == [r == 4 for r in range(10)]
+    rest = [r for r in range(10) if r != 4]
+    assert torch.equal(again[rest], out[rest])
+    # an infinity in the prefix, past row 2's end
+    g.p = ca.KvPages(g.k, g.v, g.table.cuda())
+    g.v[int(g.table[0, 150 // 16]), :, 150 % 16, 7] = -float("inf")
+    inf = g.run(q)
+    sees = [r for r in range(8) if g.lens[r] > 150]
+    assert (inf[sees, :, 7] == -float("inf")).all()
+    inf[sees, :, 7] = out[sees, :, 7]
+    assert torch.equal(inf, out)
+
+
+def test_offsets_past_32_bits():
+    """Pages whose offsets pass 2^32 bytes and 2^31 elements, for few queries a group and for many."""
+    for rows, H in ((2, 4), (9, 32)):
+        g = Groups([(64, [66 + i for i in range(rows)])], 1, 64, 16, "f16")
+        n, page = g.k.shape[0], 16 * 64
+        step = (1 << 32) // n // 8 * 8  # the last page's begins behind 3 * 2^30 elements
+        far = [torch.empty(step * (n - 1) + page, dtype=torch.float16, device="cuda").as_strided(g.k.shape, (step, page, 64, 1))
+               for _ in "kv"]
+        for to, t in zip(far, (g.k, g.v)):
+            to.copy_(t)
+        q = queries(rows, H, 64)
+        near = g.run(q)
+        g.check(q, near)
+        g.p = ca.KvPages(*far, g.table.cuda())
+        assert torch.equal(g.run(q), near)
+        del far, g
+
+
+def test_many_queries_captured():
+    """Groups that change between replays; a second graph with a workspace of its own at the same time."""
+    g = Groups([(200, [201 + 7 * i for i in range(9)])], 2, 128, 16, "bf16", seed=6)
+    q = queries(9, 64, 128).cuda()
+    lens, runs = dev(np.asarray(g.lens, np.int32)), []
+    for _ in range(2):
+        out = torch.empty_like(q)
+        work = torch.empty(g.p.prefix_workspace(64, 1, g.max_prefix, g.max_rest), dtype=torch.uint8, device="cuda")
+        run = lambda out=out, work=work: g.p.prefix_attention(q, lens, g.group_rows, g.prefix_lens, g.max_prefix, g.max_rest,  # noqa: E731
+                                                              out=out, workspace=work)
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        runs.append((graph, out, run))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for groups, prefix in (([0, 9], 200), ([0, 4], 150), ([3, 9], 199), ([9, 9], 200), ([0, 9], 201)):
+        g.group_rows.copy_(dev(groups))
+        g.prefix_lens.fill_(prefix)
+        runs[0][2]()
+        want = runs[0][1].clone()
+        for _, out, _ in runs:
+            out.fill_(0)
+        torch.cuda.synchronize()
+        for (graph, _, _), s in zip(runs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out, _ in runs:
+            assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), groups
+
+
 def test_as_without_groups():
     """No groups: chpe_paged_attention's results up to the order of the joins."""
     g = Groups([(None, [300, 1, 77, 0])], 4, 128, 16, "bf16")
