@@ -152,6 +152,8 @@ struct PartArgs : PrefixArgs {
 // query heads behind 8192 fp16 slots took 116 us there (1.1 GB through the CUs' caches at 27 bytes a cycle each, 65 us, and
 // 50 us of vector instructions).
 // Bound by the vector instructions of the softmax.
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
 template <class T>
 struct ManyParts;
 template <>
@@ -159,10 +161,15 @@ struct ManyParts<_Float16> {
   static constexpr int N = 2, kScaleExp = 15;  // (22 bits, x brought near 2^14: Parts<_Float16, 8>)
   static __device__ void split(const float (&x)[8], u32x4_t (&out)[N]) {
     h8_t hi, lo;
+    float one = -1.0f;
+    asm("" : "+v"(one));  // (a product with it takes the 16 bits as they are: without it they are widened first)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hi[e] = _Float16(x[e]);
-      lo[e] = _Float16(x[e] - float(hi[e]));
+    for (int e = 0; e < 8; e += 2) {
+      const h2_t h = __builtin_convertvector((f2_t{x[e], x[e + 1]}), h2_t);
+      const f2_t r = {fmaf(float(h.x), one, x[e]), fmaf(float(h.y), one, x[e + 1])};
+      const h2_t l = __builtin_convertvector(r, h2_t);
+      hi[e] = h.x, hi[e + 1] = h.y;
+      lo[e] = l.x, lo[e + 1] = l.y;
     }
     out[0] = __builtin_bit_cast(u32x4_t, hi);
     out[1] = __builtin_bit_cast(u32x4_t, lo);
@@ -470,8 +477,10 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   const uint64_t rest = uint64_t(c->rows) * c->kv_heads * p.hz;
   const uint64_t shared = (uint64_t(c->rows) * gq / p.ht + groups) * c->kv_heads;
   if (shared > kMaxBlocks || rest > kMaxBlocks) return p;
-  split(rest, 1024, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
-  split(shared, p.ht > 16 ? 512 : 1024, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
+  split(rest, p.ht > 16 ? 512 : 1024, (max_rest + large - 1) / large, max_rest, &p.rest_splits, &p.rest_chunk);
+  // (two workgroups of k_prefix_many a CU, 512 at once, some of them the rests': `shared` counts a tile a group too many)
+  const uint64_t likely = std::max<uint64_t>((uint64_t(c->rows) * gq + p.ht - 1) / p.ht, groups) * c->kv_heads;
+  split(p.ht > 16 ? likely : shared, p.ht > 16 ? 448 : 1024, 1, max_prefix, &p.prefix_splits, &p.prefix_chunk);
   p.rest_blocks = rest * p.rest_splits;
   p.prefix_blocks = max_prefix == 0 || groups == 0 ? 0 : shared * p.prefix_splits;
   if (p.rest_blocks + p.prefix_blocks > kMaxItems / 256) return p;
