@@ -777,16 +777,20 @@ PromptPlan prompt_plan(const chpe_delta_states* s, uint32_t tokens, uint32_t row
 
 // Rows of up to this many tokens run token by token, each state read and written once for all of them, and no launch
 // knows the rows' lengths: where there are several rows both kinds are launched and leave the other's rows alone.
-constexpr uint32_t kShort = 8;
+// A token costs the one kind some 2 us beside the states' bytes, a chunk is the same work for the other however few tokens
+// it has (9B layout, f32 / bf16, us: one row in chunks 24 / 21, of 8 tokens token by token 23 / 23, of 16 38 / 40; 8 rows 55 / 41
+// in chunks, of 16 tokens 48 / 50; 16 rows 88 / 63, of 16 62 / 61, of 24 86 / 85; 32 rows 150 / 105, of 8 68 / 65; 64 rows
+// 297 / 201, of 16 180 / 184).
+uint32_t short_rows(uint32_t rows, uint32_t v_heads) { return uint64_t(rows) * v_heads >= 512 ? 16 : 8; }
 
 template <int D, class T>
 bool launch_prompt(const PromptArgs& a, const PromptPlan& p, hipStream_t st) {
   const uint64_t items = (uint64_t(a.d.r.rows) * a.d.NV + 7) / 8 * 8;
   if (a.d.r.tokens != 0 && !launch(&k_delta_prep<D, T>, p.chunks, 256, st, a)) return false;
   // Columns of a workgroup: 16, so that few rows reach all CUs; where head dim 128 gives more workgroups than those, 32 (one
-  // row of 1000 tokens of the 9B layout in f32 84 us with 16, 100 with 32; four rows 305 and 234; bf16 53 / 66 and
-  // 141 / 137; at head dim 64 16 is ahead or within 7 % throughout), and 64 for many bf16 rows, where LDS holds
-  // that (8 rows 270 us with 32, 247 with 64; 6 rows 199 and 230).
+  // row of 1000 tokens of the 9B layout in f32 79 us with 16, 91 with 32; four rows 279 and 207; bf16 49 / 61 and
+  // 160 / 128; at head dim 64 16 is ahead or within 11 % throughout), and 64 for many bf16 rows, where LDS holds
+  // that (8 rows 247 us with 32, 233 with 64; 6 rows 182 and 210).
   const uint64_t many = uint64_t(a.d.r.rows) * a.d.NV;
   bool ok;
   if constexpr (D == 128 && __is_same(T, Bf16)) {
@@ -832,9 +836,10 @@ extern "C" int chpe_delta_prompt(const chpe_delta_states* states, const chpe_del
   if (workspace_bytes < p.bytes) return -2;
   a.chunks = static_cast<float*>(workspace);
   a.o32 = t->z ? a.chunks + p.off_o / 4 : nullptr;
-  const bool some_short = rows > 1 || tokens <= kShort, some_long = tokens > kShort;
-  a.shortest = some_short ? kShort + 1 : 0;
-  if (some_short && !launch_delta_tokens(a.d, states->head_dim, t->type, kShort, st)) return -3;
+  const uint32_t few = short_rows(rows, states->v_heads);
+  const bool some_short = rows > 1 || tokens <= few, some_long = tokens > few;
+  a.shortest = some_short ? few + 1 : 0;
+  if (some_short && !launch_delta_tokens(a.d, states->head_dim, t->type, few, st)) return -3;
   if (!some_long) return 0;
   return (states->head_dim == 128 ? launch_prompt<128>(a, p, t->type, st) : launch_prompt<64>(a, p, t->type, st)) ? 0 : -3;
 }

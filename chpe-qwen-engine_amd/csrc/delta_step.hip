@@ -10,8 +10,8 @@ using namespace dev;
 // A workgroup takes one value head of one row: its threads hold the state, 4 columns of D / 16 or D / 8 rows each (16 or 8
 // groups of rows), 16 bytes a lane, read once and written once.  The column sums (S^T k before the update, S^T q after it) meet
 // over the groups of a wave, then over the waves in LDS, in a fixed order.
-// Bound by memory: 2 x 64 KB a head of 128 (256 rows of the 9B layout, 1.08 GB: 195 us, 5.5 TB/s; one row, 4 MB: 5 us, two
-// memory latencies and the sums).  ONE: a token per row, with nothing to load ahead; else rows of up to `longest`, the
+// Bound by memory: 2 x 64 KB a head of 128 (256 rows of the 9B layout, 1.08 GB: 189 us, 5.7 TB/s; 33 rows, 141 MB: 25 us; one
+// row, 4 MB: 6.5 us, the latencies of the slot's number, the state and the sums).  ONE: a token per row, with nothing to load ahead; else rows of up to `longest`, the
 // next token's inputs on the way meanwhile.  (16 groups for one token at D = 128: 256 rows take 207 us with 8; 8 for
 // more: 32 rows of 5 tokens take 54 us with 16, 46 with 8.)
 template <int D, bool ONE>

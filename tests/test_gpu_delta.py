@@ -201,6 +201,19 @@ def test_prompt_columns(dtype, rows):
         L.check(int(starts[r]), int(starts[r + 1]), out, state[r], before(old, r), r)
 
 
+@pytest.mark.parametrize("NK,NV,hd,dtype", [(16, 32, 128, "f32"), (16, 32, 128, "bf16"), (8, 64, 64, "f16"), (2, 4, 64, "f32")])
+def test_prompt_of_short_rows(NK, NV, hd, dtype):
+    """Lengths about those from which on a row runs in chunks, in few rows and in many."""
+    for lens in ([8, 9, 16, 17, 1, 0, 7, 15, 18, 64, 65, 8, 16, 17, 2, 9], [17, 8], [9], [8], [16]):
+        starts = np.concatenate([[0], np.cumsum(lens)])
+        L = Layer(int(starts[-1]), NK, NV, hd, dtype, True, seed=len(lens))
+        _, state = pool(len(lens), NV, hd, 5)
+        old = state.clone()
+        out = ca.DeltaStates(state, NK).prompt(*L.args(), dev(starts), dev(np.arange(len(lens))), **L.kw())
+        for r, n in enumerate(lens):
+            L.check(starts[r], starts[r + 1], out, state[r], before(old, r), (lens, r))
+
+
 def test_prompt_in_pieces_and_again():
     """A prompt in one call, in two, and the same call again: the last bit for bit, the pieces within the roundings."""
     NK, NV, hd, n = 4, 8, 128, 150
