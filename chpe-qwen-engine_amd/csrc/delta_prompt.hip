@@ -170,6 +170,9 @@ __device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e30f; }
 // (I + A)^-1: the four 16 x 16 blocks on the diagonal by substitution, a column a lane; then row i from the right,
 // T_ij = -(sum_(j < k <= i) T_ik A_kj) T_jj, in a wave's registers.  |k| <= 1 and b < 1 keep T's elements within products
 // of contractions; a series in powers of A would not stay there.
+// Bound by its chain of steps (three workgroups a CU overlap theirs) and by the 38 KB of operands that it leaves: 128 chunks
+// of 32 heads in f32, 155 MB, 95 us; with bf16 keys, one product where f32 takes six, 8 chunks 11.2 us.  T and o's matrix
+// as f32 would be two thirds of the bytes, but each of the scan's workgroups would take them apart in its chain, which was slower.
 template <int D, class T>
 __global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
@@ -375,6 +378,10 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
 // form the outputs of 16 tokens each: Q S in 2., o in 3.  Everybody loads its own operands of the next chunk where the
 // others leave it time.  (Rows behind the end are the last token again: b, and so u, is 0 there.)
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
+// Bound, for few rows, by the chain of a chunk's three steps, each a wait on LDS, a run of dependent products and a barrier: 3.6 us a
+// chunk of f32 keys (8189 tokens of 32 heads on 256 workgroups, 460 us; with four waves for everything 6.5),
+// 2.7 of bf16; for many rows by the 38 KB a chunk and head that every column block reads (24 bf16 prompts of 49 thousand
+// tokens together, 64 columns a workgroup: 1.04 ms) at the 27 bytes a cycle that a CU takes in.
 template <int D, class T, int NT>
 __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
@@ -721,7 +728,8 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
         st_once(a.state + uint64_t(to) * a.slot_stride + (size_t(h) * D + dim(r, u)) * D + c0 + 16 * ct + n, S[u][ct][r]);
 }
 
-// ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per 16 tokens of a (chunk, value head), 4 dims a lane ------
+// ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per 16 tokens of a (chunk, value head), 4 dims a lane.  Its f32
+// outputs come from the scan's stores, mostly out of the caches (501 tokens of 32 heads of 128, 16 MB: 5.1 us, a launch's time) ------
 constexpr int kNormTokens = 16;
 template <int D, class T>
 __global__ void __launch_bounds__(256) k_delta_gnorm(PromptArgs pa) {

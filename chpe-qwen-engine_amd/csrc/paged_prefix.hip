@@ -151,7 +151,9 @@ struct PartArgs : PrefixArgs {
 // k_paged_16 reads each K and V row once per 16 queries, and every lane pair forms a score's weight twice: 64 rows of 8
 // query heads behind 8192 fp16 slots took 116 us there (1.1 GB through the CUs' caches at 27 bytes a cycle each, 65 us, and
 // 50 us of vector instructions).
-// Bound by the vector instructions of the softmax.
+// Now 57 us, 0.6 PFLOP/s with the queries' and weights' two parts.  Two workgroups a CU; for 32 slots of one a SIMD's matrix cores
+// are busy 1024 cycles and its vector ALU about 1000 (softmax, parts, addresses), which the two overlap in part: 1800 cycles.
+// A workgroup's own start (group, page numbers, K, V and queries behind each other) and end are 8 us.
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 template <class T>
@@ -389,7 +391,8 @@ __global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
   }
 }
 
-// ---- the join: a workgroup per (row, query head), 256 / (HD / 4) parts at a time ----------------------------------
+// ---- the join: a workgroup per (row, query head), 256 / (HD / 4) parts at a time.  Bound by latency for few rows (5 rows
+// 3.2 us), by the parts' bytes for many (64 rows of 64 heads of 128, 14 parts each, 30 MB: 9.8 us) ---------------------------------
 template <int HD>
 __global__ void __launch_bounds__(256) k_prefix_join(PrefixArgs a) {
   constexpr int D4 = HD / 4, GR = 256 / D4;
@@ -467,7 +470,7 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   const bool many = gq > 8 || (max_prefix != 0 && groups != 0 && uint64_t(c->rows) * gq > 8 * uint64_t(groups));
   p.ht = c->type == 0 || (many && c->head_dim <= kWaveDims) ? 16 : 8;
   // ... and k_prefix_many where they have more than a few, the calls are not all latency, and the rows' own slots, for which it
-  // has most of its columns idle, do not count: behind 4096 slots with 64 of their own 64 rows of the 72B layout take 53 us
+  // has most of its columns idle, do not count: behind 4096 slots with 64 of their own 64 rows of the 72B layout took 53 us
   // there and 74 in k_paged_16, 4 rows 17 and 20; 8 rows of the 9B layout (32 queries) 20 and 18; 64 rows behind 1000 slots
   // with up to 1000 of their own 82 and 69; 8 groups of 6 rows of 6 queries 31 and 21.
   if (c->type != 0 && groups != 0 && uint64_t(c->rows) * gq >= 24 * uint64_t(groups) &&
