@@ -35,6 +35,28 @@ struct PromptArgs {
   __device__ bool range(uint32_t row, uint32_t* lo, uint32_t* hi) const {
     return d.r.range(row, lo, hi) && *hi - *lo >= shortest;
   }
+  // The n-th longest of up to 64 rows that are theirs, -1 behind the last (of more rows: row n; of equal ones in their order):
+  // workgroups start in order, and where they are several rounds a long row that starts late ends alone (24 rows of 1 to 4097
+  // tokens in random orders: the scan 1.04 to 1.2 ms as they come, 1.0 so).
+  __device__ int nth_longest(uint32_t n, uint32_t lane) const {
+    if (d.r.rows > 64) return int(n);
+    uint32_t lo = 0, hi = 0, rank = 0;
+    const bool there = lane < d.r.rows && range(lane, &lo, &hi);
+    const uint64_t all = __ballot(there);
+    if (n >= uint32_t(__builtin_popcountll(all))) return -1;
+    const uint32_t len = hi - lo;
+    for (uint64_t left = all; left != 0; left &= left - 1) {
+      const uint32_t j = uint32_t(__builtin_ctzll(left)), other = lane_of(len, int(j));
+      rank += other > len || (other == len && j < lane) ? 1u : 0u;
+    }
+    return int(__builtin_ctzll(__ballot(there && rank == n)));
+  }
+  // the x-th of a row's value heads in workgroups' order: those of one key head on one XCD (workgroup i runs on XCD i % 8), whose
+  // L2 they share (with two value heads a key head 8189 tokens in f32 fetch 151 and 424 MB in the two launches instead of 286 and 558)
+  __device__ uint32_t head_of(uint32_t x) const {
+    const uint32_t r = d.NV / d.NK;
+    return d.NK % 8 != 0 ? x : (x % 8 + 8 * (x / (8 * r))) * r + x / 8 % r;
+  }
 };
 
 // ---- products in 32 bits on the 16-bit matrix cores ---------------------------------------------------------
@@ -186,14 +208,14 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
   auto s_A = reinterpret_cast<float(*)[AS]>(s_mem);
   auto s_diag = reinterpret_cast<float(*)[16][20]>(s_mem + kBytesA);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
-  const uint32_t h = blockIdx.x % a.NV, b = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
+  const uint32_t h = pa.head_of(blockIdx.x % a.NV), b = blockIdx.x / a.NV, kh = h / (a.NV / a.NK);
   const int row = a.r.row_of(b, kChunkShift, lane);
   uint32_t lo, hi;
   if (row < 0 || !pa.range(row, &lo, &hi)) return;
   const uint32_t t0 = lo + (b - a.r.first_block(row, lo, kChunkShift)) * kChunk;
   if (t0 >= hi) return;
   const uint32_t nt = min(hi - t0, uint32_t(kChunk)), mine = 16 * wave + n;
-  float* out = pa.chunks + size_t(blockIdx.x) * kChunkFloats;
+  float* out = pa.chunks + (size_t(b) * a.NV + h) * kChunkFloats;
   Row16<D, T> kr, qr;
   if (mine < nt) {
     kr.load(static_cast<const T*>(a.k) + (t0 + mine) * a.k_stride + kh * D, G);
@@ -380,8 +402,8 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
 // Bound, for few rows, by the chain of a chunk's three steps, each a wait on LDS, a run of dependent products and a barrier: 3.6 us a
 // chunk of f32 keys (8189 tokens of 32 heads on 256 workgroups, 460 us; with four waves for everything 6.5),
-// 2.7 of bf16; for many rows by the 38 KB a chunk and head that every column block reads (24 bf16 prompts of 49 thousand
-// tokens together, 64 columns a workgroup: 1.04 ms) at the 27 bytes a cycle that a CU takes in.
+// 2.7 of bf16; with 64 columns of bf16, where a CU's LDS holds one workgroup, 5.4 (24 prompts of 49 thousand tokens
+// together, 192 such chunks a CU: 1.04 ms, 0.6 PFLOP/s of parts' products).
 template <int D, class T, int NT>
 __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
@@ -398,10 +420,11 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
   // the column blocks of a head on one XCD (workgroup i runs on XCD i % 8), whose L2 they share
   const uint32_t item = blockIdx.x / (8 * CB) * 8 + blockIdx.x % 8, c0 = blockIdx.x / 8 % CB * (16 * NT);
   if (item >= a.r.rows * a.NV) return;
-  const uint32_t h = item % a.NV, row = item / a.NV, kh = h / (a.NV / a.NK);
+  const int nth = gridDim.x > 256 ? pa.nth_longest(item / a.NV, lane) : int(item / a.NV);
   uint32_t lo, hi;
   float fill;
-  if (!pa.range(row, &lo, &hi)) return;
+  if (nth < 0 || !pa.range(uint32_t(nth), &lo, &hi)) return;
+  const uint32_t row = uniform(uint32_t(nth)), h = pa.head_of(item % a.NV), kh = h / (a.NV / a.NK);
   const int slot = a.r.before(row, &fill), to = a.r.after(row);
   // the wave's rows of the state: those of its two (D = 64: of its one) operands' elements
   auto dim = [&](int r, int u) { return RT == 2 ? Row16<D, T>::dim(G, wave, u, r) : Row16<D, T>::dim(G, wave >> 1, wave & 1, r); };

@@ -214,6 +214,19 @@ def test_prompt_of_short_rows(NK, NV, hd, dtype):
             L.check(starts[r], starts[r + 1], out, state[r], before(old, r), (lens, r))
 
 
+@pytest.mark.parametrize("rows", [64, 69])
+def test_prompt_of_many_rows(rows):
+    """As many rows as are taken by their lengths, and more."""
+    lens = ([20, 3, 70, 64, 0, 129] * 12)[:rows]
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    L = Layer(int(starts[-1]), 8, 16, 64, "bf16", False, seed=rows)
+    _, state = pool(rows, 16, 64, 5)
+    old = state.clone()
+    out = ca.DeltaStates(state, 8).prompt(*L.args(), dev(starts), dev(np.arange(rows)))
+    for r in range(rows):
+        L.check(starts[r], starts[r + 1], out, state[r], before(old, r), r)
+
+
 def test_prompt_in_pieces_and_again():
     """A prompt in one call, in two, and the same call again: the last bit for bit, the pieces within the roundings."""
     NK, NV, hd, n = 4, 8, 128, 150
