@@ -24,8 +24,8 @@ struct ConvArgs {
 // A wave takes 64 x 16 bytes of channels (V of them a lane) of a block of 8 tokens of one row; the taps slide through
 // registers.  A row's first block reads the state before and writes the one after (whose inputs are x and the state
 // before), so that both may be the same slot.
-// Bound by memory: every input is read once, and by the next block's taps (8196 bf16 tokens of 8192 channels, 314 MB:
-// 53 us, 6.0 TB/s; with 16 tokens 54, with 32 and a slower SiLU 90 instead of 78).
+// Bound by memory: every input is read once, and by the next block's taps (8196 bf16 tokens of 8192 channels, 316 MB so:
+// 53 us, 6.0 TB/s, on inputs that change from call to call 58; with 16 tokens 54, with 32 and a slower SiLU 90 instead of 78).
 template <class T, int TAPS>
 __global__ void __launch_bounds__(kConvThreads) k_delta_conv(ConvArgs a) {
   constexpr int V = 16 / sizeof(T), P = TAPS - 1;

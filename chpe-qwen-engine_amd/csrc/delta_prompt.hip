@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(256, 3) k_delta_prep(PromptArgs pa) {
 // Keys as operands of k u^T have tokens inside: the transposing reads of LDS give them so.
 // Bound, for few rows, by the chain of a chunk's three steps, each a wait on LDS, a run of dependent products and a barrier: 3.6 us a
 // chunk of f32 keys (8189 tokens of 32 heads on 256 workgroups, 460 us; with four waves for everything 6.5),
-// 2.7 of bf16; with 64 columns of bf16, where a CU's LDS holds one workgroup, 5.4 (24 prompts of 49 thousand tokens
-// together, 192 such chunks a CU: 1.04 ms, 0.6 PFLOP/s of parts' products).
+// 2.7 of bf16; with 64 columns of bf16, where a CU's LDS holds one workgroup, 5.2 (24 prompts of 49 thousand tokens
+// together, 192 such chunks a CU: 1.0 ms, 0.6 PFLOP/s of parts' products).
 template <int D, class T, int NT>
 __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs pa) {
   const DeltaArgs& a = pa.d;
