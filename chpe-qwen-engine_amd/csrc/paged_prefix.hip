@@ -75,7 +75,8 @@ struct PrefixArgs {
 
 // The parts.  A workgroup's queries are HT of the query heads of one kv head, row by row: of all rows of a group for a split
 // of its prefix (blocks up to prefix_blocks), of one row for a split of its own slots.  A launch does not know the
-// groups' sizes: group g's tiles of queries have the numbers from (its first row) * gq / HT + g on.
+// groups' sizes: group g's tiles of queries have the numbers from (its first row) * gq / HT + g on (a first row behind the rows
+// counts as the one behind the last: its number lies above those of all rows, and none passes 32 bits).
 struct PartArgs : PrefixArgs {
   __device__ void at(const Place& p, uint32_t i, uint32_t* row, uint32_t* head) const {
     const uint32_t gq = H / c.KV, x = p.h0 + min(i, p.nh - 1);
@@ -105,7 +106,7 @@ struct PartArgs : PrefixArgs {
       b /= prefix_splits;
       p.kvh = b % c.KV;
       b /= c.KV;
-      auto first = [&](uint32_t r, uint32_t g) { return uint32_t(uint64_t(r) * gq / HT) + g; };
+      auto first = [&](uint32_t r, uint32_t g) { return uint32_t(uint64_t(min(r, rows)) * gq / HT) + g; };
       const int g = last_group(b, first);
       uint32_t r0 = 0, r1 = 0, prefix = 0;
       const bool there = g >= 0 && group(g, &r0, &r1, &prefix);
