@@ -61,7 +61,10 @@ struct PrefixArgs {
     bool ok = true;
     if (g >= 0) {
       ok = group(g, &r0, &r1, &prefix);
-      if (ok && row >= r1) prefix = 0;
+      if (int(r0) <= int(r1) && int(r1) <= int(row)) {  // (behind the group, whatever else it holds: in none)
+        ok = true;
+        prefix = 0;
+      }
     }
     const uint32_t len = uint32_t(gld(lens + row));
     *r = Row{(prefix + prefix_chunk - 1) / prefix_chunk, prefix, len, rest_chunk, row};

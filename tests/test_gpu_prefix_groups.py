@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_paged import TYPES
 from test_gpu_prefix import Groups, dev, queries
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,34 @@ def test_groups_that_start_behind_the_rows(H, hd, dtype, tile, more):
         out = run(g, q, groups, [prefix, 0, 0])
         assert nan_rows(out) == bad, groups
         g.check(q, out, rows=[r for r in range(8) if r not in bad])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("H", [4, 40])  # few queries a group, many
+def test_rows_behind_a_group_that_is_not_valid(H, dtype):
+    """A row in no group has no prefix, whatever the last group ahead of it holds."""
+    g = Groups([(100, [101, 140, 100]), (100, [120, 130]), (None, [40, 0, 35])], 2, 64, 16, dtype, seed=H)
+    q = queries(8, H, 64)
+    want = run(g, q, [0, 3, 5], [100, 100])
+    g.check(q, want)
+    for prefixes, bad in (([100, 101], [3, 4]), ([100, -1], [3, 4]), ([-5, 2 ** 31 - 1], [0, 1, 2, 3, 4])):
+        out = run(g, q, [0, 3, 5], prefixes)
+        assert nan_rows(out) == bad, prefixes
+        g.check(q, out, rows=[r for r in range(8) if r not in bad])
+    for groups in ([-2, 5], [-7, -2]):  # (rows 0 to 4 in a group that is not valid; in none, but longer than max_rest)
+        out = run(g, q, groups, [100])
+        assert nan_rows(out) == [0, 1, 2, 3, 4], groups
+        g.check(q, out, rows=[5, 6, 7])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("H", [4, 40])
+def test_empty_groups_pad_a_table(H, dtype):
+    """A table of a fixed number of groups, the last ones empty, whatever their prefixes' lengths are."""
+    g = Groups([(100, [101, 140, 100, 120, 130]), (None, [40, 0, 35])], 2, 64, 16, dtype, seed=H + 1)
+    q = queries(8, H, 64)
+    for pad in (0, -1, 101, 2 ** 31 - 1, 50):
+        for groups, prefixes in (([0, 5, 5, 5], [100, pad, pad]), ([0, 5, 5, 8, 8], [100, pad, 0, pad]), ([0, 0, 5], [pad, 100])):
+            out = run(g, q, groups, prefixes)
+            assert nan_rows(out) == [], (groups, prefixes)
+            g.check(q, out)
