@@ -93,6 +93,25 @@ __device__ __forceinline__ float sum_parts(float v) {
   return pair_sum(v, 8);
 }
 
+// A weight's exponent is x mult - base, base the largest product x mult so far, rounded: the product again inside the fma, so
+// that it is rounded once, as small as the difference is.  The largest one's own exponent is then what its rounding
+// lost, which from 2^22 on is 1 / 4 and more, and past 2^25 would take fp16 parts out of their range and soon leave no
+// weight at all.  Where the base is that large the rounded product counts, 0 for the largest whatever its size: x
+// becomes the exponent itself, to be taken times 1.
+constexpr float kFarScore = 4194304.0f;
+template <int N>
+__device__ __forceinline__ void far_scores(float (&x)[N], float& mult, float& base) {
+  if (!(fabsf(base) >= kFarScore)) return;  // (a column's own: its bits do not depend on the others)
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    x[e] *= mult;
+    asm("" : "+v"(x[e]));  // (not the fma again)
+    x[e] -= base;
+  }
+  mult = 1.0f;
+  base = 0.0f;
+}
+
 // The tile's row offsets (bytes from k or v): lane r of the wave finds row r's page and leaves the
 // offset in LDS for the lanes that load the row.  `next` requests the table entry ahead of its use; for the
 // first tile of a range that starts at slot 0 it does not wait for the row's length (entries behind it may
@@ -375,17 +394,19 @@ __global__ void __launch_bounds__(kWaves * 64, NT == 1 ? (HD == 64 ? 4 : 3) : (H
         }
       }
       mx = pair_max(pair_max(mx, 16), 32);
-      const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m[ht] - base);
+      float base = mx == -INFINITY ? 0.0f : mx;
+      const float f = __builtin_amdgcn_exp2f(m[ht] - base);
       if (__ballot(f != 1.0f) != 0) {
         l[ht] *= f;
 #pragma unroll
         for (int j = 0; j < VD; ++j) o[ht][j] *= f;
       }
       m[ht] = mx;
+      float mu = mult[ht];
+      far_scores(s8, mu, base);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // (the product again inside the fma: rounded once, as small as the difference is)
-        s8[e] = __builtin_amdgcn_exp2f(top[e] > -INFINITY ? fmaf(s8[e], mult[ht], -base) : top[e]);
+        s8[e] = __builtin_amdgcn_exp2f(top[e] > -INFINITY ? fmaf(s8[e], mu, -base) : top[e]);
         l[ht] += s8[e];
         s8[e] *= float(1 << P::kScaleExp);
       }
@@ -527,16 +548,21 @@ __global__ void __launch_bounds__(kWaves * 64, HD == 64 ? 4 : 3) k_paged_32(Args
             make_float4(top[0], top[1], top[2], top[3]);
     }
     mx = pair_max(pair_max(mx, 16), 32);
-    const float base = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - base);
+    float base = mx == -INFINITY ? 0.0f : mx;
+    const float f = __builtin_amdgcn_exp2f(m - base);
     if (__ballot(f != 1.0f) != 0) {
       l *= f;
 #pragma unroll
       for (int j = 0; j < VD; ++j) o[j] *= f;
     }
     m = mx;
+    float mu = mult;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s4[i] = sc[i];
+    far_scores(s4, mu, base);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s4[i] = __builtin_amdgcn_exp2f(top[i] > -INFINITY ? fmaf(sc[i], mult, -base) : top[i]);
+      s4[i] = __builtin_amdgcn_exp2f(top[i] > -INFINITY ? fmaf(s4[i], mu, -base) : top[i]);
       l += s4[i];
     }
 #pragma unroll

@@ -345,10 +345,12 @@ __global__ void __launch_bounds__(256, 2) k_prefix_many(PartArgs a) {
           for (int j = 0; j < VD; ++j) o[qt][j] *= f;
         }
         m[qt] = mx;
-        const float less = mx == -INFINITY ? 0.0f : float(P::kScaleExp) - mx;
+        float mu = mult[qt], base = mx == -INFINITY ? 0.0f : mx;
+        far_scores(x, mu, base);
+        const float less = float(P::kScaleExp) - base;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], mult[qt], less));
+          x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], mu, less));
           l[qt] += x[e];
         }
         P::split(x, pf[qt]);
