@@ -182,9 +182,14 @@ struct Raw<float> {
   static __device__ float value(float b) { return b; }
 };
 
-// Keys and queries whose squares leave this range, and gates that are NaN, make a chunk run token by token: the
-// products above take keys before their norm, and 0 times what is not finite would reach earlier tokens.
-__device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e30f; }
+// Keys and queries longer than 1e8, values from 1e20 on, states from 1e25 on, and gates that are NaN, make a chunk run token by
+// token: the products above take keys before their norm, and 0 times what is not finite would reach earlier tokens.  Within
+// these bounds a product of a key and a state stays below 1e8 sqrt(128) 1.5e25, a thousandth of f32's range over the 1e3 that a
+// row behind the end multiplies it by.  (In such chunks a state's columns grow by 1e20 sqrt(tokens) at most, 5e24 in 2^31 of them.)
+__device__ __forceinline__ bool in_range(float sum2) { return sum2 <= 1e16f; }
+__device__ __forceinline__ bool value_in_range(float v) { return fabsf(v) < 1e20f; }
+// (what is infinite or NaN in a state stays in its column either way)
+__device__ __forceinline__ bool state_in_range(float s) { return !(fabsf(s) >= 1e25f && fabsf(s) < INFINITY); }
 
 // ---- T and o's matrix of a chunk --------------------------------------------------------------------------------
 // A workgroup per (chunk, value head); wave w forms o's row w (16 tokens) and A's row 3 - w, as many products for each.
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
   __shared__ u32x4_t s_x[NT][2][3][64], s_u[NT][2][3][64], s_us[NT][2][3][64];
   __shared__ __align__(16) float s_scale[2][256];
   __shared__ float s_red[2][4], s_col[2][4][16 * NT];
-  __shared__ int s_bad[2];
+  __shared__ __align__(16) uint32_t s_bad[2][4];  // of each wave that carries the state
   const int wave8 = uniform(threadIdx.x >> 6), wave = wave8 & 3, lane = threadIdx.x & 63, G = lane >> 4, n = lane & 15;
   const bool carry = wave8 < 4;  // (uniform)
   // the column blocks of a head on one XCD (workgroup i runs on XCD i % 8), whose L2 they share
@@ -438,6 +443,21 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
         for (int r = 0; r < 4; ++r)
           S[u][ct][r] = slot >= 0 ? gld(a.state + uint64_t(slot) * a.slot_stride + (size_t(h) * D + dim(r, u)) * D + c0 + 16 * ct + n) : fill;
   }
+  auto is_bad = [&](int turn) {
+    const uint4 b = *reinterpret_cast<const uint4*>(s_bad[turn]);
+    return (b.x | b.y | b.z | b.w) != 0;
+  };
+  // has chunk `turn` run token by token if S is out of range
+  auto look_at_s = [&](int turn) {
+    bool large = false;
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) large |= !state_in_range(S[u][ct][r]);
+    if (__ballot(large) != 0 && lane == 0) s_bad[turn][wave] = 1;
+  };
   // leaves S as operands
   auto leave_s = [&] {
 #pragma unroll
@@ -604,7 +624,6 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
   };
   Row16<D, T> x16;
   u32x4_t m16[2][3];
-  if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
   int turn = 0;
   if (!carry) {
     f4_t f16;
@@ -642,7 +661,7 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
       store();
       lds_barrier();
       const float g = s_scale[turn][64 + 16 * wave + n];
-      if (s_bad[turn] != 0) {  // (the same for all)
+      if (is_bad(turn)) {  // (the same for all)
         for (uint32_t i = 3 * min(hi - t0, uint32_t(kChunk)); i != 0; --i) lds_barrier();
         from = hi;
       } else {
@@ -665,6 +684,8 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
     load_v(lo);
     load_m(m16, lo, 0);
   }
+  if (lane < 2) s_bad[lane][wave] = 0;
+  look_at_s(0);
   leave_s();
   lds_barrier();
   for (uint32_t t0 = lo; t0 < hi; t0 += kChunk, turn ^= 1) {
@@ -684,22 +705,23 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         v[ct][r] = Raw<T>::value(v16[ct][r]);
-        bad |= !(fabsf(v[ct][r]) < 1e38f);
+        bad |= !value_in_range(v[ct][r]);
       }
-    if (__ballot(bad) != 0 && lane == 0) s_bad[turn] = 1;
+    if (__ballot(bad) != 0 && lane == 0) s_bad[turn][wave] = 1;
     times_s(xf, y, std::false_type{});
     const float* scale = s_scale[turn] + 16 * wave + 4 * G;
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) leave_u(s_x[ct], v[ct] - *reinterpret_cast<const f4_t*>(scale) * y[ct]);
     lds_barrier();
-    if (s_bad[turn] != 0) {  // (the same for all)
+    if (is_bad(turn)) {  // (the same for all)
       tokens(t0, min(hi, t0 + kChunk));
+      look_at_s(turn ^ 1);
       leave_s();
       load_x(x16, a.k, a.k_stride, next);
       load_v(next);
       load_m(m16, next, 0);
       lds_barrier();
-      if (wave == 0 && lane == 0) s_bad[turn] = 0;  // (set again two chunks later)
+      if (lane == 0) s_bad[turn][wave] = 0;
       continue;
     }
     // 2.
