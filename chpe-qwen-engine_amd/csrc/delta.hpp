@@ -145,9 +145,11 @@ __device__ __forceinline__ void st_row(T* p, const float (&x)[N]) {
   }
 }
 
-// x / (1 + e^-x), off by at most 8 u, u = 2^-24: e^-x as 2^t (2 u) times 1 + what the product t lost (2 u), the sum 1 u,
-// the reciprocal 2 u, the product 1 u.  With expf and a division the convolution was bound by them: 78 us instead of 54 for
-// 67 million bf16 values.  (Beyond 200 e^-x is 0 or infinite either way.)
+// x / (1 + e^-x), off by at most 8 u of itself from x = -87 on, u = 2^-24: e^-x as 2^t (2 u) times 1 + what the product t lost
+// (2 u), the sum 1 u, the reciprocal 2 u, the product 1 u.  Below, the reciprocal is no normal number and may come out as 0,
+// and so may the result: off by 87 e^-87 = 1.4e-36 at most.  (x / (1 + expf(-x)) loses e^-x from -88.7 on, too.)  With expf and
+// a division the convolution was bound by them: 78 us instead of 54 for 67 million bf16 values.  (Beyond 200 e^-x is 0 or
+// infinite either way.)
 __device__ __forceinline__ float delta_silu(float x) {
   const float y = __builtin_amdgcn_fmed3f(x, -200.0f, 200.0f), t = y * -1.44269502f;  // log2 e rounded, and the rest of it
   const float lost = fmaf(y, -1.92596303e-8f, fmaf(y, -1.44269502f, -t));
