@@ -774,7 +774,8 @@ __global__ void __launch_bounds__(512, D == 64 ? 4 : 2) k_delta_scan(PromptArgs 
 }
 
 // ---- the gated norm: w * o / rms(o) * silu(z), a workgroup per 16 tokens of a (chunk, value head), 4 dims a lane.  Its f32
-// outputs come from the scan's stores, mostly out of the caches (501 tokens of 32 heads of 128, 16 MB: 5.1 us, a launch's time) ------
+// outputs come from the scan's stores, of few tokens mostly out of the caches (501 tokens of 32 heads of 128, 16 MB: 5.1 us, a
+// launch's time; 49 thousand, 1.6 GB: 279 us, 5.8 TB/s) -----------------------------------------------------------------------------
 constexpr int kNormTokens = 16;
 template <int D, class T>
 __global__ void __launch_bounds__(256) k_delta_gnorm(PromptArgs pa) {

@@ -155,7 +155,7 @@ struct PartArgs : PrefixArgs {
 // k_paged_16 reads each K and V row once per 16 queries, and every lane pair forms a score's weight twice: 64 rows of 8
 // query heads behind 8192 fp16 slots took 116 us there (1.1 GB through the CUs' caches at 27 bytes a cycle each, 65 us, and
 // 50 us of vector instructions).
-// Now 57 us, 0.6 PFLOP/s with the queries' and weights' two parts.  Two workgroups a CU; for 32 slots of one a SIMD's matrix cores
+// Now 57 us, 0.6 PFLOP/s with the queries' and weights' two parts (bf16, three: 74).  Two workgroups a CU; for 32 slots of one a SIMD's matrix cores
 // are busy 1024 cycles and its vector ALU about 1000 (softmax, parts, addresses), which the two overlap in part: 1800 cycles.
 // A workgroup's own start (group, page numbers, K, V and queries behind each other) and end are 8 us.
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
@@ -478,7 +478,8 @@ PrefixPlan prefix_plan(const chpe_kv_pages* c, uint32_t heads, uint32_t groups, 
   // ... and k_prefix_many where they have more than a few, the calls are not all latency, and the rows' own slots, for which it
   // has most of its columns idle, do not count: behind 4096 slots with 64 of their own 64 rows of the 72B layout took 53 us
   // there and 74 in k_paged_16, 4 rows 17 and 20; 8 rows of the 9B layout (32 queries) 20 and 18; 64 rows behind 1000 slots
-  // with up to 1000 of their own 82 and 69; 8 groups of 6 rows of 6 queries 31 and 21.
+  // with up to 1000 of their own 82 and 69; 8 groups of 6 rows of 6 queries 31 and 21.  (f32 caches: k_paged_32 always, 16
+  // queries a workgroup; 64 rows of the 72B layout behind 8192 slots 245 us, 110 of them at the f32 matrix cores' rate.)
   if (c->type != 0 && groups != 0 && uint64_t(c->rows) * gq >= 24 * uint64_t(groups) &&
       uint64_t(c->rows) * heads >= 256 && max_prefix / 2 >= max_rest)
     p.ht = many_queries(c->head_dim);

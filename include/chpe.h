@@ -285,7 +285,8 @@ size_t chpe_paged_attention_workspace(const chpe_kv_pages *cache, uint32_t heads
  * prefix.  max_prefix and max_rest bound the prefixes and what rows have behind them (and size the launches).  A row of
  * length 0 gives zeros, one shorter than its prefix sees lens[r] slots of it (and is read on its own); a row of a negative
  * length or with more than max_rest slots of its own gives NaN, and so do the rows of a group whose rows or prefix are
- * out of bounds.  Everything else as chpe_paged_attention.
+ * out of bounds (they alone: groups without rows may pad the arrays, whatever their prefix_lens are).  Everything
+ * else as chpe_paged_attention without its window and its weights: a cache that is cut by weights takes that call.
  * workspace: chpe_paged_prefix_workspace bytes for the same cache, heads, groups and bounds, at a 16-byte boundary, any
  * content; calls that may overlap need one each.
  * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
@@ -357,7 +358,8 @@ int chpe_delta_step(const chpe_delta_states *states, const chpe_delta_tokens *t,
                     const int32_t *slot_out, void *stream);
 /* Any number of tokens per row: prompts, drafts.  Sums and states are f32 as in chpe_delta_step.
  * workspace: chpe_delta_prompt_workspace bytes for the same states, tokens, rows and norm (z given), at a 16-byte
- * boundary, any content; calls that may overlap need one each.
+ * boundary, any content; calls that may overlap need one each.  (37888 for each of tokens / 64 + rows chunks and v_heads
+ * heads; with the norm the outputs in f32, too.)
  * Returns 0, -1 bad arguments, -2 workspace too small, -3 device error. */
 int chpe_delta_prompt(const chpe_delta_states *states, const chpe_delta_tokens *t, uint32_t tokens, uint32_t rows,
                       const int32_t *starts, const int32_t *slot_in, const int32_t *slot_out, void *workspace,
