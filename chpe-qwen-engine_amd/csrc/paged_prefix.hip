@@ -155,7 +155,7 @@ struct PartArgs : PrefixArgs {
 // k_paged_16 reads each K and V row once per 16 queries, and every lane pair forms a score's weight twice: 64 rows of 8
 // query heads behind 8192 fp16 slots took 116 us there (1.1 GB through the CUs' caches at 27 bytes a cycle each, 65 us, and
 // 50 us of vector instructions).
-// Now 57 us, 0.6 PFLOP/s with the queries' and weights' two parts (bf16, three: 74).  Two workgroups a CU; for 32 slots of one a SIMD's matrix cores
+// Now 57 to 59 us, 0.6 PFLOP/s with the queries' and weights' two parts (bf16, three: 74).  Two workgroups a CU; for 32 slots of one a SIMD's matrix cores
 // are busy 1024 cycles and its vector ALU about 1000 (softmax, parts, addresses), which the two overlap in part: 1800 cycles.
 // A workgroup's own start (group, page numbers, K, V and queries behind each other) and end are 8 us.
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
